@@ -293,8 +293,8 @@ int prism_copy_blocks(void* dst, const void* src, int64_t rows, int64_t dst_row_
 int prism_device_copy(void* dst, const void* src, int64_t nbytes, int workgroups_per_cu, void* stream);
 
 /*
- * Paged prefill attention (chunked / prefix-hit prefill) over paged FP8
- * K/V.  Replaces
+ * Paged prefill attention (chunked / prefix-hit prefill) over paged FP8 or
+ * 16-bit K/V.  Replaces
  *   paged_prefill_attention_reference(q, k_cache, v_cache, context, *,
  *       num_heads, num_kv_heads, scale, k_scale_cache=None, v_scale_cache=None)
  *   (prism_infer/ops/paged_attention_reference.py:185-246).
@@ -302,10 +302,11 @@ int prism_device_copy(void* dst, const void* src, int64_t nbytes, int workgroups
  * q          : [total_q, num_heads, head_dim] of q_dtype (BF16/F16), strides
  *              q_strides {token, head, dim}; dim stride 1, rows 16-byte aligned.
  *              Sequence i owns rows [cu_seqlens_q[i], cu_seqlens_q[i + 1]).
- * k/v_cache  : [num_blocks, page_size, num_kv_heads, head_dim] FP8_E4M3FN,
- *              strides k_strides / v_strides {block, token, head, dim}; dim
- *              stride 1.  head_dim 128; page_size a multiple of 16; GQA group
- *              num_heads / num_kv_heads of 1, 2, 4 or 8.
+ * k/v_cache  : [num_blocks, page_size, num_kv_heads, head_dim] FP8_E4M3FN or
+ *              q_dtype, strides k_strides / v_strides {block, token, head, dim};
+ *              dim stride 1.  page_size a multiple of 16.  FP8: head_dim 128, GQA
+ *              group num_heads / num_kv_heads of 1, 2, 4 or 8.  16-bit: head_dim
+ *              64 or 128, any group, no scales, rows of out 16-byte aligned.
  * k/v_scale  : [num_blocks, page_size, num_kv_heads] fp32 or both NULL (unit
  *              scale); strides ks_strides / vs_strides.
  * block_tables, context_lens, cu_seqlens_q : int32 device arrays ([>= batch,
@@ -355,6 +356,60 @@ int prism_paged_prefill_ws(const void* q, int q_dtype, const int64_t q_strides[3
                            int num_kv_heads, int head_dim, int page_size, int num_blocks, int width,
                            float scale, int32_t* status, void* workspace, int64_t workspace_bytes, int32_t* report,
                            void* stream);
+
+/*
+ * Causal attention over packed prompts, no counterpart among the reference's
+ * own kernels (its attention layer calls an external varlen attention,
+ * prism_infer/layers/attention.py:180-208).
+ *
+ * q, k, v    : [total_q, num_heads, head_dim], [total_k, num_kv_heads,
+ *              head_dim] of dtype (BF16/F16), strides {token, head, dim}; dim
+ *              stride 1, rows 16-byte aligned.  head_dim 64 or 128; num_heads
+ *              any multiple of num_kv_heads.
+ * cu_seqlens_q, cu_seqlens_k : int32 device arrays of batch + 1 offsets (the
+ *              same array where every query has its key).  Sequence i owns query
+ *              rows [cu_seqlens_q[i], cu_seqlens_q[i + 1]) and key rows
+ *              [cu_seqlens_k[i], cu_seqlens_k[i + 1]); its queries are its last
+ *              tokens: token j sits at position klen - qlen + j and attends to
+ *              keys 0 .. that position.  Lengths of 0 are allowed.
+ * out        : [total_q, num_heads, head_dim] of dtype, 16-byte aligned rows.
+ *              Rows that see no key, and rows outside [cu_seqlens_q[0],
+ *              cu_seqlens_q[batch]), are 0.  A sequence whose offsets are out of
+ *              order or outside the tensors is left out, its rows unspecified.
+ */
+int prism_prompt_attention(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                           const void* v, const int64_t v_strides[3], int dtype, const int32_t* cu_seqlens_q,
+                           const int32_t* cu_seqlens_k, void* out, const int64_t out_strides[3], int batch, int total_q,
+                           int total_k, int num_heads, int num_kv_heads, int head_dim, float scale, void* stream);
+
+/*
+ * A step's metadata from the requests' lengths, on the device (the reference
+ * packs it on the host: prism_infer/engine/input_preparation.py:324, 571-603).
+ *
+ * block_tables : int32 [batch, width], strides bt_strides: the first
+ *              ceil(cached_lens[i] / block_size) entries of row i are the blocks
+ *              that request i holds; the rest is not read.
+ * cached_lens, query_lens : int32 [batch], stored and new tokens (0 allowed).
+ * free_blocks : int32 [num_free]; the requests take the blocks that their new
+ *              tokens need from here, in order, from entry free_start[0] on
+ *              (NULL: from 0).
+ * packed     : int32 [prism_step_metadata_words(...)], 16-byte aligned, with T =
+ *              num_tokens rounded up to 4:
+ *                [T] slot of each new token, -1 behind the last
+ *                [T] its position, 0 behind the last
+ *                [batch + 1] offsets of the requests' tokens
+ *                [batch] context lengths, cached + new
+ *                [1] their largest   [1] next free entry
+ *                [1] lowest request that does not fit, or INT32_MAX; padding to 4
+ *                [batch, width] block tables, -1 behind a request's last block
+ * A request does not fit where a length is negative, its context exceeds width *
+ * block_size, its tokens end behind num_tokens or the free blocks do not
+ * suffice: what has no block gets -1.  batch is at most 8192.
+ */
+int64_t prism_step_metadata_words(int batch, int width, int num_tokens);
+int prism_step_metadata(const int32_t* block_tables, const int64_t bt_strides[2], const int32_t* cached_lens,
+                        const int32_t* query_lens, const int32_t* free_blocks, int num_free, const int32_t* free_start,
+                        int batch, int width, int block_size, int num_tokens, int32_t* packed, void* stream);
 
 /*
  * Test hook with no counterpart in the reference: converts n fp32 values to

@@ -1,0 +1,698 @@
+// Causal attention over 16-bit keys and values: whole prompts whose K/V are
+// packed like their queries, and chunks of new tokens over a paged cache.
+//
+//   o[j, h] = sum_{t <= p} w_t v[t, h / G],  w = softmax_t(scale q[j, h] . k[t, h / G]),  p = klen - qlen + j
+//
+// for token j of a sequence of qlen queries and klen keys (its last qlen tokens
+// are the queries'); a row that sees no key (p < 0) is 0.
+//
+// Work layout.  The G query heads of a kv head share its keys, so the rows of
+// one kv head are (token, head in the group) pairs, token major: any group size
+// and any chunk length fill the columns of the MFMAs.  A workgroup owns a block
+// of kRows of these rows of one sequence and kv head, a wave 32 of them.  Tiles
+// of 64 keys go through LDS, loaded there directly.
+//
+// Per tile a wave computes S^T = K Q^T with 32x32x16 MFMAs: a row is one lane
+// column from the scores to the output, so its running max, its sum and the
+// rescaling of its accumulators are lane-local.  P^T, rounded to the cache's
+// type (weights of at most 2^8 against fp32 sums), is the B operand of O^T +=
+// V^T P^T as it stands, V^T comes from ds_read_b64_tr_b16.
+#include "common.h"
+
+#include <algorithm>
+
+namespace prism {
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kKeys = 64;              // keys per tile
+constexpr int kWaves = 4;              // per workgroup
+constexpr int kCols = 32;              // rows per wave: the columns of a 32x32 MFMA
+constexpr float kSumLimit = 256.0f;    // largest sum of a lane's 32 weights that keeps the running max
+
+// Where keys come from: packed like the queries, pages that hold whole tiles,
+// or pages of a multiple of 16 keys.
+enum Source { kPacked, kPages, kSmallPages };
+
+struct AttnArgs {
+  const uint16_t* q;
+  int64_t q_st, q_sh;  // strides in elements (dim stride 1)
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_sn, k_st, k_sh, v_sn, v_st, v_sh;  // page, token, head
+  const int32_t* bt;
+  int64_t bt_sb, bt_sn;
+  const int32_t* ctx;   // paged: keys of each sequence
+  const int32_t* cu_q;
+  const int32_t* cu_k;  // packed
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  int batch, heads, kv_heads, group, page, num_blocks, width, total_q, total_k;
+  float scale_log2;
+  int* status;
+  int* report;  // pinned: [0] set to 1 where a sequence is flagged, [1] and [2] the packed rows' extent; or null
+};
+
+template <bool F16>
+struct Type;
+template <>
+struct Type<false> {
+  typedef bf16x8 vec;
+  typedef __bf16 elem;
+  static constexpr uint32_t kInf = 0x7F80u;
+  static __device__ __forceinline__ floatx16 mfma(vec a, vec b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Type<true> {
+  typedef f16x8 vec;
+  typedef _Float16 elem;
+  static constexpr uint32_t kInf = 0x7C00u;
+  static __device__ __forceinline__ floatx16 mfma(vec a, vec b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
+}
+
+__device__ __forceinline__ const uint8_t* uniform_ptr(const void* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<const uint8_t*>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+__device__ __forceinline__ int uniform_int(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Inclusive wave scan over lanes of non-negative values (0 is f's neutral element).
+template <typename F>
+__device__ __forceinline__ int wave_scan(int v, F f) {
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  return f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+}
+struct Add {
+  __device__ int operator()(int x, int y) const { return x + y; }
+};
+struct Max {
+  __device__ int operator()(int x, int y) const { return max(x, y); }
+};
+template <typename F>
+__device__ __forceinline__ int wave_reduce(int v, F f) {
+  return __builtin_amdgcn_readlane(wave_scan(v, f), 63);
+}
+
+struct Seq {
+  int q0, qlen, k0, klen;
+};
+
+__device__ __forceinline__ void flag_sequence(const AttnArgs& a, int i) {
+  atomicMin(a.status, i);
+  if (a.report != nullptr) a.report[0] = 1;  // (every writer stores the same)
+}
+
+// Sequence i's rows and keys; false where its lengths are not valid (packed:
+// offsets out of order or outside the tensors), which takes it out of the work.
+template <int SRC>
+__device__ __forceinline__ bool sequence(const AttnArgs& a, int i, Seq& s) {
+  const int q0 = a.cu_q[i], q1 = a.cu_q[i + 1];
+  s.q0 = q0;
+  s.qlen = q1 - q0;
+  bool ok = q0 >= 0 && q1 >= q0 && q1 <= a.total_q;
+  if constexpr (SRC == kPacked) {
+    const int k0 = a.cu_k[i], k1 = a.cu_k[i + 1];
+    s.k0 = k0;
+    s.klen = k1 - k0;
+    ok = ok && k0 >= 0 && k1 >= k0 && k1 <= a.total_k;
+  } else {
+    s.k0 = 0;
+    s.klen = a.ctx[i];
+    ok = ok && q1 > q0 && s.klen >= s.qlen && s.klen <= static_cast<int64_t>(a.width) * a.page;
+  }
+  return ok;
+}
+
+// Blocks of sequence i, and the level of its first: block j ends after about
+// (level + j) kRows / G keys.
+template <int SRC, int ROWS>
+__device__ __forceinline__ int seq_blocks(const AttnArgs& a, int i, bool flag, int& level0) {
+  Seq s;
+  level0 = 1;
+  if (!sequence<SRC>(a, i, s)) {
+    if (SRC != kPacked && flag) flag_sequence(a, i);
+    return 0;
+  }
+  level0 += static_cast<int>(static_cast<int64_t>(max(s.klen - s.qlen, 0)) * a.group / ROWS);
+  return (s.qlen * a.group + ROWS - 1) / ROWS;
+}
+
+struct Work {
+  int seq, block, head, total;
+};
+
+// Workgroup -> (sequence, block, kv head), the blocks with most keys first, so
+// that the launch ends on short ones; heads fastest, so that with 8 kv heads
+// each XCD reads one head's K/V.  A binary search over levels finds the
+// rank's level, a scan over the sequences with a block there its sequence.
+// Returns false for a workgroup beyond the real blocks.
+template <int SRC, int ROWS>
+__device__ bool locate(const AttnArgs& a, bool flag, Work& w) {
+  const int lane = __lane_id();
+  const int rank = uniform_int(static_cast<int>(blockIdx.x) / a.kv_heads);
+  w.head = static_cast<int>(blockIdx.x) - rank * a.kv_heads;
+  int total = 0, hi = 0, l0;
+  for (int base = 0; base < a.batch; base += 64) {
+    const int i = base + lane;
+    const int n = i < a.batch ? seq_blocks<SRC, ROWS>(a, i, flag, l0) : 0;
+    total += wave_reduce(n, Add());
+    hi = max(hi, wave_reduce(n == 0 ? 0 : l0 + n, Max()));
+  }
+  w.total = total;
+  if (rank >= total) return false;
+  if (a.batch <= 64) {
+    const int n = lane < a.batch ? seq_blocks<SRC, ROWS>(a, lane, false, l0) : 0;
+    auto above = [&](int u) { return min(max(l0 + n - 1 - max(u, l0 - 1), 0), n); };
+    int lo = 0;
+    while (lo < hi) {  // smallest level with at most `rank` blocks above it
+      const int mid = (lo + hi) / 2;
+      if (wave_reduce(above(mid), Add()) <= rank) hi = mid;
+      else lo = mid + 1;
+    }
+    const int at = (n > 0 && lo >= l0 && lo < l0 + n) ? 1 : 0;
+    const int incl = wave_scan(at, Add()) + wave_reduce(above(lo), Add());
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(at && incl == rank + 1));
+    w.seq = uniform_int(l);
+    w.block = lo - uniform_int(__shfl(l0, l));
+    return true;
+  }
+  // larger batches: sequence by sequence, in reverse
+  const int target = total - 1 - rank;
+  int before = 0;
+  for (int base = 0; base < a.batch; base += 64) {
+    const int i = base + lane;
+    const int n = i < a.batch ? seq_blocks<SRC, ROWS>(a, i, false, l0) : 0;
+    const int incl = wave_scan(n, Add()) + before;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(i < a.batch && target < incl && target >= incl - n);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      w.seq = uniform_int(base + l);
+      w.block = uniform_int(target - (__shfl(incl, l) - __shfl(n, l)));
+      return true;
+    }
+    before = __shfl(incl, 63);
+  }
+  return false;
+}
+
+// Rows outside every sequence are 0: the workgroups beyond the real blocks
+// (one per kv head at least) share them.
+template <int D>
+__device__ void zero_padding(const AttnArgs& a, int real_blocks) {
+  const int first = min(max(a.cu_q[0], 0), a.total_q), end = min(max(a.cu_q[a.batch], first), a.total_q);
+  const int me = static_cast<int>(blockIdx.x) - real_blocks * a.kv_heads;
+  const int64_t workers = static_cast<int64_t>(gridDim.x) - static_cast<int64_t>(real_blocks) * a.kv_heads;
+  const int64_t per_row = static_cast<int64_t>(a.heads) * (D / 8);
+  const int64_t chunks = (first + (a.total_q - end)) * per_row;
+  for (int64_t x = static_cast<int64_t>(me) * blockDim.x + threadIdx.x; x < chunks; x += workers * blockDim.x) {
+    int64_t row = x / per_row;
+    const int rest = static_cast<int>(x - row * per_row);
+    if (row >= first) row += end - first;
+    *reinterpret_cast<u32x4*>(a.out + row * a.o_st + rest / (D / 8) * a.o_sh + rest % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+  }
+}
+
+// 16-byte chunk swizzle of key t's row in LDS: chunk x holds the row's chunk
+// x ^ swz(t).  64 banks of 4 bytes; ds_read_b128 serves 16 lanes at a time,
+// ds_read_b64 (and _tr_b16) 32.  K reads (row c, chunk 2 x + g) then meet 16
+// distinct chunks of a 256-byte span, V reads (4 rows, 4 chunks of each) all of
+// it.  Rows of 64 dims are half a span: their parity is a chunk bit already.
+template <int D>
+__device__ __forceinline__ int swz(int t) {
+  const int t0 = t & 1, t1 = (t >> 1) & 1, t2 = (t >> 2) & 1, t3 = (t >> 3) & 1;
+  return D == 128 ? (t0 << 2) | (t1 << 3) | t2 | (t3 << 1) : (t1 << 2) | t2 | (t3 << 1);
+}
+
+template <bool F16, int D, int SRC>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+attention16_kernel(const AttnArgs a) {
+  using T = Type<F16>;
+  typedef typename T::vec vec;
+  constexpr int kRows = kCols * kWaves;
+  constexpr int kRow = D * 2;                 // bytes of a key's row in LDS
+  constexpr int kPayload = kKeys * kRow;
+  constexpr int kStage = 2 * kPayload;        // K, then V
+  constexpr int kSteps = D / 16;              // MFMAs per 32 x 32 scores
+  constexpr int kDims = D / 32;               // 32-dim tiles of the output
+  constexpr int kLoadRows = 1024 / kRow;      // rows per load of a wave
+  constexpr int kLoads = kKeys / kLoadRows / kWaves;
+  __shared__ __attribute__((aligned(256))) uint8_t stages[2 * kStage];
+
+  Work work;
+  const bool found = locate<SRC, kRows>(a, blockIdx.x == 0 && threadIdx.x < 64, work);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && a.report != nullptr) {
+    a.report[1] = a.cu_q[0];
+    a.report[2] = a.cu_q[a.batch];
+  }
+  if (!found) {
+    if (SRC == kPacked) zero_padding<D>(a, work.total);
+    return;
+  }
+  const int seq = uniform_int(work.seq), block = uniform_int(work.block), h = uniform_int(work.head);
+  const int tid = threadIdx.x;
+  const int wave = uniform_int(tid / 64);
+  const int lane = tid % 64;
+  const int c = lane % 32;
+  const int g = lane / 32;
+
+  Seq s;
+  sequence<SRC>(a, seq, s);
+  const int qs = uniform_int(s.q0), qlen = uniform_int(s.qlen), klen = uniform_int(s.klen);
+  const int prefix = klen - qlen;
+  const int rows = qlen * a.group;
+  const int row0 = block * kRows + wave * kCols;                               // the wave's first row
+  const int kend = min(klen, prefix + (min((block + 1) * kRows, rows) - 1) / a.group + 1);  // keys [0, kend) are needed
+  const int wpos0 = prefix + uniform_int(row0 / a.group);                      // position of the wave's first row
+  const int wlast = row0 < rows ? prefix + uniform_int((min(row0 + kCols, rows) - 1) / a.group) : -1;  // and of its last
+  const int tiles = kend > 0 ? (kend + kKeys - 1) / kKeys : 0;
+
+  // the lane's row: column c
+  const int row = row0 + c;
+  const bool colv = row < rows;
+  const int tok = colv ? row / a.group : 0;
+  const int head = h * a.group + (colv ? row - tok * a.group : 0);
+  const int pos = prefix + tok;
+  vec qop[kSteps];
+  {
+    const uint16_t* src = a.q + static_cast<int64_t>(qs + tok) * a.q_st + static_cast<int64_t>(head) * a.q_sh + 8 * g;
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x)
+      qop[x] = __builtin_bit_cast(vec, colv ? *reinterpret_cast<const u32x4*>(src + 16 * x) : u32x4{0, 0, 0, 0});
+  }
+
+  // ---- tile loads, straight into LDS.  A load of a wave covers kLoadRows rows;
+  // row and swizzled chunk of a lane do not change from load to load.
+  const int lrow = wave * kLoadRows + lane / (64 / kLoadRows);
+  const int lchunk = (lane % (64 / kLoadRows)) ^ swz<D>(lrow);
+  const int k_st = static_cast<int>(a.k_st) * 2, v_st = static_cast<int>(a.v_st) * 2;  // bytes
+  const uint8_t* k_head = reinterpret_cast<const uint8_t*>(a.k + static_cast<int64_t>(s.k0) * a.k_st + h * a.k_sh);
+  const uint8_t* v_head = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(s.k0) * a.v_st + h * a.v_sh);
+  const int32_t* bt_row = SRC == kPacked ? nullptr : a.bt + static_cast<int64_t>(seq) * a.bt_sb;
+  // 64 consecutive entries of the table row in one register
+  int pg = 0, prow = 0, ids_base = 0, ids = 0;
+  auto load_ids = [&](int base) { return bt_row[static_cast<int64_t>(min(base + lane, a.width - 1)) * a.bt_sn]; };
+  if (SRC != kPacked && tiles > 0) ids = load_ids(0);
+  auto block_at = [&](int page) {
+    if (page >= ids_base + 64) {
+      ids_base = page;
+      ids = load_ids(page);
+    }
+    return __builtin_amdgcn_readlane(ids, page - ids_base);
+  };
+  auto load_chunks = [&](const uint8_t* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(uniform_ptr(base)), "s"(lds) : "memory", "m0");
+  };
+  auto issue_tile = [&](int t, uint8_t* st) {
+    constexpr int kGroups = SRC == kSmallPages ? kKeys / 16 : 1;  // table lookups per tile
+    int blk[kGroups], at[kGroups];
+    if constexpr (SRC != kPacked) {
+      bool ok = true;
+#pragma unroll
+      for (int x = 0; x < kGroups; ++x) {
+        blk[x] = -1;
+        at[x] = prow;
+        if (SRC == kPages || t * kKeys + x * 16 < kend) {  // groups past the keys needed are not looked up
+          blk[x] = block_at(pg);
+          ok = ok && blk[x] >= 0 && blk[x] < a.num_blocks;
+          prow += kKeys / kGroups;
+          if (prow == a.page) {
+            prow = 0;
+            ++pg;
+          }
+        }
+      }
+      if (!ok) {
+        if (tid == 0) flag_sequence(a, seq);
+        return;
+      }
+    }
+    const uint32_t lds0 = lds_address(st) + static_cast<uint32_t>(wave) * 1024;
+#pragma unroll
+    for (int l = 0; l < 2 * kLoads; ++l) {
+      const bool isv = l >= kLoads;
+      const int tr = (isv ? l - kLoads : l) * kWaves * kLoadRows;  // first row of the waves' loads
+      const int st_bytes = isv ? v_st : k_st;
+      const uint8_t* base;
+      int r;  // the lane's row from there
+      if constexpr (SRC == kPacked) {
+        base = (isv ? v_head : k_head) + static_cast<int64_t>(t * kKeys) * st_bytes;
+        r = min(lrow + tr, klen - 1 - t * kKeys);  // (rows past the last key repeat it)
+      } else {
+        const int x = SRC == kPages ? 0 : uniform_int((tr + wave * kLoadRows) / 16);
+        int b = blk[0], p = at[0] + tr;
+#pragma unroll
+        for (int y = 1; y < kGroups; ++y)
+          if (x == y) b = blk[y], p = at[y] + tr - 16 * y;
+        if (SRC == kSmallPages && b < 0) continue;
+        base = (isv ? v_head + b * a.v_sn * 2 : k_head + b * a.k_sn * 2) + static_cast<int64_t>(p) * st_bytes;
+        r = lrow;
+      }
+      load_chunks(base, static_cast<uint32_t>(r * st_bytes + lchunk * 16),
+                  uniform_int(lds0 + (isv ? kPayload : 0) + static_cast<uint32_t>(tr) * kRow));
+    }
+  };
+
+  // per-lane LDS offsets inside a stage; other chunks differ by an exclusive or
+  const uint32_t stage_base = lds_address(stages);
+  const uint32_t k_rd = c * kRow + ((g ^ swz<D>(c)) << 4);
+  uint32_t v_rd;
+  {
+    const int l16 = lane % 16, t = 4 * g + (l16 >> 2);
+    v_rd = kPayload + t * kRow + (((2 * ((lane / 16) % 2) + ((l16 & 3) >> 1)) ^ swz<D>(t)) << 4) + (l16 & 1) * 8;
+  }
+
+  floatx16 acc[kDims];  // O^T: dims 32 n + 8 (r / 4) + 4 g + r % 4 of the lane's row
+  float m_run, l_run;
+
+  // A value that is no finite number multiplied by a masked weight's 0 is no
+  // 0.  Where an output is not finite the block is walked once more, carefully:
+  // on masked tiles such values are taken out of the product and added to the
+  // rows that see their key.
+  for (bool careful = false;; careful = true) {
+#pragma unroll
+    for (int n = 0; n < kDims; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
+    m_run = colv ? -INFINITY : 0.f;  // (columns without a row would otherwise count as rising on every tile)
+    l_run = 0.f;
+    pg = prow = 0;
+    if (SRC != kPacked && tiles > 0 && ids_base != 0) ids = load_ids(ids_base = 0);
+
+    if (tiles > 0) issue_tile(0, stages);
+    for (int t = 0; t < tiles; ++t) {
+      const uint32_t cur = (t & 1) * kStage;
+      __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this wave's part of tile t has landed
+      __syncthreads();                    // everyone's has, and nobody reads the other stage any more
+      if (t + 1 < tiles) issue_tile(t + 1, stages + (kStage - cur));
+      const int key0 = t * kKeys;
+      if (key0 > wlast) continue;
+      floatx16 sc[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[b][r] = 0.f;
+#pragma unroll
+        for (int x = 0; x < kSteps; ++x) {
+          const u32x4 kw = *reinterpret_cast<const u32x4*>(stages + b * 32 * kRow + ((cur + k_rd) ^ (x << 5)));
+          sc[b] = T::mfma(__builtin_bit_cast(vec, kw), qop[x], sc[b]);
+        }
+      }
+      const bool masked = key0 + kKeys - 1 > wpos0;  // (uniform)
+      const int last = colv ? pos - key0 - 4 * g : -1;  // last visible key, as a row offset of the lane
+      // Weights are first formed against the running max as it stands; their sum
+      // tells whether that was low enough, or is no number.  Only otherwise, and
+      // on masked tiles, are maxima taken and the accumulators rescaled.
+      vec pa[2][2];
+      float ps = 0.f;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[b][r], a.scale_log2, -m_run));
+          pa[b][r / 8][r % 8] = static_cast<typename T::elem>(p);
+          ps += p;
+        }
+      if (masked || __builtin_amdgcn_ballot_w64(!(ps <= kSumLimit)) != 0) {
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            sc[b][r] = 32 * b + 8 * (r / 4) + r % 4 <= last ? sc[b][r] * a.scale_log2 : -INFINITY;
+            tmax = fmaxf(tmax, sc[b][r]);
+          }
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
+        tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        const float m_new = tmax > m_run ? tmax : m_run;
+        const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int n = 0; n < kDims; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+        const float m_use = m_run == -INFINITY ? 0.f : m_run;
+        ps = 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(sc[b][r] - m_use);  // 0 where masked
+            pa[b][r / 8][r % 8] = static_cast<typename T::elem>(p);
+            ps += p;
+          }
+      }
+      l_run += ps;
+      // O^T += V^T P^T: k-slots 8 g + 0..3 of 16-key group m are keys 16 m + 4 g +
+      // 0..3, slots 8 g + 4..7 the keys 8 further, the order of the score rows
+      auto read_v = [&](int m, int n) {
+        union {
+          s16x4 half[2];
+          u32x4 w;
+        } u;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          u.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(
+              stage_base + ((cur + v_rd) ^ (n << 6) ^ (x << 5)) + (16 * m + 8 * x) * kRow));
+        if (key0 + kKeys > kend) {  // (uniform) keys that nobody sees may hold anything
+          const int left = kend - key0 - 16 * m - 4 * g;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const int j = 8 * (d / 2) + 2 * (d % 2);
+            u.w[d] &= (j < left ? 0xFFFFu : 0u) | (j + 1 < left ? 0xFFFF0000u : 0u);
+          }
+        }
+        return u.w;
+      };
+      if (careful && masked) {
+        const uint32_t one = F16 ? 0x3C00u : 0x3F80u;
+#pragma unroll 1
+        for (int m = 0; m < 4; ++m) {
+          u32x4 seen;  // 1 where the lane's row sees the key of the slot
+          vec p;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const int j = 16 * m + 8 * (d / 2) + 2 * (d % 2);
+            seen[d] = (j <= last ? one : 0u) | (j + 1 <= last ? one << 16 : 0u);
+          }
+          p = m == 0 ? pa[0][0] : m == 1 ? pa[0][1] : m == 2 ? pa[1][0] : pa[1][1];
+#pragma unroll
+          for (int n = 0; n < kDims; ++n) {
+            const u32x4 v = read_v(m, n);
+            u32x4 clean;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              const bool lo = (v[d] & T::kInf) == T::kInf, up = ((v[d] >> 16) & T::kInf) == T::kInf;
+              clean[d] = v[d] & ((lo ? 0u : 0xFFFFu) | (up ? 0u : 0xFFFF0000u));
+            }
+            acc[n] = T::mfma(__builtin_bit_cast(vec, clean), p, acc[n]);
+#pragma unroll 1
+            for (int kind = 0; kind < 3; ++kind) {  // infinities of either sign, NaN
+              u32x4 is;
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                is[d] = 0;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const uint32_t e = (v[d] >> (16 * half)) & 0xFFFFu;
+                  const bool hit = kind == 2 ? (e & 0x7FFFu) > T::kInf : e == (T::kInf | (kind == 1 ? 0x8000u : 0u));
+                  is[d] |= (hit ? one : 0u) << (16 * half);
+                }
+              }
+              floatx16 count;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) count[r] = 0.f;
+              count = T::mfma(__builtin_bit_cast(vec, is), __builtin_bit_cast(vec, seen), count);
+              const float what = kind == 2 ? __uint_as_float(0x7FC00000u) : kind == 1 ? -INFINITY : INFINITY;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) acc[n][r] = count[r] > 0.f ? acc[n][r] + what : acc[n][r];
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int n = 0; n < kDims; ++n)
+            acc[n] = T::mfma(__builtin_bit_cast(vec, read_v(m, n)), pa[m / 2][m % 2], acc[n]);
+      }
+    }
+    float check = 0.f;  // no finite number if one of them is none
+#pragma unroll
+    for (int n = 0; n < kDims; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) check = fmaf(acc[n][r], 0.f, check);
+    if (careful || !__syncthreads_or(check != 0.f)) break;
+  }
+
+  // ---- epilogue
+  const auto lsw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+  const float l_tot = __uint_as_float(lsw[0]) + __uint_as_float(lsw[1]);
+  if (!colv) return;
+  const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // (a NaN sum makes the row NaN)
+  uint16_t* dst = a.out + static_cast<int64_t>(qs + tok) * a.o_st + static_cast<int64_t>(head) * a.o_sh + 4 * g;
+#pragma unroll
+  for (int n = 0; n < kDims; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = acc[n][4 * i + j] * inv;
+        o[j] = F16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x);
+      }
+      *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) = u32x2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
+    }
+}
+
+template <bool F16, int D, int SRC>
+int launch(const AttnArgs& a, hipStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.total_q) * a.group;
+  // every sequence may end in a partial block; one more for rows outside them
+  const int64_t blocks = (ceil_div(rows, kCols * kWaves) + a.batch + 1) * a.kv_heads;
+  if (blocks > INT32_MAX || rows > INT32_MAX) {
+    set_error("attention over 16-bit keys: too many query rows for one launch");
+    return PRISM_ERR_INVALID;
+  }
+  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, stream, a);
+  return check_launch("attention16_kernel launch");
+}
+
+template <bool F16, int D>
+int by_source(const AttnArgs& a, hipStream_t stream) {
+  if (a.bt == nullptr) return launch<F16, D, kPacked>(a, stream);
+  return a.page % kKeys == 0 ? launch<F16, D, kPages>(a, stream) : launch<F16, D, kSmallPages>(a, stream);
+}
+
+int dispatch(const AttnArgs& a, int dtype, int head_dim, hipStream_t stream) {
+  if (dtype == PRISM_DTYPE_F16) return head_dim == 128 ? by_source<true, 128>(a, stream) : by_source<true, 64>(a, stream);
+  return head_dim == 128 ? by_source<false, 128>(a, stream) : by_source<false, 64>(a, stream);
+}
+
+// What both entries ask of q, K, V and out: types, heads, dims and layout.
+// Tile loads address the rows of a tile (or a page) by a 32-bit offset.
+int check_layout(const char* what, int dtype, int heads, int kv_heads, int head_dim, const void* q, const int64_t* qs,
+                 const void* k, const int64_t* ks, const void* v, const int64_t* vs, int rank, const void* out,
+                 const int64_t* os) {
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) {
+    set_error("%s: num_heads=%d must be a multiple of num_kv_heads=%d", what, heads, kv_heads);
+    return PRISM_ERR_INVALID;
+  }
+  if (dtype != PRISM_DTYPE_BF16 && dtype != PRISM_DTYPE_F16) {
+    set_error("%s: q, K and V must be bf16 or float16 (dtype code %d)", what, dtype);
+    return PRISM_ERR_LAYOUT;
+  }
+  if (head_dim != 64 && head_dim != 128) {
+    set_error("%s: head_dim must be 64 or 128, got %d", what, head_dim);
+    return PRISM_ERR_LAYOUT;
+  }
+  bool good = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16);
+  for (int i = 0; i < 3; ++i) good = good && (i == 2 ? qs[i] == 1 && os[i] == 1 : qs[i] % 8 == 0 && os[i] % 8 == 0);
+  for (int i = 0; i < rank; ++i)
+    good = good && (i == rank - 1 ? ks[i] == 1 && vs[i] == 1 : ks[i] % 8 == 0 && vs[i] % 8 == 0);
+  if (!good) {
+    set_error("%s: q, K/V and out need unit-stride head dims and 16-byte aligned rows", what);
+    return PRISM_ERR_LAYOUT;
+  }
+  for (const int64_t* s : {ks, vs})
+    if (s[rank - 3] < 0 || s[rank - 3] > INT32_MAX / (4 * kKeys)) {
+      set_error("%s: 64 key rows must span less than 1 GiB", what);
+      return PRISM_ERR_LAYOUT;
+    }
+  return PRISM_OK;
+}
+
+}  // namespace
+
+int preload_attention16() {
+  hipFuncAttributes attr;
+  return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&attention16_kernel<false, 128, kPacked>)), "preload_attention16");
+}
+
+// prism_paged_prefill_ws over 16-bit caches; its geometry and pointers are checked there.
+int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void* v, int dtype, const int64_t* ks,
+                    const int64_t* vs, const int32_t* bt, const int64_t* bts, const int32_t* ctx, const int32_t* cu_q,
+                    void* out, const int64_t* os, int batch, int total_q, int heads, int kv_heads, int head_dim, int page,
+                    int num_blocks, int width, float scale, int32_t* status, int32_t* report, hipStream_t stream) {
+  if (int rc = check_layout("prism_paged_prefill", dtype, heads, kv_heads, head_dim, q, qs, k, ks, v, vs, 4, out, os)) return rc;
+  if (page % 16 != 0) {
+    set_error("prism_paged_prefill: page size must be a multiple of 16, got %d", page);
+    return PRISM_ERR_LAYOUT;
+  }
+  if (batch == 0 || total_q == 0) return PRISM_OK;
+  AttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = qs[0], a.q_sh = qs[1];
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.k_sn = ks[0], a.k_st = ks[1], a.k_sh = ks[2];
+  a.v_sn = vs[0], a.v_st = vs[1], a.v_sh = vs[2];
+  a.bt = bt;
+  a.bt_sb = bts[0], a.bt_sn = bts[1];
+  a.ctx = ctx;
+  a.cu_q = cu_q;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_st = os[0], a.o_sh = os[1];
+  a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+  a.page = page, a.num_blocks = num_blocks, a.width = width, a.total_q = total_q;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.status = status;
+  a.report = report;
+  return dispatch(a, dtype, head_dim, stream);
+}
+
+}  // namespace prism
+
+extern "C" int prism_prompt_attention(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                                      const void* v, const int64_t v_strides[3], int dtype, const int32_t* cu_seqlens_q,
+                                      const int32_t* cu_seqlens_k, void* out, const int64_t out_strides[3], int batch,
+                                      int total_q, int total_k, int num_heads, int num_kv_heads, int head_dim, float scale,
+                                      void* stream) {
+  using namespace prism;
+  clear_error();
+  if (batch < 0 || total_q < 0 || total_k < 0) {
+    set_error("prism_prompt_attention: invalid geometry");
+    return PRISM_ERR_INVALID;
+  }
+  if (total_q == 0) return PRISM_OK;
+  if (!q || !q_strides || !k_strides || !v_strides || !out || !out_strides || !cu_seqlens_q || !cu_seqlens_k ||
+      (total_k > 0 && (!k || !v))) {
+    set_error("prism_prompt_attention: null argument");
+    return PRISM_ERR_INVALID;
+  }
+  if (int rc = check_layout("prism_prompt_attention", dtype, num_heads, num_kv_heads, head_dim, q, q_strides, k, k_strides,
+                            v, v_strides, 3, out, out_strides))
+    return rc;
+  AttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = q_strides[0], a.q_sh = q_strides[1];
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.k_st = k_strides[0], a.k_sh = k_strides[1];
+  a.v_st = v_strides[0], a.v_sh = v_strides[1];
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_st = out_strides[0], a.o_sh = out_strides[1];
+  a.batch = batch, a.heads = num_heads, a.kv_heads = num_kv_heads, a.group = num_heads / num_kv_heads;
+  a.total_q = total_q, a.total_k = total_k;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return dispatch(a, dtype, head_dim, static_cast<hipStream_t>(stream));
+}

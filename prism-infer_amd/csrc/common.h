@@ -28,6 +28,8 @@ int preload_kv_store();
 int preload_kv_compaction();
 int preload_paged_prefill();
 int preload_paged_decode();
+int preload_attention16();
+int preload_step_metadata();
 
 int device_cu_count();
 

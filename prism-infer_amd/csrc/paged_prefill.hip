@@ -941,6 +941,12 @@ int preload_paged_prefill() {
   return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&paged_prefill_kernel<PRISM_DTYPE_BF16, 4, true, true>)), "preload_paged_prefill");
 }
 
+// The same attention over 16-bit caches (attention16.hip).
+int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void* v, int dtype, const int64_t* ks,
+                    const int64_t* vs, const int32_t* bt, const int64_t* bts, const int32_t* ctx, const int32_t* cu_q,
+                    void* out, const int64_t* os, int batch, int total_q, int heads, int kv_heads, int head_dim, int page,
+                    int num_blocks, int width, float scale, int32_t* status, int32_t* report, hipStream_t stream);
+
 }  // namespace prism
 
 extern "C" int64_t prism_paged_prefill_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads,
@@ -969,6 +975,20 @@ extern "C" int prism_paged_prefill_ws(const void* q, int q_dtype, const int64_t 
       width < 0) {
     set_error("prism_paged_prefill: invalid geometry");
     return PRISM_ERR_INVALID;
+  }
+  if (cache_dtype == PRISM_DTYPE_BF16 || cache_dtype == PRISM_DTYPE_F16) {
+    if (q_dtype != cache_dtype || k_scale != nullptr || v_scale != nullptr) {
+      set_error("prism_paged_prefill: a 16-bit cache has no scales and the queries' type (dtype codes %d and %d)",
+                cache_dtype, q_dtype);
+      return PRISM_ERR_LAYOUT;
+    }
+    if (!q_strides || !k_strides || !v_strides || !bt_strides || !out_strides || !status) {
+      set_error("prism_paged_prefill: null argument");
+      return PRISM_ERR_INVALID;
+    }
+    return paged_prefill16(q, q_strides, k_cache, v_cache, cache_dtype, k_strides, v_strides, block_tables, bt_strides,
+                           context_lens, cu_seqlens_q, out, out_strides, batch, total_q, num_heads, num_kv_heads, head_dim,
+                           page_size, num_blocks, width, scale, status, report, static_cast<hipStream_t>(stream_ptr));
   }
   if (num_heads % num_kv_heads != 0 || num_heads / num_kv_heads > kPfMaxWaves) {
     set_error("prism_paged_prefill: num_heads=%d / num_kv_heads=%d must be an integer group of at most %d",

@@ -89,6 +89,12 @@ SIGNATURES: dict[str, tuple] = {
         [_VP, _I, _I64P, _VP, _VP, _I, _I64P, _I64P, _VP, _VP, _I64P, _I64P, _VP, _I64P, _VP, _VP, _VP,
          _I64P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _VP, _VP, _I64, _VP, _VP],
     ),
+    "prism_prompt_attention": (
+        _I,
+        [_VP, _I64P, _VP, _I64P, _VP, _I64P, _I, _VP, _VP, _VP, _I64P, _I, _I, _I, _I, _I, _I, _F, _VP],
+    ),
+    "prism_step_metadata_words": (_I64, [_I, _I, _I]),
+    "prism_step_metadata": (_I, [_VP, _I64P, _VP, _VP, _VP, _I, _VP, _I, _I, _I, _I, _VP, _VP]),
     "prism_debug_fp8_encode": (_I, [_VP, _VP, _I64, _VP]),
 }
 
@@ -209,6 +215,22 @@ def strides(tensor: torch.Tensor) -> ctypes.Array:
     return (ctypes.c_int64 * len(values))(*values)
 
 
+def aligned_rows(tensor: torch.Tensor) -> torch.Tensor:
+    """The tensor, or a copy where a row of its last dimension is not contiguous or does not start on 16 bytes."""
+
+    unit = 16 // tensor.element_size()
+    if (tensor.stride(-1) == 1 and tensor.data_ptr() % 16 == 0
+            and all(n == 1 or s % unit == 0 for n, s in zip(tensor.shape[:-1], tensor.stride()))):
+        return tensor
+    return tensor.clone(memory_format=torch.contiguous_format)
+
+
+def row_strides(tensor: torch.Tensor) -> ctypes.Array:
+    """Strides, 0 for leading dimensions of one entry (which may hold any number there)."""
+
+    return int64s(*(0 if n == 1 else s for n, s in zip(tensor.shape[:-1], tensor.stride())), tensor.stride(-1))
+
+
 def int64s(*values: int) -> ctypes.Array:
     return (ctypes.c_int64 * len(values))(*values)
 
@@ -230,6 +252,7 @@ def check(status: int, what: str) -> None:
 
 __all__ = [
     "ABI_VERSION",
+    "aligned_rows",
     "DTYPE_BF16",
     "DTYPE_F16",
     "DTYPE_F32",
@@ -246,6 +269,7 @@ __all__ = [
     "is_built",
     "lib",
     "library_path",
+    "row_strides",
     "stream_handle",
     "strides",
 ]

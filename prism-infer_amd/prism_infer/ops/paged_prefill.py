@@ -1,4 +1,4 @@
-"""Paged prefill attention over scaled-FP8 pages on MI355X (HIP kernel).
+"""Paged prefill attention over FP8 or 16-bit pages on MI355X (HIP kernels).
 
 Drop-in for ``paged_prefill_attention_reference``
 (prism_infer/ops/paged_attention_reference.py:185-246), which
@@ -25,9 +25,13 @@ Differences a caller can see: K/V are dequantised in fp32 (payload times
 scale applied to the fp32 scores and to the softmax weights, as the decode
 kernels do) instead of in q's dtype, so results differ from the reference
 by bf16 rounding of the dequantised cache (the GPU tests bound it).  The
-kernel covers FP8 E4M3FN caches (scaled or unit-scale), head_dim 128, page
-sizes that are multiples of 16, GQA groups of 1, 2, 4 or 8 and bf16/fp16
-queries; other cases raise ``RuntimeError`` (no CPU fallback).
+kernels cover bf16/fp16 queries and page sizes that are multiples of 16, over
+
+- FP8 E4M3FN caches (scaled or unit-scale): head_dim 128, GQA groups of 1, 2,
+  4 or 8;
+- bf16/fp16 caches of the queries' dtype: head_dim 64 or 128, any GQA group.
+
+Other cases raise ``RuntimeError`` (no CPU fallback).
 """
 
 from __future__ import annotations
@@ -43,6 +47,7 @@ _HOST = _native.host_ops()
 
 MINIMUM_PAGED_CACHE_RANK = 3
 PREFILL_HEAD_DIM = 128
+PREFILL_HEAD_DIMS_16BIT = (64, 128)
 _STATUS_OK = 2**31 - 1
 
 # Per thread and (device, stream): the status word, which holds _STATUS_OK
@@ -158,11 +163,16 @@ def _launch_paged_prefill(q, k_cache, v_cache, context, *, num_heads, num_kv_hea
     if not all(t.is_cuda for t in tensors) or any(t.device != q.device for t in tensors):
         raise RuntimeError("paged_prefill_attention runs on the GPU: q, caches and scales must share one CUDA device")
     lib = _native.device_lib(q.device)
-    if k_cache.dtype != torch.float8_e4m3fn:
-        raise RuntimeError(f"the HIP paged prefill kernel reads FP8 E4M3FN caches, got {k_cache.dtype}")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError(f"the HIP paged prefill kernel takes bf16 or float16 queries, got {q.dtype}")
-    if q.shape[2] != PREFILL_HEAD_DIM:
+    if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (torch.float8_e4m3fn, q.dtype):
+        raise RuntimeError("the HIP paged prefill kernel reads FP8 E4M3FN caches or caches of the queries' dtype, "
+                           f"got {k_cache.dtype} and {v_cache.dtype} with {q.dtype} queries")
+    if k_cache.dtype != torch.float8_e4m3fn:
+        if q.shape[2] not in PREFILL_HEAD_DIMS_16BIT:
+            raise RuntimeError("the HIP paged prefill kernel covers head_dim 64 and 128 over 16-bit caches, "
+                               f"got {q.shape[2]}")
+    elif q.shape[2] != PREFILL_HEAD_DIM:
         raise RuntimeError(f"the HIP paged prefill kernel covers head_dim {PREFILL_HEAD_DIM}, got {q.shape[2]}")
 
     device = q.device
@@ -177,7 +187,10 @@ def _launch_paged_prefill(q, k_cache, v_cache, context, *, num_heads, num_kv_hea
             f"cu_seqlens_q needs {batch + 1} entries and block_tables {batch} rows, "
             f"got {cu_seqlens_q.numel()} and {block_tables.shape[0]}"
         )
-    if q.stride(2) != 1:
+    sixteen = k_cache.dtype == q.dtype
+    if sixteen:
+        q = _native.aligned_rows(q)
+    elif q.stride(2) != 1:
         q = q.contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     status = torch.full((1,), _STATUS_OK, dtype=torch.int32, device=device)
@@ -188,7 +201,7 @@ def _launch_paged_prefill(q, k_cache, v_cache, context, *, num_heads, num_kv_hea
     zero3 = _native.int64s(0, 0, 0)
     with torch.cuda.device(device):
         rc = lib.prism_paged_prefill_ws(
-            q.data_ptr(), _native.dtype_code(q.dtype), _native.strides(q),
+            q.data_ptr(), _native.dtype_code(q.dtype), _native.row_strides(q) if sixteen else _native.strides(q),
             k_cache.data_ptr(), v_cache.data_ptr(), _native.dtype_code(k_cache.dtype),
             _native.strides(k_cache), _native.strides(v_cache),
             k_scale_cache.data_ptr() if scaled else None, v_scale_cache.data_ptr() if scaled else None,
