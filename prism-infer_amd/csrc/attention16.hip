@@ -17,9 +17,17 @@
 // rescaling of its accumulators are lane-local.  P^T, rounded to the cache's
 // type (weights of at most 2^8 against fp32 sums), is the B operand of O^T +=
 // V^T P^T as it stands, V^T comes from ds_read_b64_tr_b16.
+//
+// Bound by the MFMAs and the exponentials beside them: a wave's tile is 32
+// MFMAs of 32 cycles and about 112 VALU instructions, 32 of them exponentials
+// of 16 cycles, and two waves share a SIMD.  With the three parts of a tile one
+// after the other 2 x 8192 tokens (32 / 8 heads) took 1414 us; with the next
+// tile's scores and the last one's output beside the softmax 1055 (1042
+// TFLOP/s, 0.83 of a large library product on the same card).
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace prism {
 namespace {
@@ -241,6 +249,13 @@ __device__ __forceinline__ int swz(int t) {
   return D == 128 ? (t0 << 2) | (t1 << 3) | t2 | (t3 << 1) : (t1 << 2) | t2 | (t3 << 1);
 }
 
+// Two fp32 values -> two 16-bit ones, to nearest even.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack(float lo, float up) {
+  if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, up}, f16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, up}, bf16x2));
+}
+
 template <bool F16, int D, int SRC>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
 attention16_kernel(const AttnArgs a) {
@@ -248,13 +263,14 @@ attention16_kernel(const AttnArgs a) {
   typedef typename T::vec vec;
   constexpr int kRows = kCols * kWaves;
   constexpr int kRow = D * 2;                 // bytes of a key's row in LDS
-  constexpr int kPayload = kKeys * kRow;
-  constexpr int kStage = 2 * kPayload;        // K, then V
+  constexpr int kPayload = kKeys * kRow;      // a tile's K or V
   constexpr int kSteps = D / 16;              // MFMAs per 32 x 32 scores
   constexpr int kDims = D / 32;               // 32-dim tiles of the output
+  constexpr int kPairs = D / 8;               // K operands of a tile, and V operands
   constexpr int kLoadRows = 1024 / kRow;      // rows per load of a wave
   constexpr int kLoads = kKeys / kLoadRows / kWaves;
-  __shared__ __attribute__((aligned(256))) uint8_t stages[2 * kStage];
+  constexpr int kV = 2 * kPayload;            // two stages of K, then two of V
+  __shared__ __attribute__((aligned(256))) uint8_t lds[4 * kPayload];
 
   Work work;
   const bool found = locate<SRC, kRows>(a, blockIdx.x == 0 && threadIdx.x < 64, work);
@@ -279,289 +295,436 @@ attention16_kernel(const AttnArgs a) {
   const int prefix = klen - qlen;
   const int rows = qlen * a.group;
   const int row0 = block * kRows + wave * kCols;                               // the wave's first row
-  const int kend = min(klen, prefix + (min((block + 1) * kRows, rows) - 1) / a.group + 1);  // keys [0, kend) are needed
+  const int kend = min(klen, prefix + uniform_int((min((block + 1) * kRows, rows) - 1) / a.group) + 1);  // keys [0, kend) are needed
   const int wpos0 = prefix + uniform_int(row0 / a.group);                      // position of the wave's first row
   const int wlast = row0 < rows ? prefix + uniform_int((min(row0 + kCols, rows) - 1) / a.group) : -1;  // and of its last
-  const int tiles = kend > 0 ? (kend + kKeys - 1) / kKeys : 0;
+  const int t0 = 0, t1 = kend > 0 ? (kend + kKeys - 1) / kKeys : 0;           // the workgroup's tiles
+  const int tw = wlast >= 0 ? min(t1, wlast / kKeys + 1) : 0;                  // the wave's end
 
   // the lane's row: column c
-  const int row = row0 + c;
-  const bool colv = row < rows;
-  const int tok = colv ? row / a.group : 0;
-  const int head = h * a.group + (colv ? row - tok * a.group : 0);
-  const int pos = prefix + tok;
+  auto row_at = [&](int& tok, int& head) {
+    const int row = row0 + c;
+    tok = row / a.group;
+    head = h * a.group + (row - tok * a.group);
+    return row < rows;
+  };
+  int pos;  // position of the row's token, below 0 where it sees no key (and without a row)
   vec qop[kSteps];
   {
+    int tok, head;
+    const bool real = row_at(tok, head);
+    pos = real ? prefix + tok : -1;
     const uint16_t* src = a.q + static_cast<int64_t>(qs + tok) * a.q_st + static_cast<int64_t>(head) * a.q_sh + 8 * g;
 #pragma unroll
     for (int x = 0; x < kSteps; ++x)
-      qop[x] = __builtin_bit_cast(vec, colv ? *reinterpret_cast<const u32x4*>(src + 16 * x) : u32x4{0, 0, 0, 0});
+      qop[x] = __builtin_bit_cast(vec, real ? *reinterpret_cast<const u32x4*>(src + 16 * x) : u32x4{0, 0, 0, 0});
   }
 
   // ---- tile loads, straight into LDS.  A load of a wave covers kLoadRows rows;
-  // row and swizzled chunk of a lane do not change from load to load.
+  // row and swizzled chunk of a lane do not change from load to load.  Asm so
+  // that the compiler's wait-count pass does not drain these loads before each
+  // LDS read of another stage.
   const int lrow = wave * kLoadRows + lane / (64 / kLoadRows);
   const int lchunk = (lane % (64 / kLoadRows)) ^ swz<D>(lrow);
   const int k_st = static_cast<int>(a.k_st) * 2, v_st = static_cast<int>(a.v_st) * 2;  // bytes
   const uint8_t* k_head = reinterpret_cast<const uint8_t*>(a.k + static_cast<int64_t>(s.k0) * a.k_st + h * a.k_sh);
   const uint8_t* v_head = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(s.k0) * a.v_st + h * a.v_sh);
   const int32_t* bt_row = SRC == kPacked ? nullptr : a.bt + static_cast<int64_t>(seq) * a.bt_sb;
-  // 64 consecutive entries of the table row in one register
-  int pg = 0, prow = 0, ids_base = 0, ids = 0;
   auto load_ids = [&](int base) { return bt_row[static_cast<int64_t>(min(base + lane, a.width - 1)) * a.bt_sn]; };
-  if (SRC != kPacked && tiles > 0) ids = load_ids(0);
-  auto block_at = [&](int page) {
-    if (page >= ids_base + 64) {
+  // The table is walked tile by tile; 64 consecutive entries sit in one register.
+  constexpr int kGroups = SRC == kSmallPages ? kKeys / 16 : 1;  // entries per tile
+  struct Place {
+    int blk[kGroups], row[kGroups];  // page (-1: not needed) and first row in it, per group
+    bool ok;
+  };
+  int page = 0, page_row = 0, ids_base = 0, ids = 0;
+  auto start_walk = [&]() {
+    if constexpr (SRC != kPacked) {
+      page = uniform_int(t0 * kKeys / a.page);
+      page_row = t0 * kKeys - page * a.page;
       ids_base = page;
       ids = load_ids(page);
     }
-    return __builtin_amdgcn_readlane(ids, page - ids_base);
   };
-  auto load_chunks = [&](const uint8_t* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 : : "v"(off), "s"(uniform_ptr(base)), "s"(lds) : "memory", "m0");
-  };
-  auto issue_tile = [&](int t, uint8_t* st) {
-    constexpr int kGroups = SRC == kSmallPages ? kKeys / 16 : 1;  // table lookups per tile
-    int blk[kGroups], at[kGroups];
+  auto look_up = [&](int t) {
+    Place p;
+    p.ok = true;
     if constexpr (SRC != kPacked) {
-      bool ok = true;
 #pragma unroll
       for (int x = 0; x < kGroups; ++x) {
-        blk[x] = -1;
-        at[x] = prow;
+        p.blk[x] = -1;
+        p.row[x] = page_row;
         if (SRC == kPages || t * kKeys + x * 16 < kend) {  // groups past the keys needed are not looked up
-          blk[x] = block_at(pg);
-          ok = ok && blk[x] >= 0 && blk[x] < a.num_blocks;
-          prow += kKeys / kGroups;
-          if (prow == a.page) {
-            prow = 0;
-            ++pg;
+          if (page >= ids_base + 64) {
+            ids_base = page;
+            ids = load_ids(page);
+          }
+          p.blk[x] = __builtin_amdgcn_readlane(ids, page - ids_base);
+          p.ok = p.ok && p.blk[x] >= 0 && p.blk[x] < a.num_blocks;
+          page_row += kKeys / kGroups;
+          if (page_row == a.page) {
+            page_row = 0;
+            ++page;
           }
         }
       }
-      if (!ok) {
-        if (tid == 0) flag_sequence(a, seq);
-        return;
-      }
+      if (!p.ok && tid == 0) flag_sequence(a, seq);
     }
-    const uint32_t lds0 = lds_address(st) + static_cast<uint32_t>(wave) * 1024;
+    return p;
+  };
+  auto load_chunks = [&](const uint8_t* base, uint32_t off, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(uniform_ptr(base)), "s"(dst) : "memory", "m0");
+  };
+  const uint32_t lds0 = lds_address(lds);
+  // Starts the loads of K or V of tile t into LDS offset `stage`.  (A tile that
+  // cannot be loaded leaves the stage as it was: its sequence is flagged.)
+  auto issue = [&](int t, const Place& place, bool isv, uint32_t stage) {
+    if (!place.ok) return;
+    const int st_bytes = isv ? v_st : k_st;
+    const uint8_t* head_base = isv ? v_head : k_head;
+    const int64_t page_bytes = (isv ? a.v_sn : a.k_sn) * 2;
 #pragma unroll
-    for (int l = 0; l < 2 * kLoads; ++l) {
-      const bool isv = l >= kLoads;
-      const int tr = (isv ? l - kLoads : l) * kWaves * kLoadRows;  // first row of the waves' loads
-      const int st_bytes = isv ? v_st : k_st;
+    for (int l = 0; l < kLoads; ++l) {
+      const int tr = l * kWaves * kLoadRows;  // first row of the waves' loads
       const uint8_t* base;
       int r;  // the lane's row from there
       if constexpr (SRC == kPacked) {
-        base = (isv ? v_head : k_head) + static_cast<int64_t>(t * kKeys) * st_bytes;
+        base = head_base + static_cast<int64_t>(t * kKeys) * st_bytes;
         r = min(lrow + tr, klen - 1 - t * kKeys);  // (rows past the last key repeat it)
       } else {
         const int x = SRC == kPages ? 0 : uniform_int((tr + wave * kLoadRows) / 16);
-        int b = blk[0], p = at[0] + tr;
+        int b = place.blk[0], p = place.row[0] + tr;
 #pragma unroll
         for (int y = 1; y < kGroups; ++y)
-          if (x == y) b = blk[y], p = at[y] + tr - 16 * y;
+          if (x == y) b = place.blk[y], p = place.row[y] + tr - 16 * y;
         if (SRC == kSmallPages && b < 0) continue;
-        base = (isv ? v_head + b * a.v_sn * 2 : k_head + b * a.k_sn * 2) + static_cast<int64_t>(p) * st_bytes;
+        base = head_base + b * page_bytes + static_cast<int64_t>(p) * st_bytes;
         r = lrow;
       }
       load_chunks(base, static_cast<uint32_t>(r * st_bytes + lchunk * 16),
-                  uniform_int(lds0 + (isv ? kPayload : 0) + static_cast<uint32_t>(tr) * kRow));
+                  uniform_int(lds0 + stage + static_cast<uint32_t>(wave) * 1024 + static_cast<uint32_t>(tr) * kRow));
     }
   };
 
   // per-lane LDS offsets inside a stage; other chunks differ by an exclusive or
-  const uint32_t stage_base = lds_address(stages);
   const uint32_t k_rd = c * kRow + ((g ^ swz<D>(c)) << 4);
   uint32_t v_rd;
   {
     const int l16 = lane % 16, t = 4 * g + (l16 >> 2);
-    v_rd = kPayload + t * kRow + (((2 * ((lane / 16) % 2) + ((l16 & 3) >> 1)) ^ swz<D>(t)) << 4) + (l16 & 1) * 8;
+    v_rd = t * kRow + (((2 * ((lane / 16) % 2) + ((l16 & 3) >> 1)) ^ swz<D>(t)) << 4) + (l16 & 1) * 8;
   }
+  auto read_k = [&](uint32_t stage, int pair) {  // pair: 32-key half, MFMA step
+    const int b = pair / kSteps, x = pair % kSteps;
+    return *reinterpret_cast<const u32x4*>(lds + b * 32 * kRow + ((stage + k_rd) ^ (x << 5)));
+  };
+  // V^T operand: k-slots 8 g + 0..3 of 16-key group m are keys 16 m + 4 g + 0..3,
+  // slots 8 g + 4..7 the keys 8 further, the order of the score rows
+  auto read_v = [&](uint32_t stage, int pair) {  // pair: 16-key group m, 32-dim tile n
+    const int m = pair / kDims, n = pair % kDims;
+    union {
+      s16x4 half[2];
+      u32x4 w;
+    } u;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      u.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          reinterpret_cast<lds_s16x4*>(lds0 + ((stage + v_rd) ^ (n << 6) ^ (x << 5)) + (16 * m + 8 * x) * kRow));
+    return u.w;
+  };
+  // the same with keys that nobody sees, which may hold anything, as 0
+  auto read_v_end = [&](uint32_t stage, int pair, int key0) {
+    u32x4 w = read_v(stage, pair);
+    const int left = kend - key0 - 16 * (pair / kDims) - 4 * g;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const int j = 8 * (d / 2) + 2 * (d % 2);
+      w[d] &= (j < left ? 0xFFFFu : 0u) | (j + 1 < left ? 0xFFFF0000u : 0u);
+    }
+    return w;
+  };
 
   floatx16 acc[kDims];  // O^T: dims 32 n + 8 (r / 4) + 4 g + r % 4 of the lane's row
   float m_run, l_run;
+  auto reset = [&]() {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+    m_run = pos >= 0 ? -INFINITY : 0.f;  // (rows without a key would otherwise count as rising on every tile)
+    l_run = 0.f;
+  };
+  auto scores_step = [&](int x, const u32x4& k, floatx16& sc) {
+    if (x == 0)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+    sc = T::mfma(__builtin_bit_cast(vec, k), qop[x], sc);
+  };
+  auto output_step = [&](int pair, const u32x4& v, const u32x4 (&p)[4]) {
+    acc[pair % kDims] = T::mfma(__builtin_bit_cast(vec, v), __builtin_bit_cast(vec, p[pair / kDims]), acc[pair % kDims]);
+  };
+  // Weights of a tile with their masks: maxima are taken and the accumulators rescaled.
+  auto settle = [&](int key0, const floatx16 (&sc)[2], u32x4 (&pa)[4], float& ps) {
+    const int last = pos - key0 - 4 * g;  // last visible key, as a row offset of the lane
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        tmax = fmaxf(tmax, 32 * b + 8 * (r / 4) + r % 4 <= last ? sc[b][r] * a.scale_log2 : -INFINITY);
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
+    tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    const float m_new = tmax > m_run ? tmax : m_run;
+    // (no key seen: keep the accumulators, all zero, from (-inf) - (-inf))
+    const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    ps = 0.f;
+    int seen = last;  // (compared anew: 32 lane masks kept from above would fill the SGPRs)
+    asm("" : "+v"(seen));
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        float p[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          p[j] = 32 * b + 8 * (r / 4) + r % 4 + j <= seen
+                     ? __builtin_amdgcn_exp2f(fmaf(sc[b][r + j], a.scale_log2, -m_use)) : 0.f;
+        pa[2 * b + r / 8][r % 8 / 2] = pack<F16>(p[0], p[1]);
+        ps += p[0] + p[1];
+      }
+  };
+  // (a wave meets the others' barriers by their number, wherever in its code it stands)
+  auto barrier = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  };
+  auto landed = [&]() { __builtin_amdgcn_s_waitcnt(0xF70); };  // vmcnt(0)
+
+  // ---- the loop.  Iteration t takes the scores of tile t + 1 (MFMAs), the
+  // softmax of tile t (VALU) and the product of tile t - 1's weights with its
+  // values (MFMAs), which do not depend on each other.  An MFMA holds its wave
+  // until the one before it is through, so they are laid out by hand, in slots
+  // of one MFMA and the VALU work that fits beside it.
+  reset();
+  {
+    uint32_t k_next = kPayload, v_prev = kV;  // stages of K of tile t + 1 and V of tile t - 1
+    Place place[3] = {};  // of tiles t, t + 1 and t + 2
+    if (t0 < t1) {
+      start_walk();
+      place[0] = look_up(t0);
+      issue(t0, place[0], false, 0);
+      if (t0 + 1 < t1) {
+        place[1] = look_up(t0 + 1);
+        issue(t0 + 1, place[1], false, kPayload);
+      }
+    }
+    landed();
+    barrier();
+    floatx16 sa[2], sb[2];
+    u32x4 pa[4], pb[4];
+    if (t0 < tw) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) scores_step(i % kSteps, read_k(0, i), sa[i / kSteps]);
+    }
+    // A wave's tile t: weights pn from scores sc, next scores sn; OUT: whether there
+    // is a tile t - 1, with weights pp.  Past the last tile the scores are taken
+    // from stale bytes, for nothing.
+    auto tile = [&](auto out, int t, floatx16 (&sc)[2], floatx16 (&sn)[2], u32x4 (&pp)[4], u32x4 (&pn)[4]) {
+      constexpr bool OUT = decltype(out)::value;
+      constexpr int kPerSlot = 16 / kPairs;  // halves of a pair of weights beside an MFMA
+      constexpr int kAhead = 1;              // operands are read this many pairs ahead
+      uint32_t v_tile = v_prev;
+      if constexpr (SRC != kPacked && D == 128) asm volatile("" : "+v"(v_tile));  // (hoisted, V's eight addresses spill)
+      u32x4 kq[kAhead + 1], vq[kAhead + 1];
+      float ps = 0.f, x1 = 0.f, e0 = 0.f;
+      auto half = [&](int i) {
+        const int m = i / 8, b = m / 2, r = m % 2 * 8 + i % 8 / 2 * 2;
+        if (i % 2 == 0) {
+          e0 = __builtin_amdgcn_exp2f(fmaf(sc[b][r], a.scale_log2, -m_run));
+          x1 = fmaf(sc[b][r + 1], a.scale_log2, -m_run);
+        } else {
+          const float e1 = __builtin_amdgcn_exp2f(x1);
+          pn[m][r % 8 / 2] = pack<F16>(e0, e1);
+          ps += e0 + e1;
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        kq[i] = read_k(k_next, i);
+        if (OUT) vq[i] = read_v(v_tile, i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        if (i + kAhead < kPairs) {
+          kq[(i + kAhead) % (kAhead + 1)] = read_k(k_next, i + kAhead);
+          if (OUT) vq[(i + kAhead) % (kAhead + 1)] = read_v(v_tile, i + kAhead);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (j == 0) scores_step(i % kSteps, kq[i % (kAhead + 1)], sn[i / kSteps]);
+          else if (OUT) output_step(i, vq[i % (kAhead + 1)], pp);
+#pragma unroll
+          for (int y = 0; y < kPerSlot; ++y) half((2 * i + j) * kPerSlot + y);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      // The weights were formed against the running max as it stood; their sum tells
+      // whether that was low enough, or is no number.  Only otherwise, and on masked
+      // tiles, are maxima taken.  (The pins keep the weights in front of the branch.)
+      asm volatile("" : "+v"(ps), "+v"(pn[0]), "+v"(pn[1]), "+v"(pn[2]), "+v"(pn[3]));
+      const int key0 = t * kKeys;
+      if (key0 + kKeys - 1 > wpos0 || __builtin_amdgcn_ballot_w64(!(ps <= kSumLimit)) != 0) settle(key0, sc, pn, ps);
+      l_run += ps;
+    };
+    // The step that begins iteration t of every wave: K of tile t + 1 and V of
+    // tile t - 1 have landed for all; K of tile t + 2 and V of tile t go where K
+    // of tile t and V of tile t - 2 were, which every wave is done with.
+    auto begin = [&](int t) {
+      landed();
+      barrier();
+      if (t + 2 < t1) {
+        place[2] = look_up(t + 2);
+        issue(t + 2, place[2], false, k_next ^ kPayload);
+      }
+      if (t < t1) issue(t, place[0], true, v_prev ^ kPayload);
+      place[0] = place[1];
+      place[1] = place[2];
+    };
+    auto next = [&]() {
+      k_next ^= kPayload;
+      v_prev ^= kPayload;
+    };
+    // Waves part ways at the end of their rows' keys, but meet at as many barriers.
+    int t = t0;
+    if (t0 < tw) {
+      begin(t);
+      tile(std::false_type(), t, sa, sb, pb, pa);
+      next();
+      bool odd = false;
+      for (++t; t < tw; ++t) {
+        begin(t);
+        tile(std::true_type(), t, sb, sa, pa, pb);
+        next();
+        odd = ++t == tw;
+        if (odd) break;
+        begin(t);
+        tile(std::true_type(), t, sa, sb, pb, pa);
+        next();
+      }
+      if (odd)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) pa[m] = pb[m];
+      begin(t);
+      const int key0 = (t - 1) * kKeys;
+      const bool cut = key0 + kKeys > kend;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) output_step(i, cut ? read_v_end(v_prev, i, key0) : read_v(v_prev, i), pa);
+      next();
+      ++t;
+    }
+    for (; t <= t1; ++t) {
+      begin(t);
+      next();
+    }
+  }
 
   // A value that is no finite number multiplied by a masked weight's 0 is no
-  // 0.  Where an output is not finite the block is walked once more, carefully:
-  // on masked tiles such values are taken out of the product and added to the
-  // rows that see their key.
-  for (bool careful = false;; careful = true) {
+  // 0.  Where an output is not finite the block is walked once more, one thing
+  // after the other: on masked tiles such values are taken out of the product
+  // and added to the rows that see their key.
+  float check = 0.f;  // no finite number if one of them is none
 #pragma unroll
-    for (int n = 0; n < kDims; ++n)
+  for (int d = 0; d < kDims; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
-    m_run = colv ? -INFINITY : 0.f;  // (columns without a row would otherwise count as rising on every tile)
-    l_run = 0.f;
-    pg = prow = 0;
-    if (SRC != kPacked && tiles > 0 && ids_base != 0) ids = load_ids(ids_base = 0);
-
-    if (tiles > 0) issue_tile(0, stages);
-    for (int t = 0; t < tiles; ++t) {
-      const uint32_t cur = (t & 1) * kStage;
-      __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this wave's part of tile t has landed
-      __syncthreads();                    // everyone's has, and nobody reads the other stage any more
-      if (t + 1 < tiles) issue_tile(t + 1, stages + (kStage - cur));
-      const int key0 = t * kKeys;
-      if (key0 > wlast) continue;
-      floatx16 sc[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[b][r] = 0.f;
-#pragma unroll
-        for (int x = 0; x < kSteps; ++x) {
-          const u32x4 kw = *reinterpret_cast<const u32x4*>(stages + b * 32 * kRow + ((cur + k_rd) ^ (x << 5)));
-          sc[b] = T::mfma(__builtin_bit_cast(vec, kw), qop[x], sc[b]);
-        }
-      }
-      const bool masked = key0 + kKeys - 1 > wpos0;  // (uniform)
-      const int last = colv ? pos - key0 - 4 * g : -1;  // last visible key, as a row offset of the lane
-      // Weights are first formed against the running max as it stands; their sum
-      // tells whether that was low enough, or is no number.  Only otherwise, and
-      // on masked tiles, are maxima taken and the accumulators rescaled.
-      vec pa[2][2];
-      float ps = 0.f;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[b][r], a.scale_log2, -m_run));
-          pa[b][r / 8][r % 8] = static_cast<typename T::elem>(p);
-          ps += p;
-        }
-      if (masked || __builtin_amdgcn_ballot_w64(!(ps <= kSumLimit)) != 0) {
-        float tmax = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            sc[b][r] = 32 * b + 8 * (r / 4) + r % 4 <= last ? sc[b][r] * a.scale_log2 : -INFINITY;
-            tmax = fmaxf(tmax, sc[b][r]);
-          }
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
-        tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        const float m_new = tmax > m_run ? tmax : m_run;
-        const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
-        m_run = m_new;
-        l_run *= alpha;
-#pragma unroll
-        for (int n = 0; n < kDims; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
-        const float m_use = m_run == -INFINITY ? 0.f : m_run;
-        ps = 0.f;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float p = __builtin_amdgcn_exp2f(sc[b][r] - m_use);  // 0 where masked
-            pa[b][r / 8][r % 8] = static_cast<typename T::elem>(p);
-            ps += p;
-          }
-      }
-      l_run += ps;
-      // O^T += V^T P^T: k-slots 8 g + 0..3 of 16-key group m are keys 16 m + 4 g +
-      // 0..3, slots 8 g + 4..7 the keys 8 further, the order of the score rows
-      auto read_v = [&](int m, int n) {
-        union {
-          s16x4 half[2];
-          u32x4 w;
-        } u;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          u.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(
-              stage_base + ((cur + v_rd) ^ (n << 6) ^ (x << 5)) + (16 * m + 8 * x) * kRow));
-        if (key0 + kKeys > kend) {  // (uniform) keys that nobody sees may hold anything
-          const int left = kend - key0 - 16 * m - 4 * g;
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const int j = 8 * (d / 2) + 2 * (d % 2);
-            u.w[d] &= (j < left ? 0xFFFFu : 0u) | (j + 1 < left ? 0xFFFF0000u : 0u);
-          }
-        }
-        return u.w;
-      };
-      if (careful && masked) {
-        const uint32_t one = F16 ? 0x3C00u : 0x3F80u;
+    for (int r = 0; r < 16; ++r) check = fmaf(acc[d][r], 0.f, check);
+  if (__syncthreads_or(check != 0.f)) {
+    reset();
+    start_walk();
 #pragma unroll 1
-        for (int m = 0; m < 4; ++m) {
-          u32x4 seen;  // 1 where the lane's row sees the key of the slot
-          vec p;
+    for (int t = t0; t < t1; ++t) {
+      const Place place = look_up(t);
+      issue(t, place, false, 0);
+      issue(t, place, true, kV);
+      landed();
+      barrier();
+      if (t < tw) {
+        const int key0 = t * kKeys;
+        floatx16 sc[2];
+        u32x4 pa[4];
+        float ps;
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const int j = 16 * m + 8 * (d / 2) + 2 * (d % 2);
-            seen[d] = (j <= last ? one : 0u) | (j + 1 <= last ? one << 16 : 0u);
-          }
-          p = m == 0 ? pa[0][0] : m == 1 ? pa[0][1] : m == 2 ? pa[1][0] : pa[1][1];
+        for (int i = 0; i < kPairs; ++i) scores_step(i % kSteps, read_k(0, i), sc[i / kSteps]);
+        settle(key0, sc, pa, ps);
+        l_run += ps;
+        if (key0 + kKeys - 1 <= wpos0) {
 #pragma unroll
-          for (int n = 0; n < kDims; ++n) {
-            const u32x4 v = read_v(m, n);
-            u32x4 clean;
+          for (int i = 0; i < kPairs; ++i) output_step(i, read_v(kV, i), pa);
+        } else {
+          constexpr uint32_t kOne = F16 ? 0x3C00u : 0x3F80u;
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const u32x4 w = read_v_end(kV, i, key0);
+            const int last = pos - key0 - 4 * g - 16 * (i / kDims);
+            u32x4 clean, seen;  // seen: 1 where the lane's row sees the key of the slot
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-              const bool lo = (v[d] & T::kInf) == T::kInf, up = ((v[d] >> 16) & T::kInf) == T::kInf;
-              clean[d] = v[d] & ((lo ? 0u : 0xFFFFu) | (up ? 0u : 0xFFFF0000u));
+              const bool lo = (w[d] & T::kInf) == T::kInf, up = ((w[d] >> 16) & T::kInf) == T::kInf;
+              const int j = 8 * (d / 2) + 2 * (d % 2);
+              clean[d] = w[d] & ((lo ? 0u : 0xFFFFu) | (up ? 0u : 0xFFFF0000u));
+              seen[d] = (j <= last ? kOne : 0u) | (j + 1 <= last ? kOne << 16 : 0u);
             }
-            acc[n] = T::mfma(__builtin_bit_cast(vec, clean), p, acc[n]);
+            output_step(i, clean, pa);
 #pragma unroll 1
-            for (int kind = 0; kind < 3; ++kind) {  // infinities of either sign, NaN
+            for (int kind = 0; kind < 3; ++kind) {  // infinities of either sign, NaN: how many of them a row sees
+              const uint32_t signs = kind == 2 ? 0x7FFFu : 0xFFFFu;
               u32x4 is;
 #pragma unroll
               for (int d = 0; d < 4; ++d) {
                 is[d] = 0;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                  const uint32_t e = (v[d] >> (16 * half)) & 0xFFFFu;
-                  const bool hit = kind == 2 ? (e & 0x7FFFu) > T::kInf : e == (T::kInf | (kind == 1 ? 0x8000u : 0u));
-                  is[d] |= (hit ? one : 0u) << (16 * half);
+                for (int up = 0; up < 2; ++up) {
+                  const uint32_t e = (w[d] >> (16 * up)) & signs;
+                  const bool hit = kind == 2 ? e > T::kInf : e == (T::kInf | (kind == 1 ? 0x8000u : 0u));
+                  is[d] |= (hit ? kOne : 0u) << (16 * up);
                 }
               }
+              const float what = kind == 2 ? __uint_as_float(0x7FC00000u) : kind == 1 ? -INFINITY : INFINITY;
               floatx16 count;
 #pragma unroll
               for (int r = 0; r < 16; ++r) count[r] = 0.f;
               count = T::mfma(__builtin_bit_cast(vec, is), __builtin_bit_cast(vec, seen), count);
-              const float what = kind == 2 ? __uint_as_float(0x7FC00000u) : kind == 1 ? -INFINITY : INFINITY;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) acc[n][r] = count[r] > 0.f ? acc[n][r] + what : acc[n][r];
+              for (int r = 0; r < 16; ++r) acc[i % kDims][r] = count[r] > 0.f ? acc[i % kDims][r] + what : acc[i % kDims][r];
             }
           }
         }
-      } else {
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-          for (int n = 0; n < kDims; ++n)
-            acc[n] = T::mfma(__builtin_bit_cast(vec, read_v(m, n)), pa[m / 2][m % 2], acc[n]);
       }
+      barrier();
     }
-    float check = 0.f;  // no finite number if one of them is none
-#pragma unroll
-    for (int n = 0; n < kDims; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) check = fmaf(acc[n][r], 0.f, check);
-    if (careful || !__syncthreads_or(check != 0.f)) break;
   }
 
   // ---- epilogue
   const auto lsw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
   const float l_tot = __uint_as_float(lsw[0]) + __uint_as_float(lsw[1]);
-  if (!colv) return;
+  int tok, head;
+  if (!row_at(tok, head)) return;
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // (a NaN sum makes the row NaN)
   uint16_t* dst = a.out + static_cast<int64_t>(qs + tok) * a.o_st + static_cast<int64_t>(head) * a.o_sh + 4 * g;
 #pragma unroll
-  for (int n = 0; n < kDims; ++n)
+  for (int d = 0; d < kDims; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = acc[n][4 * i + j] * inv;
-        o[j] = F16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x);
-      }
-      *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) = u32x2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
-    }
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<u32x2*>(dst + 32 * d + 8 * i) =
+          u32x2{pack<F16>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv), pack<F16>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
 }
 
 template <bool F16, int D, int SRC>
