@@ -345,6 +345,9 @@ int prism_paged_prefill(const void* q, int q_dtype, const int64_t q_strides[3], 
  */
 int64_t prism_paged_prefill_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads, int page_size,
                                             int width);
+/* The same for 16-bit caches, whose scratch is 256-byte aligned. */
+int64_t prism_paged_prefill_16bit_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads, int head_dim,
+                                                  int page_size, int width);
 
 int prism_paged_prefill_ws(const void* q, int q_dtype, const int64_t q_strides[3], const void* k_cache,
                            const void* v_cache, int cache_dtype, const int64_t k_strides[4],
@@ -376,11 +379,19 @@ int prism_paged_prefill_ws(const void* q, int q_dtype, const int64_t q_strides[3
  *              Rows that see no key, and rows outside [cu_seqlens_q[0],
  *              cu_seqlens_q[batch]), are 0.  A sequence whose offsets are out of
  *              order or outside the tensors is left out, its rows unspecified.
+ * workspace  : device scratch (256-byte aligned, any contents) of at least
+ *              prism_prompt_attention_workspace_bytes() bytes for the same
+ *              geometry, which is 0 where none is used.  With it the keys of few,
+ *              long blocks of rows are split over several workgroups; with less,
+ *              or NULL, every block is one workgroup's.
  */
+int64_t prism_prompt_attention_workspace_bytes(int batch, int total_q, int total_k, int num_heads, int num_kv_heads,
+                                               int head_dim);
 int prism_prompt_attention(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
                            const void* v, const int64_t v_strides[3], int dtype, const int32_t* cu_seqlens_q,
                            const int32_t* cu_seqlens_k, void* out, const int64_t out_strides[3], int batch, int total_q,
-                           int total_k, int num_heads, int num_kv_heads, int head_dim, float scale, void* stream);
+                           int total_k, int num_heads, int num_kv_heads, int head_dim, float scale, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /*
  * A step's metadata from the requests' lengths, on the device (the reference

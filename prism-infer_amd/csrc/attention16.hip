@@ -38,6 +38,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kKeys = 64;              // keys per tile
 constexpr int kWaves = 4;              // per workgroup
+constexpr int kMostKeys = 0x7FFFF000;  // of a sequence: positions a few tiles further fit in 32 bits
 constexpr int kCols = 32;              // rows per wave: the columns of a 32x32 MFMA
 constexpr float kSumLimit = 256.0f;    // largest sum of a lane's 32 weights that keeps the running max
 
@@ -62,6 +63,31 @@ struct AttnArgs {
   float scale_log2;
   int* status;
   int* report;  // pinned: [0] set to 1 where a sequence is flagged, [1] and [2] the packed rows' extent; or null
+  int slots;      // workgroups that the chip holds at once
+  uint8_t* work;  // scratch of split blocks (SplitScratch), or null: no block is split
+};
+
+// A block whose keys are split: its rows, and where its parts are.
+struct SplitBlock {
+  int qs, row0, rows, head, slot, parts;
+};
+
+// Scratch of split blocks: how many there are, their descriptions, then the
+// parts by slot, kRows rows of fp32 outputs (unnormalised) and (max, sum).
+constexpr int kBlockRows = kCols * kWaves;
+struct SplitScratch {
+  int* count;
+  SplitBlock* blocks;
+  float* out;
+  float* ml;
+  __host__ __device__ SplitScratch(uint8_t* p, int slots, int dim) {
+    count = reinterpret_cast<int*>(p);
+    blocks = reinterpret_cast<SplitBlock*>(p + 256);
+    out = reinterpret_cast<float*>(p + blocks_end(slots));
+    ml = out + static_cast<int64_t>(slots) * kBlockRows * dim;
+  }
+  static __host__ __device__ int64_t blocks_end(int slots) { return 256 + (static_cast<int64_t>(slots) * sizeof(SplitBlock) + 255) / 256 * 256; }
+  static int64_t bytes(int slots, int dim) { return blocks_end(slots) + static_cast<int64_t>(slots) * kBlockRows * (dim + 2) * 4; }
 };
 
 template <bool F16>
@@ -146,77 +172,192 @@ __device__ __forceinline__ bool sequence(const AttnArgs& a, int i, Seq& s) {
     s.klen = a.ctx[i];
     ok = ok && q1 > q0 && s.klen >= s.qlen && s.klen <= static_cast<int64_t>(a.width) * a.page;
   }
-  return ok;
+  return ok && s.klen <= kMostKeys;
 }
 
-// Blocks of sequence i, and the level of its first: block j ends after about
-// (level + j) kRows / G keys.
-template <int SRC, int ROWS>
-__device__ __forceinline__ int seq_blocks(const AttnArgs& a, int i, bool flag, int& level0) {
-  Seq s;
-  level0 = 1;
-  if (!sequence<SRC>(a, i, s)) {
-    if (SRC != kPacked && flag) flag_sequence(a, i);
-    return 0;
-  }
-  level0 += static_cast<int>(static_cast<int64_t>(max(s.klen - s.qlen, 0)) * a.group / ROWS);
-  return (s.qlen * a.group + ROWS - 1) / ROWS;
-}
+constexpr int kMinPart = 4;  // tiles
+
+// Time of a launch, in units of 64 ns, whose longest block or part walks `tiles`
+// tiles; `parts` workgroups' rows are written in fp32 and merged by a second launch.
+__device__ inline int split_cost(int tiles, int parts) { return tiles * 16 + (parts > 0 ? 60 + parts / 16 : 0); }
 
 struct Work {
-  int seq, block, head, total;
+  int seq, block, head;
+  int part, parts;     // of the block's keys
+  int total;           // workgroups of one kv head
+  int split;           // 0, or its blocks where some are split: then
+  int index, slot;     // the block's number among them, and its first part's among all parts
+  Seq s;
 };
 
-// Workgroup -> (sequence, block, kv head), the blocks with most keys first, so
-// that the launch ends on short ones; heads fastest, so that with 8 kv heads
-// each XCD reads one head's K/V.  A binary search over levels finds the
-// rank's level, a scan over the sequences with a block there its sequence.
+// Workgroup -> its work, heads fastest, so that with 8 kv heads each XCD reads
+// one head's K/V.  K sequences per lane, all in registers, for batches of up to
+// 64 K: one load of the offsets, then wave reductions.
+//
+// Blocks with most keys go first, so that the launch ends on short ones: block j
+// of a sequence ends after about (level + j) ROWS / G keys, a binary search over
+// levels finds the rank's level, a scan over the sequences with a block there
+// its sequence.
+//
+// Where blocks are few and long their keys are split: into parts of the fewest
+// tiles for which all parts fit the chip at once, if that pays.
 // Returns false for a workgroup beyond the real blocks.
+template <int SRC, int ROWS, int K>
+__device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
+  const int lane = __lane_id();
+  int rank = uniform_int(static_cast<int>(blockIdx.x) / a.kv_heads);
+  w.head = static_cast<int>(blockIdx.x) - rank * a.kv_heads;
+  w.part = w.split = 0;
+  w.parts = 1;
+  Seq s[K];
+  int n[K], l0[K], blocks = 0, top = 0, longest = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = lane * K + k;
+    n[k] = 0;
+    l0[k] = 1;
+    s[k] = Seq{0, 0, 0, 0};
+    if (i < a.batch) {
+      if (sequence<SRC>(a, i, s[k])) {
+        l0[k] += static_cast<int>(min(static_cast<int64_t>(max(s[k].klen - s[k].qlen, 0)) * a.group / ROWS, static_cast<int64_t>(1 << 29)));
+        n[k] = (s[k].qlen * a.group + ROWS - 1) / ROWS;
+      } else if (SRC != kPacked && flag) {
+        flag_sequence(a, i);
+      }
+    }
+    blocks += n[k];
+    top = max(top, n[k] == 0 ? 0 : l0[k] + n[k]);
+    longest = max(longest, n[k] == 0 ? 0 : (s[k].klen - 1) / kKeys + 1);
+  }
+  w.total = wave_reduce(blocks, Add());
+  top = wave_reduce(top, Max());
+  int hit_k = 0, l = 0;
+  // parts of a sequence's blocks (more than the chip holds: any number)
+  auto parts_of = [&](int klen, int tiles) {
+    const int part = (klen - 1) / kKeys / tiles + 1;
+    return min(max(part, 1), 1 << 16);
+  };
+  auto total_parts = [&](int tiles) {
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) sum += n[k] * parts_of(s[k].klen, tiles);
+    return wave_reduce(sum, Add());
+  };
+  int tiles = 0;  // of a part
+  const int room = a.slots / a.kv_heads;
+  if (a.work != nullptr && w.total > 0 && w.total < room) {
+    longest = wave_reduce(longest, Max());
+    int lo = kMinPart, hi = max(longest, kMinPart);
+    while (lo < hi) {  // fewest tiles for which the parts fit
+      const int mid = (lo + hi) / 2;
+      if (total_parts(mid) <= room) hi = mid;
+      else lo = mid + 1;
+    }
+    const int all = total_parts(lo);
+    if (all > w.total && split_cost(lo, all * a.kv_heads) < split_cost(longest, 0)) tiles = lo;
+    if (tiles > 0) {
+      w.split = w.total;
+      w.total = all;
+      if (rank >= all) return false;
+      int mine = 0, before = 0;  // parts and blocks of the lane's sequences
+#pragma unroll
+      for (int k = 0; k < K; ++k) mine += n[k] * parts_of(s[k].klen, tiles);
+      const int incl = wave_scan(mine, Add()), incl_blocks = wave_scan(blocks, Add());
+      l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > rank));
+      rank -= uniform_int(__builtin_amdgcn_readlane(incl - mine, l));
+      int slot = __builtin_amdgcn_readlane(incl - mine, l);
+      before = __builtin_amdgcn_readlane(incl_blocks - blocks, l);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int nk = __builtin_amdgcn_readlane(n[k], l);
+        const int parts = parts_of(__builtin_amdgcn_readlane(s[k].klen, l), tiles);
+        if (rank >= 0 && rank < nk * parts) {
+          hit_k = k;
+          w.block = rank / parts;
+          w.part = rank - w.block * parts;
+          w.parts = parts;
+          w.slot = slot + w.block * parts;
+          w.index = before + w.block;
+        }
+        rank -= nk * parts;  // (below 0 once found)
+        slot += nk * parts;
+        before += nk;
+      }
+    }
+  }
+  if (tiles == 0) {
+    if (rank >= w.total) return false;
+    auto above = [&](int u) {
+      int sum = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) sum += min(max(l0[k] + n[k] - 1 - max(u, l0[k] - 1), 0), n[k]);
+      return wave_reduce(sum, Add());
+    };
+    int lo = 0, hi = top;
+    while (lo < hi) {  // smallest level with at most `rank` blocks above it
+      const int mid = (lo + hi) / 2;
+      if (above(mid) <= rank) hi = mid;
+      else lo = mid + 1;
+    }
+    int at = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) at += n[k] > 0 && lo >= l0[k] && lo < l0[k] + n[k] ? 1 : 0;
+    const int left = rank - above(lo), incl = wave_scan(at, Add());
+    l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left));
+    int skip = left - __builtin_amdgcn_readlane(incl - at, l);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int nk = __builtin_amdgcn_readlane(n[k], l), first = __builtin_amdgcn_readlane(l0[k], l);
+      const bool here = nk > 0 && lo >= first && lo < first + nk;
+      if (here && skip == 0) {
+        hit_k = k;
+        w.block = lo - first;
+      }
+      skip -= here;
+    }
+  }
+  w.seq = l * K + hit_k;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (k == hit_k)
+      w.s = Seq{__builtin_amdgcn_readlane(s[k].q0, l), __builtin_amdgcn_readlane(s[k].qlen, l),
+                __builtin_amdgcn_readlane(s[k].k0, l), __builtin_amdgcn_readlane(s[k].klen, l)};
+  return true;
+}
+
+// Larger batches: sequence by sequence, in reverse, nothing split.
 template <int SRC, int ROWS>
-__device__ bool locate(const AttnArgs& a, bool flag, Work& w) {
+__device__ __forceinline__ bool locate_many(const AttnArgs& a, bool flag, Work& w) {
   const int lane = __lane_id();
   const int rank = uniform_int(static_cast<int>(blockIdx.x) / a.kv_heads);
   w.head = static_cast<int>(blockIdx.x) - rank * a.kv_heads;
-  int total = 0, hi = 0, l0;
-  for (int base = 0; base < a.batch; base += 64) {
-    const int i = base + lane;
-    const int n = i < a.batch ? seq_blocks<SRC, ROWS>(a, i, flag, l0) : 0;
-    total += wave_reduce(n, Add());
-    hi = max(hi, wave_reduce(n == 0 ? 0 : l0 + n, Max()));
-  }
-  w.total = total;
-  if (rank >= total) return false;
-  if (a.batch <= 64) {
-    const int n = lane < a.batch ? seq_blocks<SRC, ROWS>(a, lane, false, l0) : 0;
-    auto above = [&](int u) { return min(max(l0 + n - 1 - max(u, l0 - 1), 0), n); };
-    int lo = 0;
-    while (lo < hi) {  // smallest level with at most `rank` blocks above it
-      const int mid = (lo + hi) / 2;
-      if (wave_reduce(above(mid), Add()) <= rank) hi = mid;
-      else lo = mid + 1;
-    }
-    const int at = (n > 0 && lo >= l0 && lo < l0 + n) ? 1 : 0;
-    const int incl = wave_scan(at, Add()) + wave_reduce(above(lo), Add());
-    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(at && incl == rank + 1));
-    w.seq = uniform_int(l);
-    w.block = lo - uniform_int(__shfl(l0, l));
-    return true;
-  }
-  // larger batches: sequence by sequence, in reverse
-  const int target = total - 1 - rank;
+  w.part = w.split = 0;
+  w.parts = 1;
+  auto blocks_of = [&](int i, Seq& s, bool report) {
+    if (i >= a.batch) return 0;
+    if (sequence<SRC>(a, i, s)) return (s.qlen * a.group + ROWS - 1) / ROWS;
+    if (SRC != kPacked && report) flag_sequence(a, i);
+    return 0;
+  };
+  w.total = 0;
+  Seq s;
+  for (int base = 0; base < a.batch; base += 64) w.total += wave_reduce(blocks_of(base + lane, s, flag), Add());
+  const int target = w.total - 1 - rank;
+  if (target < 0) return false;
   int before = 0;
   for (int base = 0; base < a.batch; base += 64) {
-    const int i = base + lane;
-    const int n = i < a.batch ? seq_blocks<SRC, ROWS>(a, i, false, l0) : 0;
+    const int n = blocks_of(base + lane, s, false);
     const int incl = wave_scan(n, Add()) + before;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(i < a.batch && target < incl && target >= incl - n);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(target < incl && target >= incl - n);
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
-      w.seq = uniform_int(base + l);
-      w.block = uniform_int(target - (__shfl(incl, l) - __shfl(n, l)));
+      w.seq = base + l;
+      w.block = target - __builtin_amdgcn_readlane(incl - n, l);
+      w.s = Seq{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.qlen, l), __builtin_amdgcn_readlane(s.k0, l),
+                __builtin_amdgcn_readlane(s.klen, l)};
       return true;
     }
-    before = __shfl(incl, 63);
+    before = __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
 }
@@ -261,7 +402,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 attention16_kernel(const AttnArgs a) {
   using T = Type<F16>;
   typedef typename T::vec vec;
-  constexpr int kRows = kCols * kWaves;
+  constexpr int kRows = kBlockRows;
   constexpr int kRow = D * 2;                 // bytes of a key's row in LDS
   constexpr int kPayload = kKeys * kRow;      // a tile's K or V
   constexpr int kSteps = D / 16;              // MFMAs per 32 x 32 scores
@@ -273,10 +414,15 @@ attention16_kernel(const AttnArgs a) {
   __shared__ __attribute__((aligned(256))) uint8_t lds[4 * kPayload];
 
   Work work;
-  const bool found = locate<SRC, kRows>(a, blockIdx.x == 0 && threadIdx.x < 64, work);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && a.report != nullptr) {
-    a.report[1] = a.cu_q[0];
-    a.report[2] = a.cu_q[a.batch];
+  const bool first_wave = blockIdx.x == 0 && threadIdx.x < 64;  // flags sequences
+  const bool found = a.batch <= 64 ? locate<SRC, kRows, 1>(a, first_wave, work)
+                     : a.batch <= 256 ? locate<SRC, kRows, 4>(a, first_wave, work) : locate_many<SRC, kRows>(a, first_wave, work);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (a.report != nullptr) {
+      a.report[1] = a.cu_q[0];
+      a.report[2] = a.cu_q[a.batch];
+    }
+    if (a.work != nullptr) *SplitScratch(a.work, a.slots, D).count = work.split * a.kv_heads;
   }
   if (!found) {
     if (SRC == kPacked) zero_padding<D>(a, work.total);
@@ -289,8 +435,7 @@ attention16_kernel(const AttnArgs a) {
   const int c = lane % 32;
   const int g = lane / 32;
 
-  Seq s;
-  sequence<SRC>(a, seq, s);
+  const Seq s = work.s;
   const int qs = uniform_int(s.q0), qlen = uniform_int(s.qlen), klen = uniform_int(s.klen);
   const int prefix = klen - qlen;
   const int rows = qlen * a.group;
@@ -298,8 +443,12 @@ attention16_kernel(const AttnArgs a) {
   const int kend = min(klen, prefix + uniform_int((min((block + 1) * kRows, rows) - 1) / a.group) + 1);  // keys [0, kend) are needed
   const int wpos0 = prefix + uniform_int(row0 / a.group);                      // position of the wave's first row
   const int wlast = row0 < rows ? prefix + uniform_int((min(row0 + kCols, rows) - 1) / a.group) : -1;  // and of its last
-  const int t0 = 0, t1 = kend > 0 ? (kend + kKeys - 1) / kKeys : 0;           // the workgroup's tiles
-  const int tw = wlast >= 0 ? min(t1, wlast / kKeys + 1) : 0;                  // the wave's end
+  // the workgroup's tiles, and the wave's end
+  const int part = uniform_int(work.part), parts = uniform_int(work.parts);
+  const int all_tiles = kend > 0 ? (kend - 1) / kKeys + 1 : 0;
+  const int t0 = uniform_int(static_cast<int>(static_cast<int64_t>(all_tiles) * part / parts));
+  const int t1 = uniform_int(static_cast<int>(static_cast<int64_t>(all_tiles) * (part + 1) / parts));
+  const int tw = wlast >= 0 ? min(t1, wlast / kKeys + 1) : 0;
 
   // the lane's row: column c
   auto row_at = [&](int& tok, int& head) {
@@ -521,6 +670,7 @@ attention16_kernel(const AttnArgs a) {
       start_walk();
       place[0] = look_up(t0);
       issue(t0, place[0], false, 0);
+      issue(t0, place[0], true, kV + kPayload);
       if (t0 + 1 < t1) {
         place[1] = look_up(t0 + 1);
         issue(t0 + 1, place[1], false, kPayload);
@@ -595,7 +745,7 @@ attention16_kernel(const AttnArgs a) {
         place[2] = look_up(t + 2);
         issue(t + 2, place[2], false, k_next ^ kPayload);
       }
-      if (t < t1) issue(t, place[0], true, v_prev ^ kPayload);
+      if (t > t0 && t < t1) issue(t, place[0], true, v_prev ^ kPayload);  // (the first is under way)
       place[0] = place[1];
       place[1] = place[2];
     };
@@ -716,7 +866,25 @@ attention16_kernel(const AttnArgs a) {
   const auto lsw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
   const float l_tot = __uint_as_float(lsw[0]) + __uint_as_float(lsw[1]);
   int tok, head;
-  if (!row_at(tok, head)) return;
+  const bool real = row_at(tok, head);
+  if (work.split > 0 && part == 0 && tid == 0)  // (a block of one part: no rows to join)
+    SplitScratch(a.work, a.slots, D).blocks[work.index * a.kv_heads + h] =
+        SplitBlock{qs, block * kRows, parts > 1 ? rows : 0, h, work.slot * a.kv_heads + h, parts};
+  if (parts > 1) {
+    const SplitScratch scratch(a.work, a.slots, D);
+    if (!real) return;
+    const int64_t cell = (static_cast<int64_t>(work.slot + part) * a.kv_heads + h) * kRows + wave * kCols + c;
+    float* dst = scratch.out + cell * D + 4 * g;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<floatx4*>(dst + 32 * d + 8 * i) =
+            floatx4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+    if (g == 0) *reinterpret_cast<floatx2*>(scratch.ml + 2 * cell) = floatx2{m_run, l_tot};
+    return;
+  }
+  if (!real) return;
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // (a NaN sum makes the row NaN)
   uint16_t* dst = a.out + static_cast<int64_t>(qs + tok) * a.o_st + static_cast<int64_t>(head) * a.o_sh + 4 * g;
 #pragma unroll
@@ -727,17 +895,72 @@ attention16_kernel(const AttnArgs a) {
           u32x2{pack<F16>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv), pack<F16>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
 }
 
+// Joins the parts of split blocks: eight rows of a block and kv head per
+// workgroup, 32 lanes each.
+template <bool F16, int D>
+__global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a) {
+  constexpr int kPer = D / 32;
+  const SplitScratch scratch(a.work, a.slots, D);
+  const int index = static_cast<int>(blockIdx.x) / (kBlockRows / 8);
+  if (index >= *scratch.count) return;
+  const SplitBlock b = scratch.blocks[index];
+  const int r = static_cast<int>(blockIdx.x) % (kBlockRows / 8) * 8 + threadIdx.x / 32, row = b.row0 + r;
+  if (row >= b.rows) return;
+  const int64_t step = static_cast<int64_t>(a.kv_heads) * kBlockRows;  // from part to part
+  const int64_t cell = static_cast<int64_t>(b.slot) * kBlockRows + r;
+  const floatx2* ml = reinterpret_cast<const floatx2*>(scratch.ml) + cell;
+  // Parts without a visible key hold zeros and weigh nothing; a NaN sum goes
+  // through whatever its part's weight is.
+  float m = -INFINITY;
+  for (int p = 0; p < b.parts; ++p) {
+    const floatx2 x = ml[p * step];
+    m = x[1] != 0.f ? fmaxf(m, x[0]) : m;
+  }
+  const int lane = threadIdx.x % 32;
+  const float* src = scratch.out + cell * D + lane * kPer;
+  float l = 0.f, o[kPer] = {};
+#pragma unroll 2
+  for (int p = 0; p < b.parts; ++p) {
+    const floatx2 x = ml[p * step];
+    const float w = x[1] != 0.f ? __builtin_amdgcn_exp2f(x[0] - m) : 0.f;
+    l = fmaf(w, x[1], l);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) o[j] = fmaf(w, src[p * step * D + j], o[j]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int tok = row / a.group, head = b.head * a.group + (row - tok * a.group);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(b.qs + tok) * a.o_st +
+                                              static_cast<int64_t>(head) * a.o_sh + lane * kPer);
+#pragma unroll
+  for (int j = 0; j < kPer; j += 2) dst[j / 2] = pack<F16>(o[j] * inv, o[j + 1] * inv);
+}
+
+// The chip holds two workgroups per CU (registers, LDS).
+int chip_slots() { return 2 * device_cu_count(); }
+
+// Whether blocks may be split: the fewest blocks that the rows make leave room for
+// parts, and the longest context could be more than one of them.
+bool may_split(int batch, int64_t total_q, int heads, int kv_heads, int64_t most_keys) {
+  const int64_t least = std::max<int64_t>(ceil_div(total_q * (heads / kv_heads), kBlockRows), 1) * kv_heads;
+  return batch <= 256 && 2 * least <= chip_slots() && most_keys > 2 * kMinPart * kKeys;
+}
+
 template <bool F16, int D, int SRC>
 int launch(const AttnArgs& a, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.total_q) * a.group;
   // every sequence may end in a partial block; one more for rows outside them
   const int64_t blocks = (ceil_div(rows, kCols * kWaves) + a.batch + 1) * a.kv_heads;
-  if (blocks > INT32_MAX || rows > INT32_MAX) {
+  if (blocks > INT32_MAX || rows > INT32_MAX - kBlockRows) {
     set_error("attention over 16-bit keys: too many query rows for one launch");
     return PRISM_ERR_INVALID;
   }
-  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, stream, a);
-  return check_launch("attention16_kernel launch");
+  const int64_t grid = a.work == nullptr ? blocks : std::max<int64_t>(blocks, a.slots + a.kv_heads);  // (parts never outnumber the slots)
+  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves), 0, stream, a);
+  if (int rc = check_launch("attention16_kernel launch")) return rc;
+  if (a.work == nullptr) return PRISM_OK;
+  const int64_t split = std::min<int64_t>(blocks, a.slots) * (kBlockRows / 8);
+  hipLaunchKernelGGL((attention16_join_kernel<F16, D>), dim3(static_cast<unsigned>(split)), dim3(256), 0, stream, a);
+  return check_launch("attention16_join_kernel launch");
 }
 
 template <bool F16, int D>
@@ -746,7 +969,15 @@ int by_source(const AttnArgs& a, hipStream_t stream) {
   return a.page % kKeys == 0 ? launch<F16, D, kPages>(a, stream) : launch<F16, D, kSmallPages>(a, stream);
 }
 
-int dispatch(const AttnArgs& a, int dtype, int head_dim, hipStream_t stream) {
+int64_t scratch_bytes(int batch, int64_t total_q, int heads, int kv_heads, int head_dim, int64_t most_keys) {
+  return may_split(batch, total_q, heads, kv_heads, most_keys) ? SplitScratch::bytes(chip_slots(), head_dim) : 0;
+}
+
+// Without scratch for the parts no block is split.
+int dispatch(AttnArgs a, int dtype, int head_dim, int64_t most_keys, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  a.slots = chip_slots();
+  const int64_t need = scratch_bytes(a.batch, a.total_q, a.heads, a.kv_heads, head_dim, most_keys);
+  a.work = need > 0 && workspace != nullptr && aligned(workspace, 256) && workspace_bytes >= need ? static_cast<uint8_t*>(workspace) : nullptr;
   if (dtype == PRISM_DTYPE_F16) return head_dim == 128 ? by_source<true, 128>(a, stream) : by_source<true, 64>(a, stream);
   return head_dim == 128 ? by_source<false, 128>(a, stream) : by_source<false, 64>(a, stream);
 }
@@ -795,7 +1026,8 @@ int preload_attention16() {
 int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void* v, int dtype, const int64_t* ks,
                     const int64_t* vs, const int32_t* bt, const int64_t* bts, const int32_t* ctx, const int32_t* cu_q,
                     void* out, const int64_t* os, int batch, int total_q, int heads, int kv_heads, int head_dim, int page,
-                    int num_blocks, int width, float scale, int32_t* status, int32_t* report, hipStream_t stream) {
+                    int num_blocks, int width, float scale, int32_t* status, void* workspace, int64_t workspace_bytes,
+                    int32_t* report, hipStream_t stream) {
   if (int rc = check_layout("prism_paged_prefill", dtype, heads, kv_heads, head_dim, q, qs, k, ks, v, vs, 4, out, os)) return rc;
   if (page % 16 != 0) {
     set_error("prism_paged_prefill: page size must be a multiple of 16, got %d", page);
@@ -819,16 +1051,32 @@ int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void*
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status;
   a.report = report;
-  return dispatch(a, dtype, head_dim, stream);
+  return dispatch(a, dtype, head_dim, static_cast<int64_t>(width) * page, workspace, workspace_bytes, stream);
 }
 
 }  // namespace prism
+
+extern "C" int64_t prism_prompt_attention_workspace_bytes(int batch, int total_q, int total_k, int num_heads,
+                                                          int num_kv_heads, int head_dim) {
+  if (batch <= 0 || total_q <= 0 || total_k <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      head_dim <= 0)
+    return 0;
+  return prism::scratch_bytes(batch, total_q, num_heads, num_kv_heads, head_dim, total_k);
+}
+
+extern "C" int64_t prism_paged_prefill_16bit_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads,
+                                                             int head_dim, int page_size, int width) {
+  if (batch <= 0 || total_q <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
+      page_size <= 0 || width <= 0)
+    return 0;
+  return prism::scratch_bytes(batch, total_q, num_heads, num_kv_heads, head_dim, static_cast<int64_t>(width) * page_size);
+}
 
 extern "C" int prism_prompt_attention(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
                                       const void* v, const int64_t v_strides[3], int dtype, const int32_t* cu_seqlens_q,
                                       const int32_t* cu_seqlens_k, void* out, const int64_t out_strides[3], int batch,
                                       int total_q, int total_k, int num_heads, int num_kv_heads, int head_dim, float scale,
-                                      void* stream) {
+                                      void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace prism;
   clear_error();
   if (batch < 0 || total_q < 0 || total_k < 0) {
@@ -857,5 +1105,5 @@ extern "C" int prism_prompt_attention(const void* q, const int64_t q_strides[3],
   a.batch = batch, a.heads = num_heads, a.kv_heads = num_kv_heads, a.group = num_heads / num_kv_heads;
   a.total_q = total_q, a.total_k = total_k;
   a.scale_log2 = scale * 1.4426950408889634f;
-  return dispatch(a, dtype, head_dim, static_cast<hipStream_t>(stream));
+  return dispatch(a, dtype, head_dim, total_k, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

@@ -945,7 +945,8 @@ int preload_paged_prefill() {
 int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void* v, int dtype, const int64_t* ks,
                     const int64_t* vs, const int32_t* bt, const int64_t* bts, const int32_t* ctx, const int32_t* cu_q,
                     void* out, const int64_t* os, int batch, int total_q, int heads, int kv_heads, int head_dim, int page,
-                    int num_blocks, int width, float scale, int32_t* status, int32_t* report, hipStream_t stream);
+                    int num_blocks, int width, float scale, int32_t* status, void* workspace, int64_t workspace_bytes,
+                    int32_t* report, hipStream_t stream);
 
 }  // namespace prism
 
@@ -988,7 +989,8 @@ extern "C" int prism_paged_prefill_ws(const void* q, int q_dtype, const int64_t 
     }
     return paged_prefill16(q, q_strides, k_cache, v_cache, cache_dtype, k_strides, v_strides, block_tables, bt_strides,
                            context_lens, cu_seqlens_q, out, out_strides, batch, total_q, num_heads, num_kv_heads, head_dim,
-                           page_size, num_blocks, width, scale, status, report, static_cast<hipStream_t>(stream_ptr));
+                           page_size, num_blocks, width, scale, status, workspace, workspace_bytes, report,
+                           static_cast<hipStream_t>(stream_ptr));
   }
   if (num_heads % num_kv_heads != 0 || num_heads / num_kv_heads > kPfMaxWaves) {
     set_error("prism_paged_prefill: num_heads=%d / num_kv_heads=%d must be an integer group of at most %d",

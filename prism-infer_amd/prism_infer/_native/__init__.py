@@ -91,8 +91,10 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "prism_prompt_attention": (
         _I,
-        [_VP, _I64P, _VP, _I64P, _VP, _I64P, _I, _VP, _VP, _VP, _I64P, _I, _I, _I, _I, _I, _I, _F, _VP],
+        [_VP, _I64P, _VP, _I64P, _VP, _I64P, _I, _VP, _VP, _VP, _I64P, _I, _I, _I, _I, _I, _I, _F, _VP, _I64, _VP],
     ),
+    "prism_prompt_attention_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I]),
+    "prism_paged_prefill_16bit_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
     "prism_step_metadata_words": (_I64, [_I, _I, _I]),
     "prism_step_metadata": (_I, [_VP, _I64P, _VP, _VP, _VP, _I, _VP, _I, _I, _I, _I, _VP, _VP]),
     "prism_debug_fp8_encode": (_I, [_VP, _VP, _I64, _VP]),

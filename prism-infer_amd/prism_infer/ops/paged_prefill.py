@@ -195,8 +195,12 @@ def _launch_paged_prefill(q, k_cache, v_cache, context, *, num_heads, num_kv_hea
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     status = torch.full((1,), _STATUS_OK, dtype=torch.int32, device=device)
     # scratch for split keys (static shapes only; 0 bytes where blocks are not split)
-    ws_bytes = lib.prism_paged_prefill_workspace_bytes(batch, q.shape[0], num_heads, num_kv_heads, k_cache.shape[1],
-                                                       block_tables.shape[1])
+    if sixteen:
+        ws_bytes = lib.prism_paged_prefill_16bit_workspace_bytes(batch, q.shape[0], num_heads, num_kv_heads, q.shape[2],
+                                                                 k_cache.shape[1], block_tables.shape[1])
+    else:
+        ws_bytes = lib.prism_paged_prefill_workspace_bytes(batch, q.shape[0], num_heads, num_kv_heads, k_cache.shape[1],
+                                                           block_tables.shape[1])
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 0 else None
     zero3 = _native.int64s(0, 0, 0)
     with torch.cuda.device(device):

@@ -92,11 +92,16 @@ def prompt_attention(
     cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     with torch.cuda.device(q.device):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        batch = cu_seqlens_q.numel() - 1
+        # scratch for split keys (static shapes only; 0 bytes where none are split)
+        ws_bytes = lib.prism_prompt_attention_workspace_bytes(batch, q.shape[0], k.shape[0], num_heads, num_kv_heads, q.shape[2])
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes > 0 else None
         rc = lib.prism_prompt_attention(
             q.data_ptr(), _native.row_strides(q), k.data_ptr(), _native.row_strides(k), v.data_ptr(), _native.row_strides(v),
             _native.dtype_code(q.dtype), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-            out.data_ptr(), _native.strides(out), cu_seqlens_q.numel() - 1, q.shape[0], k.shape[0],
-            num_heads, num_kv_heads, q.shape[2], float(scale), _native.stream_handle(q.device),
+            out.data_ptr(), _native.strides(out), batch, q.shape[0], k.shape[0],
+            num_heads, num_kv_heads, q.shape[2], float(scale),
+            workspace.data_ptr() if workspace is not None else None, ws_bytes, _native.stream_handle(q.device),
         )
     _native.check(rc, "prompt_attention")
     return out

@@ -58,6 +58,52 @@ def test_queries_behind_and_before_their_keys(dtype, dim):
     assert (got[cu_q[1]:cu_q[1] + 30] == 0).all() and (got[cu_q[4]:cu_q[5]] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 128), (BF16, 64), (F16, 64)])
+@pytest.mark.parametrize("batch,heads,kv_heads,longest", [(1, 8, 2, 6000), (5, 8, 1, 3000), (70, 4, 1, 1500), (255, 2, 1, 700)])
+def test_keys_split_over_workgroups(batch, heads, kv_heads, longest, dtype, dim):
+    """Few rows behind many keys, some behind few: blocks of many parts and of one, rows outside, rows without a key."""
+
+    require_gpu()
+    g = torch.Generator().manual_seed(batch)
+    lq = torch.randint(0, 4, (batch,), generator=g).tolist()
+    lk = torch.randint(0, longest, (batch,), generator=g).tolist()
+    lk[-1] = 2
+    lq[0], lk[0] = 3, longest
+    cu_q, cu_k = offsets(lq, start=2), offsets(lk, start=1)
+    q, k, v = _inputs(batch + 1, cu_q[-1] + 5, cu_k[-1] + 3, heads, kv_heads, dim, dtype)
+    got = _check(q, k, v, cu_q, cu_k)
+    assert (got[:2] == 0).all() and (got[cu_q[-1]:] == 0).all()
+    # values that are no numbers, in a part that others do not see
+    v[cu_k[1] - 1, 0, 3] = float("nan")
+    v[cu_k[0] + 40, 0, 5] = float("inf")
+    _check(q, k, v, cu_q, cu_k)
+
+
+def test_split_is_the_same_in_a_captured_graph():
+    require_gpu()
+    from prism_infer.ops.prompt_attention import prompt_attention
+
+    q, k, v = (x.cuda() for x in _inputs(21, 12, 9000, 8, 2, 128, BF16))
+    cu_q = torch.tensor([0, 5, 12], dtype=torch.int32, device="cuda")
+    cu_k = torch.tensor([0, 6000, 9000], dtype=torch.int32, device="cuda")
+
+    def call():
+        return prompt_attention(q, k, v, cu_q, num_heads=8, num_kv_heads=2, scale=0.1, cu_seqlens_k=cu_k)
+
+    call()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first, second = call(), call()
+    with torch.cuda.graph(other):
+        third = call()
+    for offs in ([0, 6000, 9000], [0, 4, 9000], [0, 9000, 9000], [0, 50, 80]):
+        cu_k.copy_(torch.tensor(offs, dtype=torch.int32))
+        graph.replay()
+        other.replay()
+        want = call()
+        assert torch.equal(first, want) and torch.equal(second, want) and torch.equal(third, want), offs
+
+
 def test_many_short_sequences():
     require_gpu()
     g = torch.Generator().manual_seed(3)

@@ -87,7 +87,7 @@ def test_abi_refuses_before_any_launch():
     def prompt(**kw):
         a = dict(q=p, qs=s3, k=p, ks=s3, v=p, vs=s3, dtype=1, cq=p, ck=p, out=p, os=s3, batch=1, tq=4, tk=4, h=4, hk=4, d=128) | kw
         rc = lib.prism_prompt_attention(a["q"], a["qs"], a["k"], a["ks"], a["v"], a["vs"], a["dtype"], a["cq"], a["ck"], a["out"],
-                                        a["os"], a["batch"], a["tq"], a["tk"], a["h"], a["hk"], a["d"], 0.1, None)
+                                        a["os"], a["batch"], a["tq"], a["tk"], a["h"], a["hk"], a["d"], 0.1, None, 0, None)
         return rc, lib.prism_last_error().decode()
 
     assert prompt(batch=-1)[0] == -1 and prompt(q=None)[0] == -1 and prompt(k=None)[0] == -1 and prompt(cq=None)[0] == -1
