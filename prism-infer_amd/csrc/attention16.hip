@@ -27,7 +27,6 @@
 #include "common.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace prism {
 namespace {
@@ -287,33 +286,30 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
   }
   if (tiles == 0) {
     if (rank >= w.total) return false;
-    auto above = [&](int u) {
-      int sum = 0;
+    if (K > 1 || w.total <= room) {  // all start at once, or many are short: sequence by sequence, in reverse
+      const int left = w.total - 1 - rank, incl = wave_scan(blocks, Add());
+      l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left));
+      w.block = left - __builtin_amdgcn_readlane(incl - blocks, l);
 #pragma unroll
-      for (int k = 0; k < K; ++k) sum += min(max(l0[k] + n[k] - 1 - max(u, l0[k] - 1), 0), n[k]);
-      return wave_reduce(sum, Add());
-    };
+      for (int k = 0; k + 1 < K; ++k) {
+        const int nk = __builtin_amdgcn_readlane(n[k], l);
+        if (hit_k == k && w.block >= nk) {
+          w.block -= nk;
+          hit_k = k + 1;
+        }
+      }
+    } else {
+    auto above = [&](int u) { return wave_reduce(min(max(l0[0] + n[0] - 1 - max(u, l0[0] - 1), 0), n[0]), Add()); };
     int lo = 0, hi = top;
     while (lo < hi) {  // smallest level with at most `rank` blocks above it
       const int mid = (lo + hi) / 2;
       if (above(mid) <= rank) hi = mid;
       else lo = mid + 1;
     }
-    int at = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) at += n[k] > 0 && lo >= l0[k] && lo < l0[k] + n[k] ? 1 : 0;
+    const int at = n[0] > 0 && lo >= l0[0] && lo < l0[0] + n[0] ? 1 : 0;
     const int left = rank - above(lo), incl = wave_scan(at, Add());
     l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left));
-    int skip = left - __builtin_amdgcn_readlane(incl - at, l);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int nk = __builtin_amdgcn_readlane(n[k], l), first = __builtin_amdgcn_readlane(l0[k], l);
-      const bool here = nk > 0 && lo >= first && lo < first + nk;
-      if (here && skip == 0) {
-        hit_k = k;
-        w.block = lo - first;
-      }
-      skip -= here;
+    w.block = lo - __builtin_amdgcn_readlane(l0[0], l);
     }
   }
   w.seq = l * K + hit_k;
@@ -468,6 +464,19 @@ attention16_kernel(const AttnArgs a) {
     for (int x = 0; x < kSteps; ++x)
       qop[x] = __builtin_bit_cast(vec, real ? *reinterpret_cast<const u32x4*>(src + 16 * x) : u32x4{0, 0, 0, 0});
   }
+  // The exponent's scale is positive, so that a masked score is -inf: a negative
+  // one is the queries' sign, and with 0 all queries are 0.
+  const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+  if (a.scale_log2 <= 0.f) {
+    const uint32_t keep = a.scale_log2 == 0.f ? 0u : ~0u;
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      u32x4 w = __builtin_bit_cast(u32x4, qop[x]);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) w[d] = (w[d] & keep) ^ (0x80008000u & keep);
+      qop[x] = __builtin_bit_cast(vec, w);
+    }
+  }
 
   // ---- tile loads, straight into LDS.  A load of a wave covers kLoadRows rows;
   // row and swizzled chunk of a lane do not change from load to load.  Asm so
@@ -612,17 +621,21 @@ attention16_kernel(const AttnArgs a) {
   auto output_step = [&](int pair, const u32x4& v, const u32x4 (&p)[4]) {
     acc[pair % kDims] = T::mfma(__builtin_bit_cast(vec, v), __builtin_bit_cast(vec, p[pair / kDims]), acc[pair % kDims]);
   };
-  // Weights of a tile with their masks: maxima are taken and the accumulators rescaled.
-  auto settle = [&](int key0, const floatx16 (&sc)[2], u32x4 (&pa)[4], float& ps) {
+  // Scores of keys that the lane's row does not see.
+  auto mask = [&](int key0, floatx16 (&sc)[2]) {
     const int last = pos - key0 - 4 * g;  // last visible key, as a row offset of the lane
-    float tmax = -INFINITY;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        tmax = fmaxf(tmax, 32 * b + 8 * (r / 4) + r % 4 <= last ? sc[b][r] * a.scale_log2 : -INFINITY);
+      for (int r = 0; r < 16; ++r) sc[b][r] = 32 * b + 8 * (r / 4) + r % 4 <= last ? sc[b][r] : -INFINITY;
+  };
+  // Weights of a tile against its maxima, which the accumulators are rescaled to.
+  auto settle = [&](const floatx16 (&sc)[2], u32x4 (&pa)[4], float& ps) {
+    float tmax = fmaxf(sc[0][0], sc[1][0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, fmaxf(sc[0][r], sc[1][r]));
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
-    tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale;
     const float m_new = tmax > m_run ? tmax : m_run;
     // (no key seen: keep the accumulators, all zero, from (-inf) - (-inf))
     const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
@@ -634,19 +647,14 @@ attention16_kernel(const AttnArgs a) {
       for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
     ps = 0.f;
-    int seen = last;  // (compared anew: 32 lane masks kept from above would fill the SGPRs)
-    asm("" : "+v"(seen));
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
-        float p[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          p[j] = 32 * b + 8 * (r / 4) + r % 4 + j <= seen
-                     ? __builtin_amdgcn_exp2f(fmaf(sc[b][r + j], a.scale_log2, -m_use)) : 0.f;
-        pa[2 * b + r / 8][r % 8 / 2] = pack<F16>(p[0], p[1]);
-        ps += p[0] + p[1];
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][r], scale, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][r + 1], scale, -m_use));
+        pa[2 * b + r / 8][r % 8 / 2] = pack<F16>(p0, p1);
+        ps += p0 + p1;
       }
   };
   // (a wave meets the others' barriers by their number, wherever in its code it stands)
@@ -684,11 +692,27 @@ attention16_kernel(const AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) scores_step(i % kSteps, read_k(0, i), sa[i / kSteps]);
     }
-    // A wave's tile t: weights pn from scores sc, next scores sn; OUT: whether there
-    // is a tile t - 1, with weights pp.  Past the last tile the scores are taken
-    // from stale bytes, for nothing.
-    auto tile = [&](auto out, int t, floatx16 (&sc)[2], floatx16 (&sn)[2], u32x4 (&pp)[4], u32x4 (&pn)[4]) {
-      constexpr bool OUT = decltype(out)::value;
+    // A wave's first tile: its weights, and the next scores where there is a next tile.
+    auto first_tile = [&](floatx16 (&sc)[2], floatx16 (&sn)[2], u32x4 (&pn)[4]) {
+      if (t0 + 1 < tw) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) scores_step(i % kSteps, read_k(k_next, i), sn[i / kSteps]);
+      }
+      if (t0 * kKeys + kKeys - 1 > wpos0) mask(t0 * kKeys, sc);
+      // (Behind a condition that the compiler cannot see through, as on the other
+      // tiles: without one the loop's registers spill, 80 of them.)
+      int always = 1;
+      asm volatile("" : "+s"(always));
+      float ps = 0.f;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) pn[m] = u32x4{0, 0, 0, 0};
+      if (always) settle(sc, pn, ps);
+      l_run += ps;
+    };
+    // Its tile t: weights pn from scores sc, next scores sn, output of tile t - 1
+    // with weights pp.  Past the last tile the scores are taken from stale bytes,
+    // for nothing.
+    auto tile = [&](int t, floatx16 (&sc)[2], floatx16 (&sn)[2], u32x4 (&pp)[4], u32x4 (&pn)[4]) {
       constexpr int kPerSlot = 16 / kPairs;  // halves of a pair of weights beside an MFMA
       constexpr int kAhead = 1;              // operands are read this many pairs ahead
       uint32_t v_tile = v_prev;
@@ -698,41 +722,41 @@ attention16_kernel(const AttnArgs a) {
       auto half = [&](int i) {
         const int m = i / 8, b = m / 2, r = m % 2 * 8 + i % 8 / 2 * 2;
         if (i % 2 == 0) {
-          e0 = __builtin_amdgcn_exp2f(fmaf(sc[b][r], a.scale_log2, -m_run));
-          x1 = fmaf(sc[b][r + 1], a.scale_log2, -m_run);
+          e0 = __builtin_amdgcn_exp2f(fmaf(sc[b][r], scale, -m_run));
+          x1 = fmaf(sc[b][r + 1], scale, -m_run);
         } else {
           const float e1 = __builtin_amdgcn_exp2f(x1);
           pn[m][r % 8 / 2] = pack<F16>(e0, e1);
           ps += e0 + e1;
         }
       };
+      if (t * kKeys + kKeys - 1 > wpos0) mask(t * kKeys, sc);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         kq[i] = read_k(k_next, i);
-        if (OUT) vq[i] = read_v(v_tile, i);
+        vq[i] = read_v(v_tile, i);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         if (i + kAhead < kPairs) {
           kq[(i + kAhead) % (kAhead + 1)] = read_k(k_next, i + kAhead);
-          if (OUT) vq[(i + kAhead) % (kAhead + 1)] = read_v(v_tile, i + kAhead);
+          vq[(i + kAhead) % (kAhead + 1)] = read_v(v_tile, i + kAhead);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (j == 0) scores_step(i % kSteps, kq[i % (kAhead + 1)], sn[i / kSteps]);
-          else if (OUT) output_step(i, vq[i % (kAhead + 1)], pp);
+          else output_step(i, vq[i % (kAhead + 1)], pp);
 #pragma unroll
           for (int y = 0; y < kPerSlot; ++y) half((2 * i + j) * kPerSlot + y);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
       // The weights were formed against the running max as it stood; their sum tells
-      // whether that was low enough, or is no number.  Only otherwise, and on masked
-      // tiles, are maxima taken.  (The pins keep the weights in front of the branch.)
+      // whether that was low enough, or is no number.  Only otherwise are maxima
+      // taken.  (The pins keep the weights in front of the branch.)
       asm volatile("" : "+v"(ps), "+v"(pn[0]), "+v"(pn[1]), "+v"(pn[2]), "+v"(pn[3]));
-      const int key0 = t * kKeys;
-      if (key0 + kKeys - 1 > wpos0 || __builtin_amdgcn_ballot_w64(!(ps <= kSumLimit)) != 0) settle(key0, sc, pn, ps);
+      if (__builtin_amdgcn_ballot_w64(!(ps <= kSumLimit)) != 0) settle(sc, pn, ps);
       l_run += ps;
     };
     // The step that begins iteration t of every wave: K of tile t + 1 and V of
@@ -757,17 +781,17 @@ attention16_kernel(const AttnArgs a) {
     int t = t0;
     if (t0 < tw) {
       begin(t);
-      tile(std::false_type(), t, sa, sb, pb, pa);
+      first_tile(sa, sb, pa);
       next();
       bool odd = false;
       for (++t; t < tw; ++t) {
         begin(t);
-        tile(std::true_type(), t, sb, sa, pa, pb);
+        tile(t, sb, sa, pa, pb);
         next();
         odd = ++t == tw;
         if (odd) break;
         begin(t);
-        tile(std::true_type(), t, sa, sb, pb, pa);
+        tile(t, sa, sb, pb, pa);
         next();
       }
       if (odd)
@@ -788,77 +812,81 @@ attention16_kernel(const AttnArgs a) {
   }
 
   // A value that is no finite number multiplied by a masked weight's 0 is no
-  // 0.  Where an output is not finite the block is walked once more, one thing
-  // after the other: on masked tiles such values are taken out of the product
-  // and added to the rows that see their key.
+  // 0.  A wave with an output that is not finite walks its tiles once more, one
+  // thing after the other and straight from memory (the others may be done):
+  // such values are taken out of the product and added to the rows that see
+  // their key.
   float check = 0.f;  // no finite number if one of them is none
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) check = fmaf(acc[d][r], 0.f, check);
-  if (__syncthreads_or(check != 0.f)) {
+  if (__builtin_amdgcn_ballot_w64(check != 0.f) != 0 && (SRC == kPacked || a.num_blocks > 0)) {
     reset();
-    start_walk();
+    auto key_row = [&](const uint8_t* head, int64_t page_bytes, int st_bytes, int key) {
+      key = min(key, kend - 1);
+      if constexpr (SRC == kPacked) return head + static_cast<int64_t>(key) * st_bytes;
+      const int page = key / a.page, blk = bt_row[static_cast<int64_t>(page) * a.bt_sn];
+      return head + min(max(blk, 0), a.num_blocks - 1) * page_bytes + static_cast<int64_t>(key - page * a.page) * st_bytes;
+    };
 #pragma unroll 1
-    for (int t = t0; t < t1; ++t) {
-      const Place place = look_up(t);
-      issue(t, place, false, 0);
-      issue(t, place, true, kV);
-      landed();
-      barrier();
-      if (t < tw) {
-        const int key0 = t * kKeys;
-        floatx16 sc[2];
-        u32x4 pa[4];
-        float ps;
+    for (int t = t0; t < tw; ++t) {
+      const int key0 = t * kKeys;
+      floatx16 sc[2];
+      u32x4 pa[4];
+      float ps;
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) scores_step(i % kSteps, read_k(0, i), sc[i / kSteps]);
-        settle(key0, sc, pa, ps);
-        l_run += ps;
-        if (key0 + kKeys - 1 <= wpos0) {
+      for (int b = 0; b < 2; ++b) {
+        const uint8_t* row = key_row(k_head, a.k_sn * 2, k_st, key0 + 32 * b + c) + 16 * g;
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) output_step(i, read_v(kV, i), pa);
-        } else {
-          constexpr uint32_t kOne = F16 ? 0x3C00u : 0x3F80u;
+        for (int x = 0; x < kSteps; ++x) scores_step(x, *reinterpret_cast<const u32x4*>(row + 32 * x), sc[b]);
+      }
+      mask(key0, sc);
+      settle(sc, pa, ps);
+      l_run += ps;
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) {
-            const u32x4 w = read_v_end(kV, i, key0);
-            const int last = pos - key0 - 4 * g - 16 * (i / kDims);
-            u32x4 clean, seen;  // seen: 1 where the lane's row sees the key of the slot
+      for (int m = 0; m < 4; ++m) {
+        const uint8_t* row[8];
+        u32x4 seen;  // 1 where the lane's row sees the key of the slot
+        constexpr uint32_t kOne = F16 ? 0x3C00u : 0x3F80u;
+        const int first = key0 + 16 * m + 4 * g;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              const bool lo = (w[d] & T::kInf) == T::kInf, up = ((w[d] >> 16) & T::kInf) == T::kInf;
-              const int j = 8 * (d / 2) + 2 * (d % 2);
-              clean[d] = w[d] & ((lo ? 0u : 0xFFFFu) | (up ? 0u : 0xFFFF0000u));
-              seen[d] = (j <= last ? kOne : 0u) | (j + 1 <= last ? kOne << 16 : 0u);
-            }
-            output_step(i, clean, pa);
+        for (int j = 0; j < 8; ++j) {
+          const int key = first + 8 * (j / 4) + j % 4;
+          row[j] = key_row(v_head, a.v_sn * 2, v_st, key) + 2 * c;
+          const uint32_t bit = key <= pos ? kOne : 0u;
+          seen[j / 2] = j % 2 ? seen[j / 2] | (bit << 16) : bit;
+        }
+#pragma unroll
+        for (int n = 0; n < kDims; ++n) {
+          u32x4 clean;
+          uint32_t value[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            value[j] = *reinterpret_cast<const uint16_t*>(row[j] + 64 * n);
+            const uint32_t finite = (value[j] & T::kInf) == T::kInf ? 0u : value[j];
+            clean[j / 2] = j % 2 ? clean[j / 2] | (finite << 16) : finite;
+          }
+          output_step(m * kDims + n, clean, pa);
 #pragma unroll 1
-            for (int kind = 0; kind < 3; ++kind) {  // infinities of either sign, NaN: how many of them a row sees
-              const uint32_t signs = kind == 2 ? 0x7FFFu : 0xFFFFu;
-              u32x4 is;
+          for (int kind = 0; kind < 3; ++kind) {  // infinities of either sign, NaN: how many of them a row sees
+            u32x4 is;
 #pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                is[d] = 0;
-#pragma unroll
-                for (int up = 0; up < 2; ++up) {
-                  const uint32_t e = (w[d] >> (16 * up)) & signs;
-                  const bool hit = kind == 2 ? e > T::kInf : e == (T::kInf | (kind == 1 ? 0x8000u : 0u));
-                  is[d] |= (hit ? kOne : 0u) << (16 * up);
-                }
-              }
-              const float what = kind == 2 ? __uint_as_float(0x7FC00000u) : kind == 1 ? -INFINITY : INFINITY;
-              floatx16 count;
-#pragma unroll
-              for (int r = 0; r < 16; ++r) count[r] = 0.f;
-              count = T::mfma(__builtin_bit_cast(vec, is), __builtin_bit_cast(vec, seen), count);
-#pragma unroll
-              for (int r = 0; r < 16; ++r) acc[i % kDims][r] = count[r] > 0.f ? acc[i % kDims][r] + what : acc[i % kDims][r];
+            for (int j = 0; j < 8; ++j) {
+              const bool hit = kind == 2 ? (value[j] & 0x7FFFu) > T::kInf : value[j] == (T::kInf | (kind == 1 ? 0x8000u : 0u));
+              const uint32_t bit = hit ? kOne : 0u;
+              is[j / 2] = j % 2 ? is[j / 2] | (bit << 16) : bit;
             }
+            const float what = kind == 2 ? __uint_as_float(0x7FC00000u) : kind == 1 ? -INFINITY : INFINITY;
+            floatx16 count;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) count[r] = 0.f;
+            count = T::mfma(__builtin_bit_cast(vec, is), __builtin_bit_cast(vec, seen), count);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[n][r] = count[r] > 0.f ? acc[n][r] + what : acc[n][r];
           }
         }
       }
-      barrier();
     }
   }
 
