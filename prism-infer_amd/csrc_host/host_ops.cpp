@@ -1,8 +1,9 @@
 // Host side of the per-layer ops: argument checks and launches without
 // Python in between.
 //
-// store_kvcache, paged_decode_attention and paged_prefill_attention run once
-// per layer and step; checked in Python and bound through ctypes, a call costs
+// store_kvcache, paged_decode_attention, paged_prefill_attention and
+// prompt_attention run once per layer and step, build_step_metadata once per
+// step; checked in Python and bound through ctypes, a call costs
 // the host more than the kernels of a small step take.  These functions do the
 // same checks on the tensors themselves and call the C ABI (one layer's store
 // and decode, B = 1, 1800 tokens: 41.8 us a step in Python, 16.1 here, where
@@ -17,6 +18,7 @@
 
 #include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -153,13 +155,25 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// rows: 0 for leading dimensions of one entry, which may hold any number there.
 struct Strides {
   int64_t v[4];
-  explicit Strides(const at::Tensor* t) : v{0, 0, 0, 0} {
+  explicit Strides(const at::Tensor* t, bool rows = false) : v{0, 0, 0, 0} {
     if (t != nullptr)
-      for (int64_t i = 0; i < t->dim() && i < 4; ++i) v[i] = t->stride(i);
+      for (int64_t i = 0; i < t->dim() && i < 4; ++i) v[i] = rows && i + 1 < t->dim() && t->size(i) == 1 ? 0 : t->stride(i);
   }
 };
+
+// Every row of the last dimension is contiguous and starts on 16 bytes.
+bool aligned_rows(const at::Tensor& t) {
+  const int64_t unit = 16 / static_cast<int64_t>(t.element_size()), last = t.dim() - 1;
+  if (t.stride(last) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+  for (int64_t i = 0; i < last; ++i)
+    if (t.size(i) != 1 && t.stride(i) % unit != 0) return false;
+  return true;
+}
+
+bool int32_vector(const at::Tensor& t) { return t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous(); }
 
 // A paged decode's arguments, checked: decode's of eleven (from args[0]).
 struct DecodeCall {
@@ -299,7 +313,8 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int device;
   if (over1 || over2 || !on_current_device(device, q, kc, vc, bt, ctx, cu, ks, vs) || capturing()) Py_RETURN_NONE;
   if (q->dim() != 3 || kc->dim() != 4 || kc->sizes() != vc->sizes() || bt->dim() != 2 ||
-      kc->scalar_type() != at::kFloat8_e4m3fn || vc->scalar_type() != at::kFloat8_e4m3fn || !scale_pair(*kc, ks, vs) ||
+      (kc->scalar_type() != at::kFloat8_e4m3fn && kc->scalar_type() != q->scalar_type()) ||
+      vc->scalar_type() != kc->scalar_type() || !scale_pair(*kc, ks, vs) ||
       bt->scalar_type() != at::kInt || ctx->scalar_type() != at::kInt || cu->scalar_type() != at::kInt ||
       ctx->dim() != 1 || cu->dim() != 1 || !ctx->is_contiguous() || !cu->is_contiguous())
     Py_RETURN_NONE;
@@ -307,18 +322,23 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int qd = dtype_code(q->scalar_type());
   if ((qd != PRISM_DTYPE_BF16 && qd != PRISM_DTYPE_F16) || total <= 0 || total > INT32_MAX || batch <= 0 ||
       batch > INT32_MAX || heads <= 0 || kv_heads <= 0 || heads > INT32_MAX || heads % kv_heads != 0 ||
-      q->size(1) != heads || dim != 128 || q->stride(2) != 1 || kc->size(2) != kv_heads || kc->size(3) != dim ||
+      q->size(1) != heads || q->stride(2) != 1 || kc->size(2) != kv_heads || kc->size(3) != dim ||
       kc->size(0) > INT32_MAX || kc->size(1) > INT32_MAX || bt->size(1) > INT32_MAX || cu->numel() < batch + 1 ||
       bt->size(0) < batch)
     Py_RETURN_NONE;
+  const bool sixteen = kc->scalar_type() == q->scalar_type();
+  if (sixteen ? (dim != 64 && dim != 128) || !aligned_rows(*q) : dim != 128) Py_RETURN_NONE;
   void* stream = current_stream(device);
   PyObject* found = by_stream(args[11], device, stream);
   if (found == nullptr || !PyTuple_CheckExact(found) || PyTuple_GET_SIZE(found) != 2) Py_RETURN_NONE;
   const at::Tensor *status = tensor(PyTuple_GET_ITEM(found, 0)), *report = tensor(PyTuple_GET_ITEM(found, 1));
   if (!status || !report) Py_RETURN_NONE;
   const int page = static_cast<int>(kc->size(1)), width = static_cast<int>(bt->size(1));
-  const int64_t need = prism_paged_prefill_workspace_bytes(static_cast<int>(batch), static_cast<int>(total),
-                                                           static_cast<int>(heads), static_cast<int>(kv_heads), page, width);
+  const int64_t need =
+      sixteen ? prism_paged_prefill_16bit_workspace_bytes(static_cast<int>(batch), static_cast<int>(total), static_cast<int>(heads),
+                                                          static_cast<int>(kv_heads), static_cast<int>(dim), page, width)
+              : prism_paged_prefill_workspace_bytes(static_cast<int>(batch), static_cast<int>(total),
+                                                    static_cast<int>(heads), static_cast<int>(kv_heads), page, width);
   at::Tensor out, ws;
   int32_t* words = static_cast<int32_t*>(report->data_ptr());
   words[0] = 0;  // (the thread's previous call on this stream has been waited for)
@@ -327,9 +347,9 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     WithoutGil released;
     out = at::empty(q->sizes(), q->options());
     if (need > 0) ws = at::empty({need}, q->options().dtype(at::kByte));
-    const Strides sq(q), sk(kc), sv(vc), sks(ks), svs(vs), sbt(bt), so(&out);
+    const Strides sq(q, sixteen), sk(kc), sv(vc), sks(ks), svs(vs), sbt(bt), so(&out);
     rc = prism_paged_prefill_ws(
-        q->data_ptr(), qd, sq.v, kc->data_ptr(), vc->data_ptr(), PRISM_DTYPE_FP8_E4M3FN, sk.v, sv.v, scales(ks),
+        q->data_ptr(), qd, sq.v, kc->data_ptr(), vc->data_ptr(), dtype_code(kc->scalar_type()), sk.v, sv.v, scales(ks),
         scales(vs), sks.v, svs.v, static_cast<const int32_t*>(bt->data_ptr()), sbt.v,
         static_cast<const int32_t*>(ctx->data_ptr()), static_cast<const int32_t*>(cu->data_ptr()), out.data_ptr(), so.v,
         static_cast<int>(batch), static_cast<int>(total), static_cast<int>(heads), static_cast<int>(kv_heads),
@@ -347,11 +367,130 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// prompt(q, k, v, cu_seqlens_q, cu_seqlens_k or None, num_heads, num_kv_heads, scale) -> output or None
+PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) Py_RETURN_NONE;
+  const bool same = args[4] == Py_None;
+  const at::Tensor *q = tensor(args[0]), *k = tensor(args[1]), *v = tensor(args[2]), *cq = tensor(args[3]),
+                   *ck = same ? cq : tensor(args[4]);
+  if (!q || !k || !v || !cq || !ck || !PyLong_CheckExact(args[5]) || !PyLong_CheckExact(args[6]) || !PyFloat_CheckExact(args[7]))
+    Py_RETURN_NONE;
+  int over1 = 0, over2 = 0;
+  const long heads = PyLong_AsLongAndOverflow(args[5], &over1), kv_heads = PyLong_AsLongAndOverflow(args[6], &over2);
+  int device;
+  if (over1 || over2 || !on_current_device(device, q, k, v, cq, ck) ||
+      (c10::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad())))
+    Py_RETURN_NONE;
+  const int type = dtype_code(q->scalar_type());
+  if (q->dim() != 3 || k->dim() != 3 || k->sizes() != v->sizes() || (type != PRISM_DTYPE_BF16 && type != PRISM_DTYPE_F16) ||
+      k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || !int32_vector(*cq) || !int32_vector(*ck))
+    Py_RETURN_NONE;
+  const int64_t total_q = q->size(0), total_k = k->size(0), dim = q->size(2), batch = cq->numel() - 1;
+  if (heads <= 0 || kv_heads <= 0 || heads > INT32_MAX || heads % kv_heads != 0 || q->size(1) != heads || k->size(1) != kv_heads ||
+      k->size(2) != dim || (dim != 64 && dim != 128) || total_q <= 0 || total_q > INT32_MAX || total_k <= 0 || total_k > INT32_MAX ||
+      batch < 0 || batch > INT32_MAX || ck->numel() != cq->numel() || (same && total_k != total_q) || !aligned_rows(*q) ||
+      !aligned_rows(*k) || !aligned_rows(*v))
+    Py_RETURN_NONE;
+  void* stream = current_stream(device);
+  const int64_t need = prism_prompt_attention_workspace_bytes(static_cast<int>(batch), static_cast<int>(total_q),
+                                                              static_cast<int>(total_k), static_cast<int>(heads),
+                                                              static_cast<int>(kv_heads), static_cast<int>(dim));
+  at::Tensor out, ws;
+  int rc;
+  {
+    WithoutGil released;
+    out = at::empty(q->sizes(), q->options());
+    if (need > 0) ws = at::empty({need}, q->options().dtype(at::kByte));
+    const Strides sq(q, true), sk(k, true), sv(v, true), so(&out);
+    rc = prism_prompt_attention(q->data_ptr(), sq.v, k->data_ptr(), sk.v, v->data_ptr(), sv.v, type,
+                                static_cast<const int32_t*>(cq->data_ptr()), static_cast<const int32_t*>(ck->data_ptr()),
+                                out.data_ptr(), so.v, static_cast<int>(batch), static_cast<int>(total_q),
+                                static_cast<int>(total_k), static_cast<int>(heads), static_cast<int>(kv_heads),
+                                static_cast<int>(dim), static_cast<float>(PyFloat_AS_DOUBLE(args[7])),
+                                need > 0 ? ws.data_ptr() : nullptr, need, stream);
+  }
+  if (rc != PRISM_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A tensor of `sizes` (contiguous) at an offset of int32 storage.
+at::Tensor int32_view(const at::Tensor& base, int64_t offset, at::IntArrayRef sizes) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), base.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
+// step_metadata(block_tables, cached_lens, query_lens, block_size, num_tokens, free_blocks or None, free_start or None)
+// -> (packed, slot_mapping, positions, cu_seqlens_q, context_lens, max_context_len, next_free, first_misfit,
+//     block_tables) or None
+PyObject* step_metadata(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  const at::Tensor *bt = tensor(args[0]), *cached = tensor(args[1]), *fresh = tensor(args[2]),
+                   *free = args[5] == Py_None ? nullptr : tensor(args[5]), *start = args[6] == Py_None ? nullptr : tensor(args[6]);
+  if (!bt || !cached || !fresh || (!free && args[5] != Py_None) || (!start && args[6] != Py_None) || !PyLong_CheckExact(args[3]) ||
+      !PyLong_CheckExact(args[4]))
+    Py_RETURN_NONE;
+  int over1 = 0, over2 = 0;
+  const long page = PyLong_AsLongAndOverflow(args[3], &over1), tokens = PyLong_AsLongAndOverflow(args[4], &over2);
+  int device;
+  if (over1 || over2 || page <= 0 || page > INT32_MAX || tokens < 0 || tokens > INT32_MAX - 4 ||
+      !on_current_device(device, bt, cached, fresh, free, start))
+    Py_RETURN_NONE;
+  if (bt->dim() != 2 || bt->scalar_type() != at::kInt || !int32_vector(*cached) || !int32_vector(*fresh) ||
+      (free && !int32_vector(*free)) || (start && (start->scalar_type() != at::kInt || start->numel() != 1)))
+    Py_RETURN_NONE;
+  const int64_t batch = bt->size(0), width = bt->size(1);
+  if (cached->numel() != batch || fresh->numel() != batch || batch > 8192 || width > INT32_MAX ||
+      (free && free->numel() > INT32_MAX))
+    Py_RETURN_NONE;
+  void* stream = current_stream(device);
+  const int64_t words = prism_step_metadata_words(static_cast<int>(batch), static_cast<int>(width), static_cast<int>(tokens));
+  at::Tensor packed;
+  int rc;
+  {
+    WithoutGil released;
+    packed = at::empty({words}, bt->options());
+    const Strides sbt(bt);
+    rc = prism_step_metadata(static_cast<const int32_t*>(bt->data_ptr()), sbt.v, static_cast<const int32_t*>(cached->data_ptr()),
+                             static_cast<const int32_t*>(fresh->data_ptr()),
+                             free ? static_cast<const int32_t*>(free->data_ptr()) : nullptr,
+                             free ? static_cast<int>(free->numel()) : 0,
+                             start ? static_cast<const int32_t*>(start->data_ptr()) : nullptr, static_cast<int>(batch),
+                             static_cast<int>(width), static_cast<int>(page), static_cast<int>(tokens),
+                             static_cast<int32_t*>(packed.data_ptr()), stream);
+  }
+  if (rc != PRISM_OK) Py_RETURN_NONE;
+  const int64_t padded = (tokens + 3) / 4 * 4, cu = 2 * padded, ctx = cu + batch + 1, tail = ctx + batch;
+  const int64_t tables = cu + (2 * batch + 4 + 3) / 4 * 4;
+  at::Tensor views[9] = {packed, int32_view(packed, 0, {tokens}), int32_view(packed, padded, {tokens}),
+                         int32_view(packed, cu, {batch + 1}), int32_view(packed, ctx, {batch}), int32_view(packed, tail, {}),
+                         int32_view(packed, tail + 1, {}), int32_view(packed, tail + 2, {}),
+                         int32_view(packed, tables, {batch, width})};
+  PyObject* result = PyTuple_New(9);
+  if (result == nullptr) return nullptr;
+  for (int i = 0; i < 9; ++i) {
+    PyObject* item = THPVariable_Wrap(std::move(views[i]));
+    if (item == nullptr) {
+      Py_DECREF(result);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(result, i, item);
+  }
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"mark_ready", mark_ready, METH_O, nullptr},
     {"store", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(store)), METH_FASTCALL, nullptr},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(decode)), METH_FASTCALL, nullptr},
     {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(step)), METH_FASTCALL, nullptr},
+    {"prompt", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(prompt)), METH_FASTCALL, nullptr},
+    {"step_metadata", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(step_metadata)), METH_FASTCALL, nullptr},
     {"prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(prefill)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -23,6 +23,8 @@ import torch
 
 from prism_infer import _native
 
+_HOST = _native.host_ops()
+
 MAX_STEP_REQUESTS = 8192
 _FITS = 2**31 - 1
 
@@ -107,6 +109,11 @@ def build_step_metadata(
     missing, and :meth:`StepMetadata.check` reports them.
     """
 
+    # calls that the native checks accept; the rest goes on below
+    if _HOST is not None and out is None:
+        done = _HOST.step_metadata(block_tables, cached_lens, query_lens, block_size, num_tokens, free_blocks, free_start)
+        if done is not None:
+            return StepMetadata(*done)
     block_size, num_tokens = int(block_size), int(num_tokens)
     if block_size <= 0 or num_tokens < 0:
         raise ValueError(f"block_size must be positive and num_tokens not negative, got {block_size} and {num_tokens}")

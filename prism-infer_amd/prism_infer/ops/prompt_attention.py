@@ -28,6 +28,7 @@ import torch
 from prism_infer import _native
 
 HAS_HIP_KERNELS = _native.available()
+_HOST = _native.host_ops()
 
 PROMPT_HEAD_DIMS = (64, 128)
 PROMPT_DTYPES = (torch.bfloat16, torch.float16)
@@ -73,6 +74,11 @@ def prompt_attention(
 ) -> torch.Tensor:
     """Attend each packed prompt to its own keys, causally; returns [total_q, num_heads, head_dim]."""
 
+    # calls that the native checks accept; the rest goes on below
+    if _HOST is not None:
+        out = _HOST.prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, num_heads, num_kv_heads, scale)
+        if out is not None:
+            return out
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
     _validate_prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, num_heads, num_kv_heads)
