@@ -25,6 +25,7 @@
 // tile's scores and the last one's output beside the softmax 1055 (1042
 // TFLOP/s, 0.83 of a large library product on the same card).
 #include "common.h"
+#include "wave_ops.h"
 
 #include <algorithm>
 
@@ -119,29 +120,6 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const void* p) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
   return reinterpret_cast<const uint8_t*>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-
-__device__ __forceinline__ int uniform_int(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// Inclusive wave scan over lanes of non-negative values (0 is f's neutral element).
-template <typename F>
-__device__ __forceinline__ int wave_scan(int v, F f) {
-  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
-  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
-  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
-  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
-  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
-  return f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
-}
-struct Add {
-  __device__ int operator()(int x, int y) const { return x + y; }
-};
-struct Max {
-  __device__ int operator()(int x, int y) const { return max(x, y); }
-};
-template <typename F>
-__device__ __forceinline__ int wave_reduce(int v, F f) {
-  return __builtin_amdgcn_readlane(wave_scan(v, f), 63);
 }
 
 struct Seq {
@@ -923,44 +901,53 @@ attention16_kernel(const AttnArgs a) {
           u32x2{pack<F16>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv), pack<F16>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
 }
 
-// Joins the parts of split blocks: eight rows of a block and kv head per
-// workgroup, 32 lanes each.
+// Joins the parts of split blocks: one wave per row, each lane D / 64 dims.  The
+// number of blocks, the block and the parts' sums are loaded at once.
 template <bool F16, int D>
 __global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a) {
-  constexpr int kPer = D / 32;
+  constexpr int kPer = D / 64;
   const SplitScratch scratch(a.work, a.slots, D);
-  const int index = static_cast<int>(blockIdx.x) / (kBlockRows / 8);
-  if (index >= *scratch.count) return;
-  const SplitBlock b = scratch.blocks[index];
-  const int r = static_cast<int>(blockIdx.x) % (kBlockRows / 8) * 8 + threadIdx.x / 32, row = b.row0 + r;
-  if (row >= b.rows) return;
+  const int lane = threadIdx.x % 64;
+  const int index = static_cast<int>(blockIdx.x) / (kBlockRows / 4);
+  const int r = uniform_int(static_cast<int>(blockIdx.x) % (kBlockRows / 4) * 4 + threadIdx.x / 64);
+  const SplitBlock b = scratch.blocks[index];  // (anything where there is none)
+  const int row = b.row0 + r;
+  if (index >= *scratch.count || row >= b.rows) return;
   const int64_t step = static_cast<int64_t>(a.kv_heads) * kBlockRows;  // from part to part
   const int64_t cell = static_cast<int64_t>(b.slot) * kBlockRows + r;
   const floatx2* ml = reinterpret_cast<const floatx2*>(scratch.ml) + cell;
+  const float* src = scratch.out + cell * D + lane * kPer;
   // Parts without a visible key hold zeros and weigh nothing; a NaN sum goes
   // through whatever its part's weight is.
-  float m = -INFINITY;
-  for (int p = 0; p < b.parts; ++p) {
-    const floatx2 x = ml[p * step];
-    m = x[1] != 0.f ? fmaxf(m, x[0]) : m;
-  }
-  const int lane = threadIdx.x % 32;
-  const float* src = scratch.out + cell * D + lane * kPer;
-  float l = 0.f, o[kPer] = {};
-#pragma unroll 2
-  for (int p = 0; p < b.parts; ++p) {
-    const floatx2 x = ml[p * step];
-    const float w = x[1] != 0.f ? __builtin_amdgcn_exp2f(x[0] - m) : 0.f;
-    l = fmaf(w, x[1], l);
+  float m = -INFINITY, l = 0.f, o[kPer] = {};
+  for (int p0 = 0; p0 < b.parts; p0 += 64) {  // lane p holds a part's sum
+    const floatx2 x = p0 + lane < b.parts ? ml[(p0 + lane) * step] : floatx2{-INFINITY, 0.f};
+    const bool live = x[1] != 0.f;
+    float top = live ? x[0] : -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) o[j] = fmaf(w, src[p * step * D + j], o[j]);
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+    const float m_new = fmaxf(m, top), old = m_new > m ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
+    m = m_new;
+    const float weight = live ? __builtin_amdgcn_exp2f(x[0] - m) : 0.f;
+    float sum = weight * x[1];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+    l = fmaf(l, old, sum);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) o[j] *= old;
+    const int n = min(b.parts - p0, 64);
+#pragma unroll 4
+    for (int p = 0; p < n; ++p) {
+      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p));
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) o[j] = fmaf(w, src[(p0 + p) * step * D + j], o[j]);
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int tok = row / a.group, head = b.head * a.group + (row - tok * a.group);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(b.qs + tok) * a.o_st +
-                                              static_cast<int64_t>(head) * a.o_sh + lane * kPer);
-#pragma unroll
-  for (int j = 0; j < kPer; j += 2) dst[j / 2] = pack<F16>(o[j] * inv, o[j + 1] * inv);
+  uint16_t* dst = a.out + static_cast<int64_t>(b.qs + tok) * a.o_st + static_cast<int64_t>(head) * a.o_sh + lane * kPer;
+  if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(dst) = pack<F16>(o[0] * inv, o[1] * inv);
+  else *dst = static_cast<uint16_t>(pack<F16>(o[0] * inv, 0.f));
 }
 
 // The chip holds two workgroups per CU (registers, LDS).
@@ -986,7 +973,7 @@ int launch(const AttnArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((attention16_kernel<F16, D, SRC>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves), 0, stream, a);
   if (int rc = check_launch("attention16_kernel launch")) return rc;
   if (a.work == nullptr) return PRISM_OK;
-  const int64_t split = std::min<int64_t>(blocks, a.slots) * (kBlockRows / 8);
+  const int64_t split = std::min<int64_t>(blocks, a.slots) * (kBlockRows / 4);
   hipLaunchKernelGGL((attention16_join_kernel<F16, D>), dim3(static_cast<unsigned>(split)), dim3(256), 0, stream, a);
   return check_launch("attention16_join_kernel launch");
 }

@@ -29,7 +29,7 @@ MAX_STEP_REQUESTS = 8192
 _FITS = 2**31 - 1
 
 
-@dataclass
+@dataclass(slots=True)
 class StepMetadata:
     packed: torch.Tensor           # int32, all of the below
     slot_mapping: torch.Tensor     # int32 [num_tokens], -1 behind the last token
