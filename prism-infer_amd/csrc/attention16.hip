@@ -25,6 +25,7 @@
 // tile's scores and the last one's output beside the softmax 1055 (1042
 // TFLOP/s, 0.83 of a large library product on the same card).
 #include "common.h"
+#include "divide.h"
 #include "wave_ops.h"
 
 #include <algorithm>
@@ -63,7 +64,9 @@ struct AttnArgs {
   float scale_log2;
   int* status;
   int* report;  // pinned: [0] set to 1 where a sequence is flagged, [1] and [2] the packed rows' extent; or null
+  Divisor by_group, by_kv_heads;
   int slots;      // workgroups that the chip holds at once
+  int room;       // of one kv head
   uint8_t* work;  // scratch of split blocks (SplitScratch), or null: no block is split
 };
 
@@ -131,25 +134,24 @@ __device__ __forceinline__ void flag_sequence(const AttnArgs& a, int i) {
   if (a.report != nullptr) a.report[0] = 1;  // (every writer stores the same)
 }
 
-// Sequence i's rows and keys; false where its lengths are not valid (packed:
-// offsets out of order or outside the tensors), which takes it out of the work.
-template <int SRC>
-__device__ __forceinline__ bool sequence(const AttnArgs& a, int i, Seq& s) {
-  const int q0 = a.cu_q[i], q1 = a.cu_q[i + 1];
-  s.q0 = q0;
-  s.qlen = q1 - q0;
-  bool ok = q0 >= 0 && q1 >= q0 && q1 <= a.total_q;
-  if constexpr (SRC == kPacked) {
-    const int k0 = a.cu_k[i], k1 = a.cu_k[i + 1];
-    s.k0 = k0;
-    s.klen = k1 - k0;
-    ok = ok && k0 >= 0 && k1 >= k0 && k1 <= a.total_k;
-  } else {
-    s.k0 = 0;
-    s.klen = a.ctx[i];
-    ok = ok && q1 > q0 && s.klen >= s.qlen && s.klen <= static_cast<int64_t>(a.width) * a.page;
+// Rows and keys of K sequences from i on; good: whether their lengths are valid
+// (packed: offsets in order and inside the tensors).  Others are out of the work.
+template <int SRC, int K>
+__device__ __forceinline__ void sequences(const AttnArgs& a, int i, Seq (&s)[K], bool (&good)[K]) {
+  int q[K + 1], k[K + 1];
+#pragma unroll
+  for (int j = 0; j <= K; ++j) {
+    q[j] = a.cu_q[min(i + j, a.batch)];
+    if (SRC == kPacked) k[j] = a.cu_k[min(i + j, a.batch)];
+    else k[j] = a.ctx[min(i + j, a.batch - 1)];
   }
-  return ok && s.klen <= kMostKeys;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    s[j] = SRC == kPacked ? Seq{q[j], q[j + 1] - q[j], k[j], k[j + 1] - k[j]} : Seq{q[j], q[j + 1] - q[j], 0, k[j]};
+    good[j] = i + j < a.batch && q[j] >= 0 && q[j + 1] >= q[j] && q[j + 1] <= a.total_q && s[j].klen <= kMostKeys;
+    if (SRC == kPacked) good[j] = good[j] && k[j] >= 0 && k[j + 1] >= k[j] && k[j + 1] <= a.total_k;
+    else good[j] = good[j] && q[j + 1] > q[j] && s[j].klen >= s[j].qlen && s[j].klen <= static_cast<int64_t>(a.width) * a.page;
+  }
 }
 
 constexpr int kMinPart = 4;  // tiles
@@ -182,32 +184,24 @@ struct Work {
 template <int SRC, int ROWS, int K>
 __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
   const int lane = __lane_id();
-  int rank = uniform_int(static_cast<int>(blockIdx.x) / a.kv_heads);
+  int rank = divide(static_cast<int>(blockIdx.x), a.by_kv_heads);
   w.head = static_cast<int>(blockIdx.x) - rank * a.kv_heads;
   w.part = w.split = 0;
   w.parts = 1;
   Seq s[K];
+  bool good[K];
+  sequences<SRC, K>(a, lane * K, s, good);
   int n[K], l0[K], blocks = 0, top = 0, longest = 0;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int i = lane * K + k;
-    n[k] = 0;
-    l0[k] = 1;
-    s[k] = Seq{0, 0, 0, 0};
-    if (i < a.batch) {
-      if (sequence<SRC>(a, i, s[k])) {
-        l0[k] += static_cast<int>(min(static_cast<int64_t>(max(s[k].klen - s[k].qlen, 0)) * a.group / ROWS, static_cast<int64_t>(1 << 29)));
-        n[k] = (s[k].qlen * a.group + ROWS - 1) / ROWS;
-      } else if (SRC != kPacked && flag) {
-        flag_sequence(a, i);
-      }
-    }
+    n[k] = good[k] ? (s[k].qlen * a.group + ROWS - 1) / ROWS : 0;
+    l0[k] = 1 + static_cast<int>(min(static_cast<int64_t>(max(s[k].klen - s[k].qlen, 0)) * a.group / ROWS, static_cast<int64_t>(1 << 29)));
+    if (SRC != kPacked && flag && !good[k] && lane * K + k < a.batch) flag_sequence(a, lane * K + k);
     blocks += n[k];
     top = max(top, n[k] == 0 ? 0 : l0[k] + n[k]);
     longest = max(longest, n[k] == 0 ? 0 : (s[k].klen - 1) / kKeys + 1);
   }
   w.total = wave_reduce(blocks, Add());
-  top = wave_reduce(top, Max());
   int hit_k = 0, l = 0;
   // parts of a sequence's blocks (more than the chip holds: any number)
   auto parts_of = [&](int klen, int tiles) {
@@ -221,13 +215,12 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
     return wave_reduce(sum, Add());
   };
   int tiles = 0;  // of a part
-  const int room = a.slots / a.kv_heads;
-  if (a.work != nullptr && w.total > 0 && w.total < room) {
+  if (a.work != nullptr && w.total > 0 && w.total < a.room) {
     longest = wave_reduce(longest, Max());
     int lo = kMinPart, hi = max(longest, kMinPart);
     while (lo < hi) {  // fewest tiles for which the parts fit
       const int mid = (lo + hi) / 2;
-      if (total_parts(mid) <= room) hi = mid;
+      if (total_parts(mid) <= a.room) hi = mid;
       else lo = mid + 1;
     }
     const int all = total_parts(lo);
@@ -264,7 +257,7 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
   }
   if (tiles == 0) {
     if (rank >= w.total) return false;
-    if (K > 1 || w.total <= room) {  // all start at once, or many are short: sequence by sequence, in reverse
+    if (K > 1 || w.total <= a.room) {  // all start at once, or many are short: sequence by sequence, in reverse
       const int left = w.total - 1 - rank, incl = wave_scan(blocks, Add());
       l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left));
       w.block = left - __builtin_amdgcn_readlane(incl - blocks, l);
@@ -278,7 +271,7 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
       }
     } else {
     auto above = [&](int u) { return wave_reduce(min(max(l0[0] + n[0] - 1 - max(u, l0[0] - 1), 0), n[0]), Add()); };
-    int lo = 0, hi = top;
+    int lo = 0, hi = wave_reduce(top, Max());
     while (lo < hi) {  // smallest level with at most `rank` blocks above it
       const int mid = (lo + hi) / 2;
       if (above(mid) <= rank) hi = mid;
@@ -303,15 +296,17 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
 template <int SRC, int ROWS>
 __device__ __forceinline__ bool locate_many(const AttnArgs& a, bool flag, Work& w) {
   const int lane = __lane_id();
-  const int rank = uniform_int(static_cast<int>(blockIdx.x) / a.kv_heads);
+  const int rank = divide(static_cast<int>(blockIdx.x), a.by_kv_heads);
   w.head = static_cast<int>(blockIdx.x) - rank * a.kv_heads;
   w.part = w.split = 0;
   w.parts = 1;
   auto blocks_of = [&](int i, Seq& s, bool report) {
-    if (i >= a.batch) return 0;
-    if (sequence<SRC>(a, i, s)) return (s.qlen * a.group + ROWS - 1) / ROWS;
-    if (SRC != kPacked && report) flag_sequence(a, i);
-    return 0;
+    Seq one[1];
+    bool good[1];
+    sequences<SRC, 1>(a, i, one, good);
+    s = one[0];
+    if (SRC != kPacked && report && !good[0] && i < a.batch) flag_sequence(a, i);
+    return good[0] ? (s.qlen * a.group + ROWS - 1) / ROWS : 0;
   };
   w.total = 0;
   Seq s;
@@ -414,20 +409,24 @@ attention16_kernel(const AttnArgs a) {
   const int prefix = klen - qlen;
   const int rows = qlen * a.group;
   const int row0 = block * kRows + wave * kCols;                               // the wave's first row
-  const int kend = min(klen, prefix + uniform_int((min((block + 1) * kRows, rows) - 1) / a.group) + 1);  // keys [0, kend) are needed
-  const int wpos0 = prefix + uniform_int(row0 / a.group);                      // position of the wave's first row
-  const int wlast = row0 < rows ? prefix + uniform_int((min(row0 + kCols, rows) - 1) / a.group) : -1;  // and of its last
+  const int kend = min(klen, prefix + divide(min((block + 1) * kRows, rows) - 1, a.by_group) + 1);  // keys [0, kend) are needed
+  const int wpos0 = prefix + divide(row0, a.by_group);                      // position of the wave's first row
+  const int wlast = row0 < rows ? prefix + divide(min(row0 + kCols, rows) - 1, a.by_group) : -1;  // and of its last
   // the workgroup's tiles, and the wave's end
   const int part = uniform_int(work.part), parts = uniform_int(work.parts);
   const int all_tiles = kend > 0 ? (kend - 1) / kKeys + 1 : 0;
-  const int t0 = uniform_int(static_cast<int>(static_cast<int64_t>(all_tiles) * part / parts));
-  const int t1 = uniform_int(static_cast<int>(static_cast<int64_t>(all_tiles) * (part + 1) / parts));
+  int t0 = 0, t1 = all_tiles;
+  if (parts > 1) {
+    const int per_part = uniform_int((all_tiles + parts - 1) / parts);
+    t0 = min(part * per_part, all_tiles);
+    t1 = min(t0 + per_part, all_tiles);
+  }
   const int tw = wlast >= 0 ? min(t1, wlast / kKeys + 1) : 0;
 
   // the lane's row: column c
   auto row_at = [&](int& tok, int& head) {
     const int row = row0 + c;
-    tok = row / a.group;
+    tok = divide(row, a.by_group);
     head = h * a.group + (row - tok * a.group);
     return row < rows;
   };
@@ -476,7 +475,7 @@ attention16_kernel(const AttnArgs a) {
   int page = 0, page_row = 0, ids_base = 0, ids = 0;
   auto start_walk = [&]() {
     if constexpr (SRC != kPacked) {
-      page = uniform_int(t0 * kKeys / a.page);
+      page = t0 == 0 ? 0 : uniform_int(t0 * kKeys / a.page);
       page_row = t0 * kKeys - page * a.page;
       ids_base = page;
       ids = load_ids(page);
@@ -944,7 +943,7 @@ __global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a)
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int tok = row / a.group, head = b.head * a.group + (row - tok * a.group);
+  const int tok = divide(row, a.by_group), head = b.head * a.group + (row - tok * a.group);
   uint16_t* dst = a.out + static_cast<int64_t>(b.qs + tok) * a.o_st + static_cast<int64_t>(head) * a.o_sh + lane * kPer;
   if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(dst) = pack<F16>(o[0] * inv, o[1] * inv);
   else *dst = static_cast<uint16_t>(pack<F16>(o[0] * inv, 0.f));
@@ -991,6 +990,9 @@ int64_t scratch_bytes(int batch, int64_t total_q, int heads, int kv_heads, int h
 // Without scratch for the parts no block is split.
 int dispatch(AttnArgs a, int dtype, int head_dim, int64_t most_keys, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   a.slots = chip_slots();
+  a.room = a.slots / a.kv_heads;
+  a.by_group = divisor(a.group);
+  a.by_kv_heads = divisor(a.kv_heads);
   const int64_t need = scratch_bytes(a.batch, a.total_q, a.heads, a.kv_heads, head_dim, most_keys);
   a.work = need > 0 && workspace != nullptr && aligned(workspace, 256) && workspace_bytes >= need ? static_cast<uint8_t*>(workspace) : nullptr;
   if (dtype == PRISM_DTYPE_F16) return head_dim == 128 ? by_source<true, 128>(a, stream) : by_source<true, 64>(a, stream);

@@ -18,6 +18,7 @@
 // 5.9 (the scan alone 2.6, 2.8 and 3.6); with 64-bit divisions, scans through LDS
 // and an atomic per lane 9.6, 9.8 and 14.8.
 #include "common.h"
+#include "divide.h"
 #include "wave_ops.h"
 
 #include <algorithm>
@@ -31,20 +32,6 @@ constexpr int kMaxInt = 0x7FFFFFFF;
 constexpr int kMostItems = kMaxInt - 64;  // tokens, table steps
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-// n / d for 0 <= n < 2^31: with 2^l the smallest power of two >= d and m =
-// ceil(2^(31 + l) / d), n m is above n 2^(31 + l) / d by less than n 2^l / d, so
-// that its floor is n / d's.
-struct Divisor {
-  uint32_t m;
-  int shift;
-};
-
-Divisor divisor(int d) {
-  int l = 0;
-  while ((int64_t{1} << l) < d) ++l;
-  return Divisor{static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), 31 + l};
-}
 
 struct MetaArgs {
   const int32_t* tables;
@@ -64,10 +51,6 @@ struct MetaArgs {
   int32_t* tail;  // max context length, next free entry, lowest request that does not fit
   int32_t* out;
 };
-
-__device__ __forceinline__ int divide(int n, Divisor d) {
-  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * d.m) >> d.shift);
-}
 
 // Sums stay at INT32_MAX once they reach it.
 __device__ __forceinline__ int add_sat(int x, int y) {
