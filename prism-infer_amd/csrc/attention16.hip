@@ -900,15 +900,16 @@ attention16_kernel(const AttnArgs a) {
           u32x2{pack<F16>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv), pack<F16>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
 }
 
-// Joins the parts of split blocks: one wave per row, each lane D / 64 dims.  The
-// number of blocks, the block and the parts' sums are loaded at once.
+// Joins the parts of split blocks: half a wave per row, each lane D / 32 dims.
+// Eight parts' sums and rows are loaded at once.
 template <bool F16, int D>
 __global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a) {
-  constexpr int kPer = D / 64;
+  constexpr int kPer = D / 32, kBatch = 8;
+  typedef float vals __attribute__((ext_vector_type(kPer)));
   const SplitScratch scratch(a.work, a.slots, D);
-  const int lane = threadIdx.x % 64;
-  const int index = static_cast<int>(blockIdx.x) / (kBlockRows / 4);
-  const int r = uniform_int(static_cast<int>(blockIdx.x) % (kBlockRows / 4) * 4 + threadIdx.x / 64);
+  const int lane = threadIdx.x % 32;
+  const int index = static_cast<int>(blockIdx.x) / (kBlockRows / 8);
+  const int r = static_cast<int>(blockIdx.x) % (kBlockRows / 8) * 8 + threadIdx.x / 32;
   const SplitBlock b = scratch.blocks[index];  // (anything where there is none)
   const int row = b.row0 + r;
   if (index >= *scratch.count || row >= b.rows) return;
@@ -916,37 +917,41 @@ __global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a)
   const int64_t cell = static_cast<int64_t>(b.slot) * kBlockRows + r;
   const floatx2* ml = reinterpret_cast<const floatx2*>(scratch.ml) + cell;
   const float* src = scratch.out + cell * D + lane * kPer;
-  // Parts without a visible key hold zeros and weigh nothing; a NaN sum goes
-  // through whatever its part's weight is.
-  float m = -INFINITY, l = 0.f, o[kPer] = {};
-  for (int p0 = 0; p0 < b.parts; p0 += 64) {  // lane p holds a part's sum
-    const floatx2 x = p0 + lane < b.parts ? ml[(p0 + lane) * step] : floatx2{-INFINITY, 0.f};
-    const bool live = x[1] != 0.f;
-    float top = live ? x[0] : -INFINITY;
+  float m = -INFINITY, l = 0.f;
+  vals o = {};
+  for (int p0 = 0; p0 < b.parts; p0 += kBatch) {
+    floatx2 x[kBatch];
+    vals v[kBatch];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-    const float m_new = fmaxf(m, top), old = m_new > m ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
-    m = m_new;
-    const float weight = live ? __builtin_amdgcn_exp2f(x[0] - m) : 0.f;
-    float sum = weight * x[1];
+    for (int p = 0; p < kBatch; ++p) {
+      const int64_t at = min(p0 + p, b.parts - 1) * step;  // (the last again where there is none: it weighs nothing)
+      x[p] = ml[at];
+      v[p] = *reinterpret_cast<const vals*>(src + at * D);
+    }
+    // Parts without a visible key hold zeros and weigh nothing; a NaN sum goes
+    // through whatever its part's weight is.
+    float top = m;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
-    l = fmaf(l, old, sum);
+    for (int p = 0; p < kBatch; ++p) top = x[p][1] != 0.f ? fmaxf(top, x[p][0]) : top;
+    const float old = top > m ? __builtin_amdgcn_exp2f(m - top) : 1.f;
+    m = top;
+    l *= old;
+    o *= old;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) o[j] *= old;
-    const int n = min(b.parts - p0, 64);
-#pragma unroll 4
-    for (int p = 0; p < n; ++p) {
-      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), p));
+    for (int p = 0; p < kBatch; ++p) {
+      const bool live = p0 + p < b.parts && x[p][1] != 0.f;
+      const float w = live ? __builtin_amdgcn_exp2f(x[p][0] - m) : 0.f;
+      l = live ? fmaf(w, x[p][1], l) : l;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) o[j] = fmaf(w, src[(p0 + p) * step * D + j], o[j]);
+      for (int j = 0; j < kPer; ++j) o[j] = live ? fmaf(w, v[p][j], o[j]) : o[j];
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int tok = divide(row, a.by_group), head = b.head * a.group + (row - tok * a.group);
-  uint16_t* dst = a.out + static_cast<int64_t>(b.qs + tok) * a.o_st + static_cast<int64_t>(head) * a.o_sh + lane * kPer;
-  if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(dst) = pack<F16>(o[0] * inv, o[1] * inv);
-  else *dst = static_cast<uint16_t>(pack<F16>(o[0] * inv, 0.f));
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(b.qs + tok) * a.o_st +
+                                              static_cast<int64_t>(head) * a.o_sh + lane * kPer);
+#pragma unroll
+  for (int j = 0; j < kPer; j += 2) dst[j / 2] = pack<F16>(o[j] * inv, o[j + 1] * inv);
 }
 
 // The chip holds two workgroups per CU (registers, LDS).
@@ -972,7 +977,7 @@ int launch(const AttnArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((attention16_kernel<F16, D, SRC>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves), 0, stream, a);
   if (int rc = check_launch("attention16_kernel launch")) return rc;
   if (a.work == nullptr) return PRISM_OK;
-  const int64_t split = std::min<int64_t>(blocks, a.slots) * (kBlockRows / 4);
+  const int64_t split = std::min<int64_t>(blocks, a.slots) * (kBlockRows / 8);
   hipLaunchKernelGGL((attention16_join_kernel<F16, D>), dim3(static_cast<unsigned>(split)), dim3(256), 0, stream, a);
   return check_launch("attention16_join_kernel launch");
 }
