@@ -423,38 +423,6 @@ attention16_kernel(const AttnArgs a) {
   }
   const int tw = wlast >= 0 ? min(t1, wlast / kKeys + 1) : 0;
 
-  // the lane's row: column c
-  auto row_at = [&](int& tok, int& head) {
-    const int row = row0 + c;
-    tok = divide(row, a.by_group);
-    head = h * a.group + (row - tok * a.group);
-    return row < rows;
-  };
-  int pos;  // position of the row's token, below 0 where it sees no key (and without a row)
-  vec qop[kSteps];
-  {
-    int tok, head;
-    const bool real = row_at(tok, head);
-    pos = real ? prefix + tok : -1;
-    const uint16_t* src = a.q + static_cast<int64_t>(qs + tok) * a.q_st + static_cast<int64_t>(head) * a.q_sh + 8 * g;
-#pragma unroll
-    for (int x = 0; x < kSteps; ++x)
-      qop[x] = __builtin_bit_cast(vec, real ? *reinterpret_cast<const u32x4*>(src + 16 * x) : u32x4{0, 0, 0, 0});
-  }
-  // The exponent's scale is positive, so that a masked score is -inf: a negative
-  // one is the queries' sign, and with 0 all queries are 0.
-  const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  if (a.scale_log2 <= 0.f) {
-    const uint32_t keep = a.scale_log2 == 0.f ? 0u : ~0u;
-#pragma unroll
-    for (int x = 0; x < kSteps; ++x) {
-      u32x4 w = __builtin_bit_cast(u32x4, qop[x]);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) w[d] = (w[d] & keep) ^ (0x80008000u & keep);
-      qop[x] = __builtin_bit_cast(vec, w);
-    }
-  }
-
   // ---- tile loads, straight into LDS.  A load of a wave covers kLoadRows rows;
   // row and swizzled chunk of a lane do not change from load to load.  Asm so
   // that the compiler's wait-count pass does not drain these loads before each
@@ -541,6 +509,51 @@ attention16_kernel(const AttnArgs a) {
                   uniform_int(lds0 + stage + static_cast<uint32_t>(wave) * 1024 + static_cast<uint32_t>(tr) * kRow));
     }
   };
+
+  // the first tiles' loads, then the queries'
+  Place place[3] = {};  // of tiles t, t + 1 and t + 2
+  if (t0 < t1) {
+    start_walk();
+    place[0] = look_up(t0);
+    issue(t0, place[0], false, 0);
+    issue(t0, place[0], true, kV + kPayload);
+    if (t0 + 1 < t1) {
+      place[1] = look_up(t0 + 1);
+      issue(t0 + 1, place[1], false, kPayload);
+    }
+  }
+
+  // the lane's row: column c
+  auto row_at = [&](int& tok, int& head) {
+    const int row = row0 + c;
+    tok = divide(row, a.by_group);
+    head = h * a.group + (row - tok * a.group);
+    return row < rows;
+  };
+  int pos;  // position of the row's token, below 0 where it sees no key (and without a row)
+  vec qop[kSteps];
+  {
+    int tok, head;
+    const bool real = row_at(tok, head);
+    pos = real ? prefix + tok : -1;
+    const uint16_t* src = a.q + static_cast<int64_t>(qs + tok) * a.q_st + static_cast<int64_t>(head) * a.q_sh + 8 * g;
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x)
+      qop[x] = __builtin_bit_cast(vec, real ? *reinterpret_cast<const u32x4*>(src + 16 * x) : u32x4{0, 0, 0, 0});
+  }
+  // The exponent's scale is positive, so that a masked score is -inf: a negative
+  // one is the queries' sign, and with 0 all queries are 0.
+  const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+  if (a.scale_log2 <= 0.f) {
+    const uint32_t keep = a.scale_log2 == 0.f ? 0u : ~0u;
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      u32x4 w = __builtin_bit_cast(u32x4, qop[x]);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) w[d] = (w[d] & keep) ^ (0x80008000u & keep);
+      qop[x] = __builtin_bit_cast(vec, w);
+    }
+  }
 
   // per-lane LDS offsets inside a stage; other chunks differ by an exclusive or
   const uint32_t k_rd = c * kRow + ((g ^ swz<D>(c)) << 4);
@@ -650,17 +663,6 @@ attention16_kernel(const AttnArgs a) {
   reset();
   {
     uint32_t k_next = kPayload, v_prev = kV;  // stages of K of tile t + 1 and V of tile t - 1
-    Place place[3] = {};  // of tiles t, t + 1 and t + 2
-    if (t0 < t1) {
-      start_walk();
-      place[0] = look_up(t0);
-      issue(t0, place[0], false, 0);
-      issue(t0, place[0], true, kV + kPayload);
-      if (t0 + 1 < t1) {
-        place[1] = look_up(t0 + 1);
-        issue(t0 + 1, place[1], false, kPayload);
-      }
-    }
     landed();
     barrier();
     floatx16 sa[2], sb[2];
@@ -870,14 +872,12 @@ attention16_kernel(const AttnArgs a) {
   // ---- epilogue
   const auto lsw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
   const float l_tot = __uint_as_float(lsw[0]) + __uint_as_float(lsw[1]);
-  int tok, head;
-  const bool real = row_at(tok, head);
   if (work.split > 0 && part == 0 && tid == 0)  // (a block of one part: no rows to join)
     SplitScratch(a.work, a.slots, D).blocks[work.index * a.kv_heads + h] =
         SplitBlock{qs, block * kRows, parts > 1 ? rows : 0, h, work.slot * a.kv_heads + h, parts};
   if (parts > 1) {
     const SplitScratch scratch(a.work, a.slots, D);
-    if (!real) return;
+    if (row0 + c >= rows) return;
     const int64_t cell = (static_cast<int64_t>(work.slot + part) * a.kv_heads + h) * kRows + wave * kCols + c;
     float* dst = scratch.out + cell * D + 4 * g;
 #pragma unroll
@@ -889,15 +889,26 @@ attention16_kernel(const AttnArgs a) {
     if (g == 0) *reinterpret_cast<floatx2*>(scratch.ml + 2 * cell) = floatx2{m_run, l_tot};
     return;
   }
-  if (!real) return;
+  // Rows leave through LDS (K's stages: every wave is past the last scores), so
+  // that a store covers whole rows.  Chunks are swizzled by row.
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // (a NaN sum makes the row NaN)
-  uint16_t* dst = a.out + static_cast<int64_t>(qs + tok) * a.o_st + static_cast<int64_t>(head) * a.o_sh + 4 * g;
+  constexpr int kChunks = kRow / 16;  // of an output row
+  uint8_t* mine = lds + wave * kCols * kRow;
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<u32x2*>(dst + 32 * d + 8 * i) =
+      *reinterpret_cast<u32x2*>(mine + c * kRow + (((4 * d + i) ^ (c % kChunks)) << 4) + 8 * g) =
           u32x2{pack<F16>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv), pack<F16>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
+#pragma unroll
+  for (int j = 0; j < kCols * kChunks / 64; ++j) {
+    const int r = j * (64 / kChunks) + lane / kChunks, chunk = lane % kChunks, row = row0 + r;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(mine + r * kRow + ((chunk ^ (r % kChunks)) << 4));
+    const int at = divide(row, a.by_group), in_group = row - at * a.group;
+    if (row < rows)
+      *reinterpret_cast<u32x4*>(a.out + static_cast<int64_t>(qs + at) * a.o_st + static_cast<int64_t>(h * a.group + in_group) * a.o_sh +
+                                8 * chunk) = x;
+  }
 }
 
 // Joins the parts of split blocks: half a wave per row, each lane D / 32 dims.
