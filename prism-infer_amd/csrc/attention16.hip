@@ -580,16 +580,14 @@ attention16_kernel(const AttnArgs a) {
           reinterpret_cast<lds_s16x4*>(lds0 + ((stage + v_rd) ^ (n << 6) ^ (x << 5)) + (16 * m + 8 * x) * kRow));
     return u.w;
   };
-  // the same with keys that nobody sees, which may hold anything, as 0
-  auto read_v_end = [&](uint32_t stage, int pair, int key0) {
-    u32x4 w = read_v(stage, pair);
+  // keys that nobody sees, which may hold anything, as 0
+  auto drop_unseen = [&](u32x4& w, int pair, int key0) {
     const int left = kend - key0 - 16 * (pair / kDims) - 4 * g;
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
       const int j = 8 * (d / 2) + 2 * (d % 2);
       w[d] &= (j < left ? 0xFFFFu : 0u) | (j + 1 < left ? 0xFFFF0000u : 0u);
     }
-    return w;
   };
 
   floatx16 acc[kDims];  // O^T: dims 32 n + 8 (r / 4) + 4 g + r % 4 of the lane's row
@@ -779,8 +777,14 @@ attention16_kernel(const AttnArgs a) {
       begin(t);
       const int key0 = (t - 1) * kKeys;
       const bool cut = key0 + kKeys > kend;
+      u32x4 v[kPairs];  // (the scores' registers are free)
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) output_step(i, cut ? read_v_end(v_prev, i, key0) : read_v(v_prev, i), pa);
+      for (int i = 0; i < kPairs; ++i) v[i] = read_v(v_prev, i);
+      if (cut)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) drop_unseen(v[i], i, key0);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) output_step(i, v[i], pa);
       next();
       ++t;
     }
