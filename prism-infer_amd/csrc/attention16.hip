@@ -156,9 +156,15 @@ __device__ __forceinline__ void sequences(const AttnArgs& a, int i, Seq (&s)[K],
 
 constexpr int kMinPart = 4;  // tiles
 
-// Time of a launch, in units of 64 ns, whose longest block or part walks `tiles`
-// tiles; `parts` workgroups' rows are written in fp32 and merged by a second launch.
-__device__ inline int split_cost(int tiles, int parts) { return tiles * 16 + (parts > 0 ? 60 + parts / 16 : 0); }
+// Time of a launch of `wgs` workgroups, in units of 64 ns, whose longest walks
+// `tiles` tiles (1.1 us each, 1.9 where the CUs hold two workgroups); of split
+// blocks, the parts' rows in fp32 and the second launch.  Not split and split, us:
+// one token behind 700 keys 14.8 and 11.4, behind 12000 153 and 21, 200 tokens of
+// two sequences behind 4000 63.9 and 46.3 (32 / 8 heads); behind 700 19.9 and 30.5.
+__device__ inline int split_cost(const AttnArgs& a, int tiles, int wgs, bool split) {
+  const int tile = 2 * wgs > a.slots ? 30 : 17;
+  return tiles * tile + (split ? 90 + wgs / 3 : 0);
+}
 
 struct Work {
   int seq, block, head;
@@ -224,7 +230,7 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
       else lo = mid + 1;
     }
     const int all = total_parts(lo);
-    if (all > w.total && split_cost(lo, all * a.kv_heads) < split_cost(longest, 0)) tiles = lo;
+    if (all > w.total && split_cost(a, lo, all * a.kv_heads, true) < split_cost(a, longest, w.total * a.kv_heads, false)) tiles = lo;
     if (tiles > 0) {
       w.split = w.total;
       w.total = all;
@@ -366,8 +372,8 @@ __device__ __forceinline__ uint32_t pack(float lo, float up) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, up}, bf16x2));
 }
 
-template <bool F16, int D, int SRC>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+template <bool F16, int D, int SRC, int GROUPS>
+__global__ void __launch_bounds__(64 * kWaves * GROUPS) __attribute__((amdgpu_waves_per_eu(2)))
 attention16_kernel(const AttnArgs a) {
   using T = Type<F16>;
   typedef typename T::vec vec;
@@ -380,7 +386,8 @@ attention16_kernel(const AttnArgs a) {
   constexpr int kLoadRows = 1024 / kRow;      // rows per load of a wave
   constexpr int kLoads = kKeys / kLoadRows / kWaves;
   constexpr int kV = 2 * kPayload;            // two stages of K, then two of V
-  __shared__ __attribute__((aligned(256))) uint8_t lds[4 * kPayload];
+  constexpr int kShare = 4 * kPayload;        // of a group
+  __shared__ __attribute__((aligned(256))) uint8_t lds[GROUPS * kShare];
 
   Work work;
   const bool first_wave = blockIdx.x == 0 && threadIdx.x < 64;  // flags sequences
@@ -398,8 +405,9 @@ attention16_kernel(const AttnArgs a) {
     return;
   }
   const int seq = uniform_int(work.seq), block = uniform_int(work.block), h = uniform_int(work.head);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x % (64 * kWaves);  // in the group
   const int wave = uniform_int(tid / 64);
+  const int group = GROUPS == 1 ? 0 : uniform_int(threadIdx.x / (64 * kWaves));
   const int lane = tid % 64;
   const int c = lane % 32;
   const int g = lane / 32;
@@ -412,7 +420,7 @@ attention16_kernel(const AttnArgs a) {
   const int kend = min(klen, prefix + divide(min((block + 1) * kRows, rows) - 1, a.by_group) + 1);  // keys [0, kend) are needed
   const int wpos0 = prefix + divide(row0, a.by_group);                      // position of the wave's first row
   const int wlast = row0 < rows ? prefix + divide(min(row0 + kCols, rows) - 1, a.by_group) : -1;  // and of its last
-  // the workgroup's tiles, and the wave's end
+  // the group's tiles, and the wave's end
   const int part = uniform_int(work.part), parts = uniform_int(work.parts);
   const int all_tiles = kend > 0 ? (kend - 1) / kKeys + 1 : 0;
   int t0 = 0, t1 = all_tiles;
@@ -420,6 +428,11 @@ attention16_kernel(const AttnArgs a) {
     const int per_part = uniform_int((all_tiles + parts - 1) / parts);
     t0 = min(part * per_part, all_tiles);
     t1 = min(t0 + per_part, all_tiles);
+  }
+  const int steps = (t1 - t0 + GROUPS - 1) / GROUPS;  // tiles of a group, the same for the barriers of all
+  if (GROUPS > 1) {
+    t0 = min(t0 + group * steps, t1);
+    t1 = min(t0 + steps, t1);
   }
   const int tw = wlast >= 0 ? min(t1, wlast / kKeys + 1) : 0;
 
@@ -479,7 +492,8 @@ attention16_kernel(const AttnArgs a) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  : : "v"(off), "s"(uniform_ptr(base)), "s"(dst) : "memory", "m0");
   };
-  const uint32_t lds0 = lds_address(lds);
+  uint8_t* const share = lds + group * kShare;
+  const uint32_t lds0 = lds_address(share);
   // Starts the loads of K or V of tile t into LDS offset `stage`.  (A tile that
   // cannot be loaded leaves the stage as it was: its sequence is flagged.)
   auto issue = [&](int t, const Place& place, bool isv, uint32_t stage) {
@@ -564,7 +578,7 @@ attention16_kernel(const AttnArgs a) {
   }
   auto read_k = [&](uint32_t stage, int pair) {  // pair: 32-key half, MFMA step
     const int b = pair / kSteps, x = pair % kSteps;
-    return *reinterpret_cast<const u32x4*>(lds + b * 32 * kRow + ((stage + k_rd) ^ (x << 5)));
+    return *reinterpret_cast<const u32x4*>(share + b * 32 * kRow + ((stage + k_rd) ^ (x << 5)));
   };
   // V^T operand: k-slots 8 g + 0..3 of 16-key group m are keys 16 m + 4 g + 0..3,
   // slots 8 g + 4..7 the keys 8 further, the order of the score rows
@@ -788,7 +802,7 @@ attention16_kernel(const AttnArgs a) {
       next();
       ++t;
     }
-    for (; t <= t1; ++t) {
+    for (; t <= t0 + steps; ++t) {
       begin(t);
       next();
     }
@@ -875,7 +889,41 @@ attention16_kernel(const AttnArgs a) {
 
   // ---- epilogue
   const auto lsw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
-  const float l_tot = __uint_as_float(lsw[0]) + __uint_as_float(lsw[1]);
+  float l_tot = __uint_as_float(lsw[0]) + __uint_as_float(lsw[1]);
+  uint8_t* const mine = lds + wave * kCols * kRow;  // K's stages of the first group: every wave is past the last scores
+  if constexpr (GROUPS > 1) {
+    // The second group's waves leave their outputs in its stages, lane by lane, for
+    // the first one's to join.
+    static_assert(GROUPS == 2 && kWaves * kDims * 4 * 1024 == kShare, "an output fills a group's stages");
+    barrier();  // (every wave is past its last values)
+    uint8_t* const theirs = lds + kShare + wave * kDims * 4 * 1024 + lane * 16;
+    if (group == 1) {
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<floatx4*>(theirs + (4 * d + i) * 1024) =
+              floatx4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+      *reinterpret_cast<floatx2*>(mine + lane * 8) = floatx2{m_run, l_tot};
+    }
+    barrier();
+    if (group == 1) return;
+    // a group without a visible key holds zeros and weighs nothing; a NaN sum goes through
+    const floatx2 other = *reinterpret_cast<const floatx2*>(mine + lane * 8);
+    const bool live0 = l_tot != 0.f, live1 = other[1] != 0.f;
+    const float m = fmaxf(live0 ? m_run : -INFINITY, live1 ? other[0] : -INFINITY);
+    const float w0 = live0 ? __builtin_amdgcn_exp2f(m_run - m) : 0.f, w1 = live1 ? __builtin_amdgcn_exp2f(other[0] - m) : 0.f;
+    if (live0 || live1) m_run = m;
+    l_tot = l_tot * w0 + other[1] * w1;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const floatx4 x = *reinterpret_cast<const floatx4*>(theirs + (4 * d + i) * 1024);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[d][4 * i + j] = acc[d][4 * i + j] * w0 + x[j] * w1;
+      }
+  }
   if (work.split > 0 && part == 0 && tid == 0)  // (a block of one part: no rows to join)
     SplitScratch(a.work, a.slots, D).blocks[work.index * a.kv_heads + h] =
         SplitBlock{qs, block * kRows, parts > 1 ? rows : 0, h, work.slot * a.kv_heads + h, parts};
@@ -893,11 +941,10 @@ attention16_kernel(const AttnArgs a) {
     if (g == 0) *reinterpret_cast<floatx2*>(scratch.ml + 2 * cell) = floatx2{m_run, l_tot};
     return;
   }
-  // Rows leave through LDS (K's stages: every wave is past the last scores), so
-  // that a store covers whole rows.  Chunks are swizzled by row.
+  // Rows leave through LDS, so that a store covers whole rows.  Chunks are
+  // swizzled by row.
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // (a NaN sum makes the row NaN)
   constexpr int kChunks = kRow / 16;  // of an output row
-  uint8_t* mine = lds + wave * kCols * kRow;
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
@@ -969,17 +1016,35 @@ __global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a)
   for (int j = 0; j < kPer; j += 2) dst[j / 2] = pack<F16>(o[j] * inv, o[j + 1] * inv);
 }
 
-// The chip holds two workgroups per CU (registers, LDS).
-int chip_slots() { return 2 * device_cu_count(); }
+// The chip holds eight waves per CU (registers, LDS).
+int chip_slots(int groups) { return 2 / groups * device_cu_count(); }
+
+int64_t block_bound(int batch, int64_t total_q, int heads, int kv_heads) {
+  return (ceil_div(total_q * (heads / kv_heads), kBlockRows) + batch) * kv_heads;
+}
+
+// Groups of waves per workgroup: two, each with half of a block's keys, where
+// there are about as many blocks as CUs and they are long.  One group per
+// workgroup and two workgroups per CU hide each other's first loads and last
+// stores, which more blocks need; fewer blocks are split over the chip.  us with
+// one group and with two: one prompt of 1000 tokens (32 / 8 heads) 25.5 and 22.9,
+// of 2048 (16 heads of 64 dims) 30.4 and 22.4, four of 200 to 3500 (8 / 2 heads)
+// 65.3 and 54.2; 32 of 100 (32 / 8 heads) 23.8 and 37.6, one of 4096 143 and 168
+// (1032 blocks), one of 4096 over 4 / 1 heads 42.9 and 55.1 (129).
+int wave_groups(int batch, int64_t total_q, int heads, int kv_heads, int64_t average_keys) {
+  const int64_t cus = device_cu_count(), blocks = block_bound(batch, total_q, heads, kv_heads);
+  return 2 * blocks > cus + 2 * kv_heads && 4 * blocks <= 7 * cus && total_q * (heads / kv_heads) >= int64_t{4} * kBlockRows * batch &&
+                 average_keys >= 12 * kKeys ? 2 : 1;
+}
 
 // Whether blocks may be split: the fewest blocks that the rows make leave room for
 // parts, and the longest context could be more than one of them.
-bool may_split(int batch, int64_t total_q, int heads, int kv_heads, int64_t most_keys) {
+bool may_split(int batch, int64_t total_q, int heads, int kv_heads, int64_t most_keys, int groups) {
   const int64_t least = std::max<int64_t>(ceil_div(total_q * (heads / kv_heads), kBlockRows), 1) * kv_heads;
-  return batch <= 256 && 2 * least <= chip_slots() && most_keys > 2 * kMinPart * kKeys;
+  return batch <= 256 && 2 * least <= chip_slots(groups) && most_keys > 2 * kMinPart * groups * kKeys;
 }
 
-template <bool F16, int D, int SRC>
+template <bool F16, int D, int SRC, int GROUPS>
 int launch(const AttnArgs& a, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.total_q) * a.group;
   // every sequence may end in a partial block; one more for rows outside them
@@ -989,7 +1054,8 @@ int launch(const AttnArgs& a, hipStream_t stream) {
     return PRISM_ERR_INVALID;
   }
   const int64_t grid = a.work == nullptr ? blocks : std::max<int64_t>(blocks, a.slots + a.kv_heads);  // (parts never outnumber the slots)
-  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves), 0, stream, a);
+  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC, GROUPS>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves * GROUPS), 0,
+                     stream, a);
   if (int rc = check_launch("attention16_kernel launch")) return rc;
   if (a.work == nullptr) return PRISM_OK;
   const int64_t split = std::min<int64_t>(blocks, a.slots) * (kBlockRows / 8);
@@ -997,26 +1063,48 @@ int launch(const AttnArgs& a, hipStream_t stream) {
   return check_launch("attention16_join_kernel launch");
 }
 
-template <bool F16, int D>
+template <bool F16, int D, int GROUPS>
 int by_source(const AttnArgs& a, hipStream_t stream) {
-  if (a.bt == nullptr) return launch<F16, D, kPacked>(a, stream);
-  return a.page % kKeys == 0 ? launch<F16, D, kPages>(a, stream) : launch<F16, D, kSmallPages>(a, stream);
+  if (a.bt == nullptr) return launch<F16, D, kPacked, GROUPS>(a, stream);
+  return a.page % kKeys == 0 ? launch<F16, D, kPages, GROUPS>(a, stream) : launch<F16, D, kSmallPages, GROUPS>(a, stream);
 }
 
-int64_t scratch_bytes(int batch, int64_t total_q, int heads, int kv_heads, int head_dim, int64_t most_keys) {
-  return may_split(batch, total_q, heads, kv_heads, most_keys) ? SplitScratch::bytes(chip_slots(), head_dim) : 0;
+template <bool F16, int D>
+int by_groups(const AttnArgs& a, int groups, hipStream_t stream) {
+  return groups == 2 ? by_source<F16, D, 2>(a, stream) : by_source<F16, D, 1>(a, stream);
+}
+
+// How a launch is laid out, from static sizes; most_keys and average_keys: of a sequence.
+struct Layout {
+  int groups, slots;
+  bool split;
+  Layout(int batch, int64_t total_q, int heads, int kv_heads, int64_t most_keys, int64_t average_keys)
+      : groups(wave_groups(batch, total_q, heads, kv_heads, average_keys)), slots(chip_slots(groups)),
+        split(may_split(batch, total_q, heads, kv_heads, most_keys, groups)) {}
+  int64_t scratch(int head_dim) const { return split ? SplitScratch::bytes(slots, head_dim) : 0; }
+};
+
+Layout packed_layout(int batch, int total_q, int total_k, int heads, int kv_heads) {
+  return Layout(batch, total_q, heads, kv_heads, total_k, total_k / std::max(batch, 1));
+}
+
+Layout paged_layout(int batch, int total_q, int heads, int kv_heads, int page, int width) {
+  const int64_t capacity = static_cast<int64_t>(width) * page;
+  return Layout(batch, total_q, heads, kv_heads, capacity, capacity);
 }
 
 // Without scratch for the parts no block is split.
-int dispatch(AttnArgs a, int dtype, int head_dim, int64_t most_keys, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  a.slots = chip_slots();
+int dispatch(AttnArgs a, int dtype, int head_dim, const Layout& layout, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  a.slots = layout.slots;
+  const int groups = layout.groups;
+  const int64_t need = layout.scratch(head_dim);
+  a.work = need > 0 && workspace != nullptr && aligned(workspace, 256) && workspace_bytes >= need ? static_cast<uint8_t*>(workspace) : nullptr;
   a.room = a.slots / a.kv_heads;
   a.by_group = divisor(a.group);
   a.by_kv_heads = divisor(a.kv_heads);
-  const int64_t need = scratch_bytes(a.batch, a.total_q, a.heads, a.kv_heads, head_dim, most_keys);
-  a.work = need > 0 && workspace != nullptr && aligned(workspace, 256) && workspace_bytes >= need ? static_cast<uint8_t*>(workspace) : nullptr;
-  if (dtype == PRISM_DTYPE_F16) return head_dim == 128 ? by_source<true, 128>(a, stream) : by_source<true, 64>(a, stream);
-  return head_dim == 128 ? by_source<false, 128>(a, stream) : by_source<false, 64>(a, stream);
+  if (dtype == PRISM_DTYPE_F16)
+    return head_dim == 128 ? by_groups<true, 128>(a, groups, stream) : by_groups<true, 64>(a, groups, stream);
+  return head_dim == 128 ? by_groups<false, 128>(a, groups, stream) : by_groups<false, 64>(a, groups, stream);
 }
 
 // What both entries ask of q, K, V and out: types, heads, dims and layout.
@@ -1056,7 +1144,7 @@ int check_layout(const char* what, int dtype, int heads, int kv_heads, int head_
 
 int preload_attention16() {
   hipFuncAttributes attr;
-  return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&attention16_kernel<false, 128, kPacked>)), "preload_attention16");
+  return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&attention16_kernel<false, 128, kPacked, 1>)), "preload_attention16");
 }
 
 // prism_paged_prefill_ws over 16-bit caches; its geometry and pointers are checked there.
@@ -1088,7 +1176,7 @@ int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void*
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status;
   a.report = report;
-  return dispatch(a, dtype, head_dim, static_cast<int64_t>(width) * page, workspace, workspace_bytes, stream);
+  return dispatch(a, dtype, head_dim, paged_layout(batch, total_q, heads, kv_heads, page, width), workspace, workspace_bytes, stream);
 }
 
 }  // namespace prism
@@ -1098,7 +1186,7 @@ extern "C" int64_t prism_prompt_attention_workspace_bytes(int batch, int total_q
   if (batch <= 0 || total_q <= 0 || total_k <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       head_dim <= 0)
     return 0;
-  return prism::scratch_bytes(batch, total_q, num_heads, num_kv_heads, head_dim, total_k);
+  return prism::packed_layout(batch, total_q, total_k, num_heads, num_kv_heads).scratch(head_dim);
 }
 
 extern "C" int64_t prism_paged_prefill_16bit_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads,
@@ -1106,7 +1194,7 @@ extern "C" int64_t prism_paged_prefill_16bit_workspace_bytes(int batch, int tota
   if (batch <= 0 || total_q <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
       page_size <= 0 || width <= 0)
     return 0;
-  return prism::scratch_bytes(batch, total_q, num_heads, num_kv_heads, head_dim, static_cast<int64_t>(width) * page_size);
+  return prism::paged_layout(batch, total_q, num_heads, num_kv_heads, page_size, width).scratch(head_dim);
 }
 
 extern "C" int prism_prompt_attention(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
@@ -1142,5 +1230,6 @@ extern "C" int prism_prompt_attention(const void* q, const int64_t q_strides[3],
   a.batch = batch, a.heads = num_heads, a.kv_heads = num_kv_heads, a.group = num_heads / num_kv_heads;
   a.total_q = total_q, a.total_k = total_k;
   a.scale_log2 = scale * 1.4426950408889634f;
-  return dispatch(a, dtype, head_dim, total_k, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+  return dispatch(a, dtype, head_dim, packed_layout(batch, total_q, total_k, num_heads, num_kv_heads), workspace, workspace_bytes,
+                  static_cast<hipStream_t>(stream));
 }
