@@ -338,10 +338,12 @@ int prism_paged_prefill(const void* q, int q_dtype, const int64_t q_strides[3], 
  * 0 where none is used.  With it, few query blocks behind long contexts have
  * their keys split over several workgroups, whose fp32 partials a second
  * kernel merges; with less, or NULL, every block is one workgroup's.
- * `report` (int32[3] in pinned host memory, or NULL) lets a host see the
- * outcome with one wait for the stream and no copy: report[0], set to 0 by the
- * caller, becomes 1 where a sequence is recorded in `status`; report[1] and
- * report[2] get cu_seqlens_q[0] and cu_seqlens_q[batch].
+ * `report` (int32[4] in pinned host memory, or NULL) lets a host see the
+ * outcome with no copy: report[0], set to 0 by the caller, becomes 1 where a
+ * sequence is recorded in `status`; report[1] and report[2] get
+ * cu_seqlens_q[0] and cu_seqlens_q[batch].  Over FP8 caches they hold once the
+ * stream is done (report[3] is not used).  Over 16-bit caches report[3], set to
+ * 0 by the caller, becomes 1 once the others hold, before the attention is done.
  */
 int64_t prism_paged_prefill_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads, int page_size,
                                             int width);

@@ -63,7 +63,8 @@ struct AttnArgs {
   int batch, heads, kv_heads, group, page, num_blocks, width, total_q, total_k;
   float scale_log2;
   int* status;
-  int* report;  // pinned: [0] set to 1 where a sequence is flagged, [1] and [2] the packed rows' extent; or null
+  int* report;  // pinned, or null: [0] set to 1 where a sequence is flagged, [1] and [2] the packed rows' extent, [3] set
+                // to 1 once these are known
   Divisor by_group, by_kv_heads;
   int slots;      // workgroups that the chip holds at once
   int room;       // of one kv head
@@ -188,10 +189,10 @@ struct Work {
 // tiles for which all parts fit the chip at once, if that pays.
 // Returns false for a workgroup beyond the real blocks.
 template <int SRC, int ROWS, int K>
-__device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
+__device__ __forceinline__ bool locate(const AttnArgs& a, int me, bool flag, Work& w) {
   const int lane = __lane_id();
-  int rank = divide(static_cast<int>(blockIdx.x), a.by_kv_heads);
-  w.head = static_cast<int>(blockIdx.x) - rank * a.kv_heads;
+  int rank = divide(me, a.by_kv_heads);
+  w.head = me - rank * a.kv_heads;
   w.part = w.split = 0;
   w.parts = 1;
   Seq s[K];
@@ -300,10 +301,10 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, bool flag, Work& w) {
 
 // Larger batches: sequence by sequence, in reverse, nothing split.
 template <int SRC, int ROWS>
-__device__ __forceinline__ bool locate_many(const AttnArgs& a, bool flag, Work& w) {
+__device__ __forceinline__ bool locate_many(const AttnArgs& a, int me, bool flag, Work& w) {
   const int lane = __lane_id();
-  const int rank = divide(static_cast<int>(blockIdx.x), a.by_kv_heads);
-  w.head = static_cast<int>(blockIdx.x) - rank * a.kv_heads;
+  const int rank = divide(me, a.by_kv_heads);
+  w.head = me - rank * a.kv_heads;
   w.part = w.split = 0;
   w.parts = 1;
   auto blocks_of = [&](int i, Seq& s, bool report) {
@@ -335,6 +336,41 @@ __device__ __forceinline__ bool locate_many(const AttnArgs& a, bool flag, Work& 
     before = __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
+}
+
+// The outcome that a host waits for, from the first workgroup alone and long
+// before the others are done: every sequence's lengths and block ids.  Threads
+// are spread over the sequences first, then over a sequence's pages.
+template <int SRC>
+__device__ void check_metadata(const AttnArgs& a) {
+  __shared__ int first_bad;
+  constexpr int kAtOnce = 8;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  if (tid == 0) first_bad = INT32_MAX;
+  __syncthreads();
+  int across = 1;  // sequences at a time
+  while (across < a.batch && across < threads) across *= 2;
+  for (int i = tid & (across - 1); i < a.batch; i += across) {
+    Seq s[1];
+    bool good[1];
+    sequences<SRC, 1>(a, i, s, good);
+    const int pages = good[0] ? (s[0].klen - 1) / a.page + 1 : 0;
+    for (int p = tid / across; p < pages; p += kAtOnce * (threads / across)) {
+      int id[kAtOnce];
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x)
+        id[x] = a.bt[static_cast<int64_t>(i) * a.bt_sb + static_cast<int64_t>(min(p + x * (threads / across), pages - 1)) * a.bt_sn];
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) good[0] = good[0] && id[x] >= 0 && id[x] < a.num_blocks;
+    }
+    if (!good[0]) atomicMin(&first_bad, i);
+  }
+  __syncthreads();
+  if (tid != 0) return;
+  if (first_bad != INT32_MAX) flag_sequence(a, first_bad);
+  a.report[1] = a.cu_q[0];
+  a.report[2] = a.cu_q[a.batch];
+  __hip_atomic_store(a.report + 3, 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
 // Rows outside every sequence are 0: the workgroups beyond the real blocks
@@ -389,17 +425,19 @@ attention16_kernel(const AttnArgs a) {
   constexpr int kShare = 4 * kPayload;        // of a group
   __shared__ __attribute__((aligned(256))) uint8_t lds[GROUPS * kShare];
 
-  Work work;
-  const bool first_wave = blockIdx.x == 0 && threadIdx.x < 64;  // flags sequences
-  const bool found = a.batch <= 64 ? locate<SRC, kRows, 1>(a, first_wave, work)
-                     : a.batch <= 256 ? locate<SRC, kRows, 4>(a, first_wave, work) : locate_many<SRC, kRows>(a, first_wave, work);
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    if (a.report != nullptr) {
-      a.report[1] = a.cu_q[0];
-      a.report[2] = a.cu_q[a.batch];
-    }
-    if (a.work != nullptr) *SplitScratch(a.work, a.slots, D).count = work.split * a.kv_heads;
+  // With a report the first workgroups (one per kv head, which keeps the others'
+  // XCDs) are the check's.
+  const int checks = SRC != kPacked && a.report != nullptr ? a.kv_heads : 0;
+  const int me = static_cast<int>(blockIdx.x) - checks;
+  if (me < 0) {
+    if (blockIdx.x == 0) check_metadata<SRC>(a);
+    return;
   }
+  Work work;
+  const bool first_wave = me == 0 && checks == 0 && threadIdx.x < 64;  // flags sequences
+  const bool found = a.batch <= 64 ? locate<SRC, kRows, 1>(a, me, first_wave, work)
+                     : a.batch <= 256 ? locate<SRC, kRows, 4>(a, me, first_wave, work) : locate_many<SRC, kRows>(a, me, first_wave, work);
+  if (me == 0 && threadIdx.x == 0 && a.work != nullptr) *SplitScratch(a.work, a.slots, D).count = work.split * a.kv_heads;
   if (!found) {
     if (SRC == kPacked) zero_padding<D>(a, work.total);
     return;
@@ -1049,12 +1087,13 @@ int launch(const AttnArgs& a, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.total_q) * a.group;
   // every sequence may end in a partial block; one more for rows outside them
   const int64_t blocks = (ceil_div(rows, kCols * kWaves) + a.batch + 1) * a.kv_heads;
-  if (blocks > INT32_MAX || rows > INT32_MAX - kBlockRows) {
+  if (blocks > INT32_MAX - 2 * a.kv_heads || rows > INT32_MAX - kBlockRows) {
     set_error("attention over 16-bit keys: too many query rows for one launch");
     return PRISM_ERR_INVALID;
   }
   const int64_t grid = a.work == nullptr ? blocks : std::max<int64_t>(blocks, a.slots + a.kv_heads);  // (parts never outnumber the slots)
-  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC, GROUPS>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves * GROUPS), 0,
+  const int64_t checks = SRC != kPacked && a.report != nullptr ? a.kv_heads : 0;
+  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC, GROUPS>), dim3(static_cast<unsigned>(grid + checks)), dim3(64 * kWaves * GROUPS), 0,
                      stream, a);
   if (int rc = check_launch("attention16_kernel launch")) return rc;
   if (a.work == nullptr) return PRISM_OK;

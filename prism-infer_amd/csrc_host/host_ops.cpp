@@ -294,12 +294,26 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Waits until the word is set; false where the stream is done, or has failed,
+// without that.
+bool outcome_known(const int32_t* word, void* stream) {
+  while (true) {
+    for (int i = 0; i < 2000; ++i) {
+      if (__atomic_load_n(word, __ATOMIC_ACQUIRE) != 0) return true;
+      __builtin_ia32_pause();
+    }
+    if (hipStreamQuery(static_cast<hipStream_t>(stream)) != hipErrorNotReady) return __atomic_load_n(word, __ATOMIC_ACQUIRE) != 0;
+    (void)hipGetLastError();  // (not ready: no error for the next launch's check to find)
+  }
+}
+
 // prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, num_heads, num_kv_heads, scale, k_scale,
 //         v_scale, buffers) -> (out, first bad sequence, first row, end row) or None
 //
 // buffers: this thread's {(device, stream): (status int32[1] on the device,
-// pinned int32[3])}; status holds INT32_MAX between calls.  Waits for the
-// stream, as the caller's check of the status does.
+// pinned int32[4])}; status holds INT32_MAX between calls.  Waits for the
+// outcome: over FP8 caches with the stream, over 16-bit ones for the word that
+// the launch's check sets.
 PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 12) Py_RETURN_NONE;
@@ -341,7 +355,7 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                                     static_cast<int>(heads), static_cast<int>(kv_heads), page, width);
   at::Tensor out, ws;
   int32_t* words = static_cast<int32_t*>(report->data_ptr());
-  words[0] = 0;  // (the thread's previous call on this stream has been waited for)
+  words[0] = words[3] = 0;  // (the thread's previous call on this stream has its outcome: nothing writes them any more)
   int rc;
   {
     WithoutGil released;
@@ -355,7 +369,8 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
         static_cast<int>(batch), static_cast<int>(total), static_cast<int>(heads), static_cast<int>(kv_heads),
         static_cast<int>(dim), page, static_cast<int>(kc->size(0)), width, static_cast<float>(scale),
         static_cast<int32_t*>(status->data_ptr()), need > 0 ? ws.data_ptr() : nullptr, need, words, stream);
-    if (rc == PRISM_OK) C10_HIP_CHECK(hipStreamSynchronize(static_cast<hipStream_t>(stream)));
+    if (rc == PRISM_OK && (!sixteen || !outcome_known(words + 3, stream) || *static_cast<volatile int32_t*>(words) != 0))
+      C10_HIP_CHECK(hipStreamSynchronize(static_cast<hipStream_t>(stream)));
   }
   if (rc != PRISM_OK) Py_RETURN_NONE;
   const volatile int32_t* r = words;

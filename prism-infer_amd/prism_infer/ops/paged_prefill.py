@@ -15,10 +15,12 @@ prefill (prism_infer/layers/attention.py:448-459):
 
 The reference loops over sequences on the host (one ``.item()`` sync per
 sequence) and gathers pages into dense tensors.  Here one kernel launch
-reads the pages in place, with the metadata on the device, and the host
-synchronises once at the end to raise the reference's errors: invalid
-lengths, a block id past the cache, or a block table too short for the
-context.  Under graph capture that check is skipped (invalid sequences then
+reads the pages in place, with the metadata on the device, and the host waits
+once to raise the reference's errors: invalid lengths, a block id past the
+cache, or a block table too short for the context.  Over FP8 caches it waits
+for the result; over 16-bit caches only until the metadata is checked, which
+the launch does first (the result is then ready in stream order, as any
+op's).  Under graph capture that check is skipped (invalid sequences then
 leave their rows unspecified).
 
 Differences a caller can see: K/V are dequantised in fp32 (payload times
@@ -52,8 +54,8 @@ _STATUS_OK = 2**31 - 1
 
 # Per thread and (device, stream): the status word, which holds _STATUS_OK
 # between calls, and the pinned words that a call's outcome is read from.  A call
-# waits for its stream before it returns, so a thread's next call finds them
-# free; other threads have their own.
+# waits for its outcome before it returns, after which nothing writes them, so a
+# thread's next call finds them free; other threads have their own.
 _OUTCOME = threading.local()
 _MAX_OUTCOME_STREAMS = 16
 
@@ -73,7 +75,7 @@ def _add_outcome_buffers(buffers: dict, device: torch.device) -> None:
     if len(buffers) >= _MAX_OUTCOME_STREAMS:
         buffers.clear()
     status = torch.full((1,), _STATUS_OK, dtype=torch.int32, device=device)
-    buffers[key] = (status, torch.empty(3, dtype=torch.int32, pin_memory=True))
+    buffers[key] = (status, torch.empty(4, dtype=torch.int32, pin_memory=True))
 
 
 def _validate_caches(k_cache, v_cache, k_scale_cache, v_scale_cache) -> bool:

@@ -126,6 +126,48 @@ def test_paged(host, dtype, dim):
     assert torch.equal(call(), host.python(call))
 
 
+@pytest.mark.parametrize("batch,page,longest", [(1, 16, 9000), (3, 64, 700), (300, 16, 60), (600, 32, 40)])
+def test_paged_outcome_is_known_before_the_result(host, batch, page, longest):
+    """The metadata's check sees every length and every needed block id, and no other; good calls follow one another."""
+
+    _, paged, _ = _modules()
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(1, longest + 1, (batch,), generator=g)
+    lens[batch // 2] = longest
+    width = -(-longest // page) + 2
+    k, v = (torch.randn(64, page, 1, 64, generator=g).to(BF16).cuda() for _ in range(2))
+    q = torch.randn(batch, 2, 64, generator=g).to(BF16).cuda()
+    tables = torch.randint(0, 64, (batch, width), generator=g, dtype=torch.int32)
+    tables.masked_fill_(torch.arange(width)[None, :] >= -(-lens[:, None] // page), 10**6)  # (not needed: anything)
+    good, good_lens = tables.cuda(), lens.int().cuda()
+    ctx = SimpleNamespace(block_tables=good.clone(), context_lens=good_lens.clone(),
+                          cu_seqlens_q=torch.arange(batch + 1, dtype=torch.int32, device="cuda"))
+
+    def call():
+        return paged.paged_prefill_attention(q, k, v, ctx, num_heads=2, num_kv_heads=1, scale=0.1)
+
+    want = host.python(call)
+    call()
+    host.taken["prefill"] = 0
+    outs = [call() for _ in range(20)]
+    assert all(torch.equal(o, want) for o in outs) and host.taken["prefill"] == 20
+    for seq in {0, batch // 2, batch - 1}:
+        last = -(-int(lens[seq]) // page) - 1
+        for entry in {0, last}:
+            for bad in (-1, 64):
+                ctx.block_tables[seq, entry] = bad
+                with pytest.raises(RuntimeError, match="exceeds cache capacity|invalid block table"):
+                    call()
+                ctx.block_tables.copy_(good)
+        for bad in (0, width * page + 1):
+            ctx.context_lens[seq] = bad
+            with pytest.raises(RuntimeError, match="invalid paged prefill lengths|invalid block table|exceeds cache capacity"):
+                call()
+            ctx.context_lens.copy_(good_lens)
+        assert torch.equal(call(), want)
+    assert torch.equal(call(), want)
+
+
 def test_metadata(host):
     _, _, meta = _modules()
     tables = torch.arange(40, dtype=torch.int32, device="cuda").view(5, 8)
