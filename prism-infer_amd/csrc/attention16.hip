@@ -488,7 +488,8 @@ attention16_kernel(const AttnArgs a) {
   // The table is walked tile by tile; 64 consecutive entries sit in one register.
   constexpr int kGroups = SRC == kSmallPages ? kKeys / 16 : 1;  // entries per tile
   struct Place {
-    int blk[kGroups], row[kGroups];  // page (-1: not needed) and first row in it, per group
+    int blk[kGroups];  // pages, per 16 keys where a tile may lie in several (-1: not needed)
+    int row;           // of the first key in its page
     bool ok;
   };
   int page = 0, page_row = 0, ids_base = 0, ids = 0;
@@ -504,10 +505,10 @@ attention16_kernel(const AttnArgs a) {
     Place p;
     p.ok = true;
     if constexpr (SRC != kPacked) {
+      p.row = page_row;
 #pragma unroll
       for (int x = 0; x < kGroups; ++x) {
         p.blk[x] = -1;
-        p.row[x] = page_row;
         if (SRC == kPages || t * kKeys + x * 16 < kend) {  // groups past the keys needed are not looked up
           if (page >= ids_base + 64) {
             ids_base = page;
@@ -549,11 +550,14 @@ attention16_kernel(const AttnArgs a) {
         r = min(lrow + tr, klen - 1 - t * kKeys);  // (rows past the last key repeat it)
       } else {
         const int x = SRC == kPages ? 0 : uniform_int((tr + wave * kLoadRows) / 16);
-        int b = place.blk[0], p = place.row[0] + tr;
+        int b = place.blk[0], p = place.row + 16 * x;
 #pragma unroll
-        for (int y = 1; y < kGroups; ++y)
-          if (x == y) b = place.blk[y], p = place.row[y] + tr - 16 * y;
+        for (int y = 1; y < kGroups; ++y) {
+          if (x == y) b = place.blk[y];
+          if (p >= a.page) p -= a.page;
+        }
         if (SRC == kSmallPages && b < 0) continue;
+        p += tr - 16 * x;
         base = head_base + b * page_bytes + static_cast<int64_t>(p) * st_bytes;
         r = lrow;
       }
