@@ -380,7 +380,9 @@ int prism_paged_prefill_ws(const void* q, int q_dtype, const int64_t q_strides[3
  * out        : [total_q, num_heads, head_dim] of dtype, 16-byte aligned rows.
  *              Rows that see no key, and rows outside [cu_seqlens_q[0],
  *              cu_seqlens_q[batch]), are 0.  A sequence whose offsets are out of
- *              order or outside the tensors is left out, its rows unspecified.
+ *              order or outside the tensors is left out, its rows unspecified;
+ *              so are all rows where sequences share some.  total_q * num_heads /
+ *              num_kv_heads is at most 2^29.
  * workspace  : device scratch (256-byte aligned, any contents) of at least
  *              prism_prompt_attention_workspace_bytes() bytes for the same
  *              geometry, which is 0 where none is used.  With it the keys of few,

@@ -18,12 +18,16 @@
 // type (weights of at most 2^8 against fp32 sums), is the B operand of O^T +=
 // V^T P^T as it stands, V^T comes from ds_read_b64_tr_b16.
 //
-// Bound by the MFMAs and the exponentials beside them: a wave's tile is 32
-// MFMAs of 32 cycles and about 112 VALU instructions, 32 of them exponentials
-// of 16 cycles, and two waves share a SIMD.  With the three parts of a tile one
-// after the other 2 x 8192 tokens (32 / 8 heads) took 1414 us; with the next
-// tile's scores and the last one's output beside the softmax 1055 (1042
-// TFLOP/s, 0.83 of a large library product on the same card).
+// Bound by the MFMAs (busy 70% of the cycles) and the exponentials beside them: a
+// wave's tile is 32 MFMAs of 32 cycles and about 112 VALU instructions, 32 of
+// them exponentials of 16 cycles, and two waves share a SIMD.  With the three
+// parts of a tile one after the other 2 x 8192 tokens (32 / 8 heads) took 1414
+// us; with the next tile's scores and the last one's output beside the softmax
+// 975 to 1013 (1085 to 1130 TFLOP/s, 0.88 of a large library product on the same
+// card).  Prompts of one to three tiles are bound by what is around the loop:
+// lookup, first loads and scores, last values, stores (80 prompts of 100 tokens,
+// 64 / 8 heads: 133 us with stores of 8 bytes a lane, dependent reads in the last
+// product and a division per use, 91 now).
 #include "common.h"
 #include "divide.h"
 #include "wave_ops.h"
@@ -38,8 +42,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kKeys = 64;              // keys per tile
-constexpr int kWaves = 4;              // per workgroup
+constexpr int kWaves = 4;              // per group of waves
 constexpr int kMostKeys = 0x7FFFF000;  // of a sequence: positions a few tiles further fit in 32 bits
+constexpr int kMostRows = 1 << 29;     // of a kv head: sums of blocks over 256 sequences fit in 32 bits
 constexpr int kCols = 32;              // rows per wave: the columns of a 32x32 MFMA
 constexpr float kSumLimit = 256.0f;    // largest sum of a lane's 32 weights that keeps the running max
 
@@ -99,7 +104,6 @@ struct Type;
 template <>
 struct Type<false> {
   typedef bf16x8 vec;
-  typedef __bf16 elem;
   static constexpr uint32_t kInf = 0x7F80u;
   static __device__ __forceinline__ floatx16 mfma(vec a, vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -108,7 +112,6 @@ struct Type<false> {
 template <>
 struct Type<true> {
   typedef f16x8 vec;
-  typedef _Float16 elem;
   static constexpr uint32_t kInf = 0x7C00u;
   static __device__ __forceinline__ floatx16 mfma(vec a, vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -277,17 +280,17 @@ __device__ __forceinline__ bool locate(const AttnArgs& a, int me, bool flag, Wor
         }
       }
     } else {
-    auto above = [&](int u) { return wave_reduce(min(max(l0[0] + n[0] - 1 - max(u, l0[0] - 1), 0), n[0]), Add()); };
-    int lo = 0, hi = wave_reduce(top, Max());
-    while (lo < hi) {  // smallest level with at most `rank` blocks above it
-      const int mid = (lo + hi) / 2;
-      if (above(mid) <= rank) hi = mid;
-      else lo = mid + 1;
-    }
-    const int at = n[0] > 0 && lo >= l0[0] && lo < l0[0] + n[0] ? 1 : 0;
-    const int left = rank - above(lo), incl = wave_scan(at, Add());
-    l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left));
-    w.block = lo - __builtin_amdgcn_readlane(l0[0], l);
+      auto above = [&](int u) { return wave_reduce(min(max(l0[0] + n[0] - 1 - max(u, l0[0] - 1), 0), n[0]), Add()); };
+      int lo = 0, hi = wave_reduce(top, Max());
+      while (lo < hi) {  // smallest level with at most `rank` blocks above it
+        const int mid = (lo + hi) / 2;
+        if (above(mid) <= rank) hi = mid;
+        else lo = mid + 1;
+      }
+      const int at = n[0] > 0 && lo >= l0[0] && lo < l0[0] + n[0] ? 1 : 0;
+      const int left = rank - above(lo), incl = wave_scan(at, Add());
+      l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left));
+      w.block = lo - __builtin_amdgcn_readlane(l0[0], l);
     }
   }
   w.seq = l * K + hit_k;
@@ -317,13 +320,14 @@ __device__ __forceinline__ bool locate_many(const AttnArgs& a, int me, bool flag
   };
   w.total = 0;
   Seq s;
-  for (int base = 0; base < a.batch; base += 64) w.total += wave_reduce(blocks_of(base + lane, s, flag), Add());
+  // (sequences that overlap could make any number of blocks)
+  for (int base = 0; base < a.batch; base += 64) w.total = min(w.total + wave_reduce(blocks_of(base + lane, s, flag), Add()), 1 << 30);
   const int target = w.total - 1 - rank;
   if (target < 0) return false;
   int before = 0;
   for (int base = 0; base < a.batch; base += 64) {
     const int n = blocks_of(base + lane, s, false);
-    const int incl = wave_scan(n, Add()) + before;
+    const int incl = wave_scan(n, Add()) + before;  // (at most 2^28 beyond the total's limit)
     const uint64_t hit = __builtin_amdgcn_ballot_w64(target < incl && target >= incl - n);
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
@@ -1091,13 +1095,13 @@ int launch(const AttnArgs& a, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.total_q) * a.group;
   // every sequence may end in a partial block; one more for rows outside them
   const int64_t blocks = (ceil_div(rows, kCols * kWaves) + a.batch + 1) * a.kv_heads;
-  if (blocks > INT32_MAX - 2 * a.kv_heads || rows > INT32_MAX - kBlockRows) {
+  const int64_t checks = SRC != kPacked && a.report != nullptr ? a.kv_heads : 0;
+  const int64_t grid = checks + (a.work == nullptr ? blocks : std::max<int64_t>(blocks, a.slots + a.kv_heads));  // (parts never outnumber the slots)
+  if (rows > kMostRows || grid * 64 * kWaves * GROUPS > UINT32_MAX) {
     set_error("attention over 16-bit keys: too many query rows for one launch");
     return PRISM_ERR_INVALID;
   }
-  const int64_t grid = a.work == nullptr ? blocks : std::max<int64_t>(blocks, a.slots + a.kv_heads);  // (parts never outnumber the slots)
-  const int64_t checks = SRC != kPacked && a.report != nullptr ? a.kv_heads : 0;
-  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC, GROUPS>), dim3(static_cast<unsigned>(grid + checks)), dim3(64 * kWaves * GROUPS), 0,
+  hipLaunchKernelGGL((attention16_kernel<F16, D, SRC, GROUPS>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves * GROUPS), 0,
                      stream, a);
   if (int rc = check_launch("attention16_kernel launch")) return rc;
   if (a.work == nullptr) return PRISM_OK;
@@ -1255,6 +1259,10 @@ extern "C" int prism_prompt_attention(const void* q, const int64_t q_strides[3],
   if (!q || !q_strides || !k_strides || !v_strides || !out || !out_strides || !cu_seqlens_q || !cu_seqlens_k ||
       (total_k > 0 && (!k || !v))) {
     set_error("prism_prompt_attention: null argument");
+    return PRISM_ERR_INVALID;
+  }
+  if (total_k > kMostKeys) {
+    set_error("prism_prompt_attention: too many keys, %d", total_k);
     return PRISM_ERR_INVALID;
   }
   if (int rc = check_layout("prism_prompt_attention", dtype, num_heads, num_kv_heads, head_dim, q, q_strides, k, k_strides,

@@ -372,8 +372,8 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (rc == PRISM_OK && (!sixteen || !outcome_known(words + 3, stream) || *static_cast<volatile int32_t*>(words) != 0))
       C10_HIP_CHECK(hipStreamSynchronize(static_cast<hipStream_t>(stream)));
   }
-  if (rc != PRISM_OK) Py_RETURN_NONE;
   const volatile int32_t* r = words;
+  if (rc != PRISM_OK || (sixteen && r[3] == 0)) Py_RETURN_NONE;
   const int row0 = r[1], row1 = r[2];
   const int bad = r[0] == 0 ? INT32_MAX : status->item<int32_t>();
   PyObject* wrapped = THPVariable_Wrap(std::move(out));
@@ -403,7 +403,7 @@ PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int64_t total_q = q->size(0), total_k = k->size(0), dim = q->size(2), batch = cq->numel() - 1;
   if (heads <= 0 || kv_heads <= 0 || heads > INT32_MAX || heads % kv_heads != 0 || q->size(1) != heads || k->size(1) != kv_heads ||
-      k->size(2) != dim || (dim != 64 && dim != 128) || total_q <= 0 || total_q > INT32_MAX || total_k <= 0 || total_k > INT32_MAX ||
+      k->size(2) != dim || (dim != 64 && dim != 128) || total_q <= 0 || total_q > (1 << 29) || total_k <= 0 || total_k > (1 << 29) ||
       batch < 0 || batch > INT32_MAX || ck->numel() != cq->numel() || (same && total_k != total_q) || !aligned_rows(*q) ||
       !aligned_rows(*k) || !aligned_rows(*v))
     Py_RETURN_NONE;
@@ -452,7 +452,7 @@ PyObject* step_metadata(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int over1 = 0, over2 = 0;
   const long page = PyLong_AsLongAndOverflow(args[3], &over1), tokens = PyLong_AsLongAndOverflow(args[4], &over2);
   int device;
-  if (over1 || over2 || page <= 0 || page > INT32_MAX || tokens < 0 || tokens > INT32_MAX - 4 ||
+  if (over1 || over2 || page <= 0 || page > INT32_MAX || tokens < 0 || tokens > (1 << 30) ||
       !on_current_device(device, bt, cached, fresh, free, start))
     Py_RETURN_NONE;
   if (bt->dim() != 2 || bt->scalar_type() != at::kInt || !int32_vector(*cached) || !int32_vector(*fresh) ||

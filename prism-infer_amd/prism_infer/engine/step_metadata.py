@@ -26,6 +26,7 @@ from prism_infer import _native
 _HOST = _native.host_ops()
 
 MAX_STEP_REQUESTS = 8192
+MAX_STEP_TOKENS = 2**30
 _FITS = 2**31 - 1
 
 
@@ -102,8 +103,8 @@ def build_step_metadata(
     ``ceil(cached / block_size)`` entries; the rest is ignored.  Blocks that new
     tokens need are taken from ``free_blocks``, request by request, from entry
     ``free_start`` (an int32 tensor of one value, default 0) on.  ``num_tokens``
-    is the number of token rows, which may exceed the tokens (padded rows get
-    slot -1).  ``out`` is filled in place, as a captured graph's buffers are; it
+    is the number of token rows, at most 2**30, which may exceed the tokens (padded
+    rows get slot -1).  ``out`` is filled in place, as a captured graph's buffers are; it
     must not share memory with the inputs.  All tensors are int32 on one device.
     Nothing is synchronised: requests that do not fit get -1 where a block is
     missing, and :meth:`StepMetadata.check` reports them.
@@ -117,6 +118,8 @@ def build_step_metadata(
     block_size, num_tokens = int(block_size), int(num_tokens)
     if block_size <= 0 or num_tokens < 0:
         raise ValueError(f"block_size must be positive and num_tokens not negative, got {block_size} and {num_tokens}")
+    if block_size > _FITS or num_tokens > MAX_STEP_TOKENS:
+        raise ValueError(f"block_size must be below 2**31 and num_tokens at most {MAX_STEP_TOKENS}, got {block_size} and {num_tokens}")
     if block_tables.ndim != 2 or cached_lens.ndim != 1 or query_lens.ndim != 1:
         raise ValueError("block_tables must be [B, W], cached_lens and query_lens [B], got "
                          f"{list(block_tables.shape)}, {list(cached_lens.shape)} and {list(query_lens.shape)}")

@@ -16,7 +16,9 @@ when nothing is cached in front of a prompt (prism_infer/layers/attention.py:
 
 The offsets stay on the device and the call does not synchronise: it can be
 captured, and a replay follows the offsets of its time.  A sequence whose offsets
-are out of order or outside the tensors is left out; its rows are unspecified.
+are out of order or outside the tensors is left out; its rows are unspecified, and
+so are all rows where sequences share some.  A call takes up to 2**29 query rows
+per kv head and as many keys.
 There is no backward pass: inputs that require gradients are refused while
 gradients are recorded.
 """
@@ -31,10 +33,13 @@ HAS_HIP_KERNELS = _native.available()
 _HOST = _native.host_ops()
 
 PROMPT_HEAD_DIMS = (64, 128)
+MAX_PROMPT_TOKENS = 2**29
 PROMPT_DTYPES = (torch.bfloat16, torch.float16)
 
 
 def _validate_prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, num_heads: int, num_kv_heads: int) -> None:
+    same_tokens = cu_seqlens_k is None
+    cu_seqlens_k = cu_seqlens_q if same_tokens else cu_seqlens_k
     if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
         raise ValueError(
             "num_heads must be divisible by num_kv_heads, "
@@ -56,7 +61,7 @@ def _validate_prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, num_heads: i
     if cu_seqlens_k.numel() != cu_seqlens_q.numel():
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have the same length, "
                          f"got {cu_seqlens_q.numel()} and {cu_seqlens_k.numel()}")
-    if cu_seqlens_k is cu_seqlens_q and k.shape[0] != q.shape[0]:
+    if same_tokens and k.shape[0] != q.shape[0]:
         raise ValueError("without cu_seqlens_k q, k and v must have the same tokens, "
                          f"got {q.shape[0]} and {k.shape[0]}")
 
@@ -79,9 +84,11 @@ def prompt_attention(
         out = _HOST.prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, num_heads, num_kv_heads, scale)
         if out is not None:
             return out
+    _validate_prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, num_heads, num_kv_heads)
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
-    _validate_prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, num_heads, num_kv_heads)
+    if max(q.shape[0], k.shape[0]) > MAX_PROMPT_TOKENS:
+        raise RuntimeError(f"prompt_attention takes at most {MAX_PROMPT_TOKENS} tokens, got {q.shape[0]} and {k.shape[0]}")
     _native.lib()  # raises with the reason the library is unavailable
     tensors = (q, k, v, cu_seqlens_q, cu_seqlens_k)
     if not all(t.is_cuda for t in tensors) or any(t.device != q.device for t in tensors):

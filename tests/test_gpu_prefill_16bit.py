@@ -84,6 +84,49 @@ def test_short_chunks_behind_long_contexts(page, dtype):
     assert_within(_run(c), *_want(c))
 
 
+@pytest.mark.parametrize("seqs,heads,kv_heads,dim", [([(1000, 1000)], 32, 8, 128), ([(600, 1003), (520, 700)], 32, 8, 128),
+                                                     ([(1001, 1200)], 20, 20, 64)])
+@pytest.mark.parametrize("page,dtype", [(64, BF16), (16, F16)])
+def test_as_many_blocks_as_cus(page, dtype, seqs, heads, kv_heads, dim):
+    require_gpu()
+    c = _case(dim + page, seqs, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype)
+    assert_within(_run(c), *_want(c))
+
+
+def test_threads_on_streams_of_their_own():
+    """Each thread finds its own outcomes: results of its own lengths, and its own bad table."""
+
+    require_gpu()
+    import threading
+
+    cases = [_case(40 + i, [(30 + i, 400 + 90 * i), (5, 60)], page=16) for i in range(4)]
+    wants = [_want(c) for c in cases]
+    failed, start = [], threading.Barrier(len(cases))
+
+    def work(i):
+        try:
+            c = cases[i]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for turn in range(20):
+                    if (turn + i) % 5 == 0:
+                        tables = c.tables.clone()
+                        tables[i % 2, 1] = c.k.shape[0]
+                        with pytest.raises((ValueError, RuntimeError, IndexError)):
+                            _run(c, tables=tables)
+                    else:
+                        assert_within(_run(c), *wants[i])
+        except BaseException as e:  # noqa: BLE001 (reported by the test's own thread)
+            failed.append((i, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
 def test_large_batch_and_ragged_chunks():
     require_gpu()
     g = torch.Generator().manual_seed(6)

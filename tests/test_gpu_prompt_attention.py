@@ -79,6 +79,33 @@ def test_keys_split_over_workgroups(batch, heads, kv_heads, longest, dtype, dim)
     _check(q, k, v, cu_q, cu_k)
 
 
+# few long sequences whose blocks are about as many as the CUs of a chip with 256: (query lengths, more keys, heads, kv heads)
+WIDE = [([1000], [0], 32, 8, 128), ([600, 520], [400, 180], 32, 8, 128), ([1001], [0], 20, 20, 64), ([2040, 7], [9, 0], 16, 16, 64),
+        ([200, 200, 112], [2800, 700, 288], 32, 8, 128)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lq,more,heads,kv_heads,dim", WIDE)
+def test_as_many_blocks_as_cus(lq, more, heads, kv_heads, dim, dtype):
+    require_gpu()
+    lk = [n + m for n, m in zip(lq, more)]
+    cu_q, cu_k = offsets(lq, 3), offsets(lk, 5)
+    q, k, v = _inputs(25 + dim, cu_q[-1] + 2, cu_k[-1] + 1, heads, kv_heads, dim, dtype)
+    want, bound = packed_attention64(q, k, v, cu_q, cu_k, dim ** -0.5)
+    k[:5] = k[-1:] = v[:5] = v[-1:] = float("nan")
+    assert_within(_op(q.cuda(), k.cuda(), v.cuda(), cu_q, cu_k=cu_k), want, bound)
+
+
+@pytest.mark.parametrize("what", ["nan", "-inf"])
+def test_no_numbers_where_blocks_are_as_many_as_cus(what):
+    require_gpu()
+    q, k, v = _inputs(26, 1001, 1001, 20, 20, 64, BF16)
+    v[300, 2, 5] = v[850, 7, 60] = float(what)
+    want, bound = attention64(q, k, v, 0.125)
+    assert not want.isfinite().all()
+    assert_within(_op(q.cuda(), k.cuda(), v.cuda(), [0, 1001]), want, bound)
+
+
 def test_split_is_the_same_in_a_captured_graph():
     require_gpu()
     from prism_infer.ops.prompt_attention import prompt_attention
@@ -231,6 +258,39 @@ def test_offsets_out_of_order_leave_the_other_sequences_alone():
         first = 0 if a == 0 else 40
         want, bound = attention64(q[first:b], k[first:b], v[first:b], 128 ** -0.5)
         assert_within(got[a:b], want[a - first:], bound[a - first:], f"rows {a}..{b}")
+
+
+def test_no_keys_and_no_queries():
+    require_gpu()
+    q, k, v = (x.cuda() for x in _inputs(22, 30, 30, 4, 2, 64, BF16))
+    assert (_op(q, k[:0], v[:0], [0, 10, 30], cu_k=[0, 0, 0]) == 0).all()
+    assert _op(q[:0], k, v, [0, 0], cu_k=[0, 30]).shape == (0, 4, 64)
+    assert _op(q[:0], k[:0], v[:0], [0]).shape == (0, 4, 64)
+
+
+def test_the_same_offsets_passed_twice_over_longer_keys():
+    require_gpu()
+    from prism_infer.ops.prompt_attention import prompt_attention
+
+    q, k, v = _inputs(23, 50, 60, 4, 2, 128, BF16)
+    cu = torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda")
+    got = prompt_attention(q.cuda(), k.cuda(), v.cuda(), cu, num_heads=4, num_kv_heads=2, scale=0.1, cu_seqlens_k=cu)
+    want, bound = packed_attention64(q, k, v, [0, 20, 50], [0, 20, 50], 0.1)
+    assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("batch", [40, 200, 3001])
+def test_offsets_that_go_back_and_forth(batch):
+    """Sequences that overlap write the same rows over and over, or not at all where they go back; nothing else."""
+
+    require_gpu()
+    q, k, v = (x.cuda() for x in _inputs(24, 150, 150, 2, 1, 64, BF16))
+    cu = [150 * (i % 2) for i in range(batch + 1)]
+    guard = torch.zeros(1 << 20, device="cuda")
+    got = _op(q, k, v, cu)
+    assert got.shape == q.shape and (guard == 0).all()
+    want, bound = attention64(q.cpu(), k.cpu(), v.cpu(), 64 ** -0.5)
+    assert_within(_op(q, k, v, [0, 150]), want, bound)
 
 
 def test_captured_and_replayed_with_other_offsets_on_another_stream():

@@ -86,6 +86,8 @@ def test_no_requests_and_no_tokens():
     _same(_build(torch.zeros(0, 4, dtype=torch.int32), [], [], 16, 6, []), plain(torch.zeros(0, 4), [], [], 16, 6, []))
     case = (torch.tensor([[7, -1]], dtype=torch.int32), [16], [0], 16, 0, [])
     _same(_build(*case), plain(*case))
+    case = (torch.zeros(3, 0, dtype=torch.int32), [0, 0, 5], [0, 2, 1], 16, 8, [4])  # tables without entries
+    _same(_build(*case), plain(*case))
 
 
 @pytest.mark.parametrize("what", ["free", "width", "tokens", "negative", "start", "held", "huge"])

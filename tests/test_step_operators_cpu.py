@@ -30,6 +30,14 @@ def test_prompt_attention_contract(kw, match):
         _prompt(**kw)
 
 
+def test_prompt_attention_takes_only_so_many_tokens():
+    from prism_infer.ops.prompt_attention import MAX_PROMPT_TOKENS, prompt_attention
+
+    x = torch.zeros(1, 1, 64, dtype=BF16).expand(MAX_PROMPT_TOKENS + 1, 1, 64)
+    with pytest.raises(RuntimeError, match="at most"):
+        prompt_attention(x, x, x, torch.tensor([0, 1], dtype=torch.int32), num_heads=1, num_kv_heads=1, scale=0.1)
+
+
 def test_prompt_attention_has_no_cpu_path():
     with pytest.raises(RuntimeError, match="runs on the GPU|not built|cannot load"):
         _prompt()
@@ -58,7 +66,8 @@ def _meta(tables=(2, 3), cached=2, new=2, dtype=torch.int32, size=16, tokens=4, 
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(size=0), "positive"), (dict(tokens=-1), "not negative"), (dict(tables=(2,)), "block_tables must be"),
+    (dict(size=0), "positive"), (dict(tokens=-1), "not negative"), (dict(size=2**31), "below"),
+    (dict(tokens=2**30 + 1), "at most"), (dict(tables=(2,)), "block_tables must be"),
     (dict(cached=3), "one entry per request"), (dict(new=1), "one entry per request"), (dict(dtype=torch.int64), "torch.int32"),
     (dict(free_blocks=torch.zeros(2, 2, dtype=torch.int32)), "one-dimensional"),
     (dict(free_start=torch.zeros(2, dtype=torch.int32)), "one value"),
@@ -95,7 +104,8 @@ def test_abi_refuses_before_any_launch():
     assert prompt(dtype=0)[0] == -2 and prompt(dtype=3)[0] == -2 and prompt(d=96)[0] == -2
     assert prompt(q=p + 2)[0] == -2 and prompt(ks=_native.int64s(513, 128, 1))[0] == -2
     assert "span" in prompt(ks=_native.int64s(2**30, 128, 1))[1]
-    assert "too many" in prompt(tq=2**31 - 1, h=8, hk=1)[1]
+    assert "too many" in prompt(tq=2**31 - 1, h=8, hk=1)[1] and "too many" in prompt(tq=2**29 + 1)[1]
+    assert "too many" in prompt(tq=2**28, h=64, hk=64)[1] and "too many" in prompt(tk=2**31 - 1)[1]
     assert prompt(tq=0, q=None, out=None)[0] == 0
 
     def paged(q_dtype=1, dtype=1, d=128, page=16, ks=None, h=4, status=p):
