@@ -26,8 +26,8 @@
 // 975 to 1013 (1085 to 1130 TFLOP/s, 0.88 of a large library product on the same
 // card).  Prompts of one to three tiles are bound by what is around the loop:
 // lookup, first loads and scores, last values, stores (80 prompts of 100 tokens,
-// 64 / 8 heads: 133 us with stores of 8 bytes a lane, dependent reads in the last
-// product and a division per use, 91 now).
+// 64 / 8 heads: 133 us with loads and stores of parts of lines, dependent reads in
+// the last product and a division per use, 87 now).
 #include "common.h"
 #include "divide.h"
 #include "wave_ops.h"
@@ -346,8 +346,7 @@ __device__ __forceinline__ bool locate_many(const AttnArgs& a, int me, bool flag
 // before the others are done: every sequence's lengths and block ids.  Threads
 // are spread over the sequences first, then over a sequence's pages.
 template <int SRC>
-__device__ void check_metadata(const AttnArgs& a) {
-  __shared__ int first_bad;
+__device__ void check_metadata(const AttnArgs& a, int& first_bad) {  // (in LDS)
   constexpr int kAtOnce = 8;
   const int tid = threadIdx.x, threads = blockDim.x;
   if (tid == 0) first_bad = INT32_MAX;
@@ -426,7 +425,7 @@ attention16_kernel(const AttnArgs a) {
   constexpr int kLoadRows = 1024 / kRow;      // rows per load of a wave
   constexpr int kLoads = kKeys / kLoadRows / kWaves;
   constexpr int kV = 2 * kPayload;            // two stages of K, then two of V
-  constexpr int kShare = 4 * kPayload;        // of a group
+  constexpr int kShare = 4 * kPayload + 2 * kCols * kRow;  // of a group, with the last two waves' queries
   __shared__ __attribute__((aligned(256))) uint8_t lds[GROUPS * kShare];
 
   // With a report the first workgroups (one per kv head, which keeps the others'
@@ -434,7 +433,7 @@ attention16_kernel(const AttnArgs a) {
   const int checks = SRC != kPacked && a.report != nullptr ? a.kv_heads : 0;
   const int me = static_cast<int>(blockIdx.x) - checks;
   if (me < 0) {
-    if (blockIdx.x == 0) check_metadata<SRC>(a);
+    if (blockIdx.x == 0) check_metadata<SRC>(a, *reinterpret_cast<int*>(lds));
     return;
   }
   Work work;
@@ -583,37 +582,23 @@ attention16_kernel(const AttnArgs a) {
     }
   }
 
-  // the lane's row: column c
-  auto row_at = [&](int& tok, int& head) {
-    const int row = row0 + c;
-    tok = divide(row, a.by_group);
-    head = h * a.group + (row - tok * a.group);
-    return row < rows;
-  };
-  int pos;  // position of the row's token, below 0 where it sees no key (and without a row)
+  // The queries: whole rows through LDS (where V of the second tile goes, and
+  // behind the stages), swizzled as K's.  (16 bytes a lane of 32 rows at a time, as
+  // the MFMA wants them, take four loads per line: 80 prompts of 100 tokens 94 us, 87 now.)
+  const int pos = row0 + c < rows ? prefix + divide(row0 + c, a.by_group) : -1;  // of the lane's row; below 0: it sees no key, or is none
+  const uint32_t q_lds = wave < 2 ? kV + wave * kCols * kRow : 4 * kPayload + (wave - 2) * kCols * kRow;
+#pragma unroll
+  for (int l = 0; l < kCols / kLoadRows; ++l) {
+    const int r = l * kLoadRows + lane / (64 / kLoadRows), row = min(row0 + r, rows - 1);
+    const int tok = divide(row, a.by_group), head = h * a.group + (row - tok * a.group);
+    const uint16_t* src = a.q + static_cast<int64_t>(qs + tok) * a.q_st + static_cast<int64_t>(head) * a.q_sh +
+                          8 * ((lane % (64 / kLoadRows)) ^ swz<D>(r));
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 : : "v"(src), "s"(uniform_int(lds0 + q_lds + l * 1024)) : "memory", "m0");
+  }
+
   vec qop[kSteps];
-  {
-    int tok, head;
-    const bool real = row_at(tok, head);
-    pos = real ? prefix + tok : -1;
-    const uint16_t* src = a.q + static_cast<int64_t>(qs + tok) * a.q_st + static_cast<int64_t>(head) * a.q_sh + 8 * g;
-#pragma unroll
-    for (int x = 0; x < kSteps; ++x)
-      qop[x] = __builtin_bit_cast(vec, real ? *reinterpret_cast<const u32x4*>(src + 16 * x) : u32x4{0, 0, 0, 0});
-  }
-  // The exponent's scale is positive, so that a masked score is -inf: a negative
-  // one is the queries' sign, and with 0 all queries are 0.
   const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  if (a.scale_log2 <= 0.f) {
-    const uint32_t keep = a.scale_log2 == 0.f ? 0u : ~0u;
-#pragma unroll
-    for (int x = 0; x < kSteps; ++x) {
-      u32x4 w = __builtin_bit_cast(u32x4, qop[x]);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) w[d] = (w[d] & keep) ^ (0x80008000u & keep);
-      qop[x] = __builtin_bit_cast(vec, w);
-    }
-  }
 
   // per-lane LDS offsets inside a stage; other chunks differ by an exclusive or
   const uint32_t k_rd = c * kRow + ((g ^ swz<D>(c)) << 4);
@@ -723,6 +708,21 @@ attention16_kernel(const AttnArgs a) {
     uint32_t k_next = kPayload, v_prev = kV;  // stages of K of tile t + 1 and V of tile t - 1
     landed();
     barrier();
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) qop[x] = __builtin_bit_cast(vec, *reinterpret_cast<const u32x4*>(share + ((q_lds + k_rd) ^ (x << 5))));
+    // The exponent's scale is positive, so that a masked score is -inf: a negative
+    // one is the queries' sign, and with 0 all queries are 0, as they are without a row.
+    if (a.scale_log2 <= 0.f || row0 + kCols > rows) {
+      const uint32_t keep = a.scale_log2 == 0.f || row0 + c >= rows ? 0u : ~0u;
+      const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u & keep : 0u;
+#pragma unroll
+      for (int x = 0; x < kSteps; ++x) {
+        u32x4 w = __builtin_bit_cast(u32x4, qop[x]);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) w[d] = (w[d] & keep) ^ flip;
+        qop[x] = __builtin_bit_cast(vec, w);
+      }
+    }
     floatx16 sa[2], sb[2];
     u32x4 pa[4], pb[4];
     if (t0 < tw) {
@@ -940,7 +940,7 @@ attention16_kernel(const AttnArgs a) {
   if constexpr (GROUPS > 1) {
     // The second group's waves leave their outputs in its stages, lane by lane, for
     // the first one's to join.
-    static_assert(GROUPS == 2 && kWaves * kDims * 4 * 1024 == kShare, "an output fills a group's stages");
+    static_assert(GROUPS == 2 && kWaves * kDims * 4 * 1024 == 4 * kPayload, "an output fills a group's stages");
     barrier();  // (every wave is past its last values)
     uint8_t* const theirs = lds + kShare + wave * kDims * 4 * 1024 + lane * 16;
     if (group == 1) {
