@@ -27,7 +27,7 @@
 // card).  Prompts of one to three tiles are bound by what is around the loop:
 // lookup, first loads and scores, last values, stores (80 prompts of 100 tokens,
 // 64 / 8 heads: 133 us with loads and stores of parts of lines, dependent reads in
-// the last product and a division per use, 87 now).
+// the last product and a division per use, 74 now).
 #include "common.h"
 #include "divide.h"
 #include "wave_ops.h"
@@ -987,7 +987,8 @@ attention16_kernel(const AttnArgs a) {
     if (g == 0) *reinterpret_cast<floatx2*>(scratch.ml + 2 * cell) = floatx2{m_run, l_tot};
     return;
   }
-  // Rows leave through LDS, so that a store covers whole rows.  Chunks are
+  // Rows leave through LDS, so that a store covers whole rows, and past the L2,
+  // which keeps K and V (80 prompts of 100 tokens 87 us, 74 so).  Chunks are
   // swizzled by row.
   const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // (a NaN sum makes the row NaN)
   constexpr int kChunks = kRow / 16;  // of an output row
@@ -1003,8 +1004,8 @@ attention16_kernel(const AttnArgs a) {
     const u32x4 x = *reinterpret_cast<const u32x4*>(mine + r * kRow + ((chunk ^ (r % kChunks)) << 4));
     const int at = divide(row, a.by_group), in_group = row - at * a.group;
     if (row < rows)
-      *reinterpret_cast<u32x4*>(a.out + static_cast<int64_t>(qs + at) * a.o_st + static_cast<int64_t>(h * a.group + in_group) * a.o_sh +
-                                8 * chunk) = x;
+      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(a.out + static_cast<int64_t>(qs + at) * a.o_st +
+                                                              static_cast<int64_t>(h * a.group + in_group) * a.o_sh + 8 * chunk));
   }
 }
 
