@@ -18,12 +18,12 @@
 // type (weights of at most 2^8 against fp32 sums), is the B operand of O^T +=
 // V^T P^T as it stands, V^T comes from ds_read_b64_tr_b16.
 //
-// Bound by the MFMAs (busy 70% of the cycles) and the exponentials beside them: a
+// Bound by the MFMAs (busy 71% of the cycles) and the exponentials beside them: a
 // wave's tile is 32 MFMAs of 32 cycles and about 112 VALU instructions, 32 of
 // them exponentials of 16 cycles, and two waves share a SIMD.  With the three
 // parts of a tile one after the other 2 x 8192 tokens (32 / 8 heads) took 1414
 // us; with the next tile's scores and the last one's output beside the softmax
-// 975 to 1013 (1085 to 1130 TFLOP/s, 0.88 of a large library product on the same
+// 946 to 1004 (1095 to 1162 TFLOP/s, 0.9 of a large library product on the same
 // card).  Prompts of one to three tiles are bound by what is around the loop:
 // lookup, first loads and scores, last values, stores (80 prompts of 100 tokens,
 // 64 / 8 heads: 133 us with loads and stores of parts of lines, dependent reads in
