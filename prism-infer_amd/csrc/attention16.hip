@@ -62,7 +62,7 @@ struct AttnArgs {
   int64_t bt_sb, bt_sn;
   const int32_t* ctx;   // paged: keys of each sequence
   const int32_t* cu_q;
-  const int32_t* cu_k;  // packed
+  const int32_t* cu_k;  // packed; null over pages
   uint16_t* out;
   int64_t o_st, o_sh;
   int batch, heads, kv_heads, group, page, num_blocks, width, total_q, total_k;
@@ -1113,7 +1113,7 @@ int launch(const AttnArgs& a, hipStream_t stream) {
 
 template <bool F16, int D, int GROUPS>
 int by_source(const AttnArgs& a, hipStream_t stream) {
-  if (a.bt == nullptr) return launch<F16, D, kPacked, GROUPS>(a, stream);
+  if (a.cu_k != nullptr) return launch<F16, D, kPacked, GROUPS>(a, stream);  // (a table without columns has no address)
   return a.page % kKeys == 0 ? launch<F16, D, kPages, GROUPS>(a, stream) : launch<F16, D, kSmallPages, GROUPS>(a, stream);
 }
 
@@ -1195,7 +1195,7 @@ int preload_attention16() {
   return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&attention16_kernel<false, 128, kPacked, 1>)), "preload_attention16");
 }
 
-// prism_paged_prefill_ws over 16-bit caches; its geometry and pointers are checked there.
+// prism_paged_prefill_ws over 16-bit caches; its geometry, strides and status are checked there.
 int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void* v, int dtype, const int64_t* ks,
                     const int64_t* vs, const int32_t* bt, const int64_t* bts, const int32_t* ctx, const int32_t* cu_q,
                     void* out, const int64_t* os, int batch, int total_q, int heads, int kv_heads, int head_dim, int page,
@@ -1207,6 +1207,11 @@ int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void*
     return PRISM_ERR_LAYOUT;
   }
   if (batch == 0 || total_q == 0) return PRISM_OK;
+  // (without columns, or without pages, every sequence is flagged before a table, or a cache, is read)
+  if (!q || !out || !ctx || !cu_q || (width > 0 && !bt) || (num_blocks > 0 && (!k || !v))) {
+    set_error("prism_paged_prefill: null argument");
+    return PRISM_ERR_INVALID;
+  }
   AttnArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_st = qs[0], a.q_sh = qs[1];
