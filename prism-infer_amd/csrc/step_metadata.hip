@@ -43,7 +43,7 @@ struct MetaArgs {
   int num_free, batch, width, page, num_tokens;
   Divisor by_page, by_row;  // by_row: entries of a table row, in steps of `wide`
   int wide;                 // table entries per thread: 4 where rows hold whole quads, else 1
-  int quads;                // the tables' rows can be loaded four entries at a time
+  int quads;                // of the tables: a thread's four entries can be loaded at once, they start on 16 bytes
   int32_t* slots;
   int32_t* positions;
   int32_t* cu;
@@ -257,7 +257,7 @@ extern "C" int prism_step_metadata(const int32_t* block_tables, const int64_t bt
   a.free_start = free_start;
   a.num_free = num_free, a.batch = batch, a.width = width, a.page = block_size, a.num_tokens = num_tokens;
   a.wide = width > 0 && width % 4 == 0 ? 4 : 1;
-  a.quads = a.t_sw == 1 && a.t_sb % 4 == 0 && aligned(block_tables, 16);
+  a.quads = a.wide == 4 && a.t_sw == 1 && a.t_sb % 4 == 0 && aligned(block_tables, 16);
   a.by_page = divisor(block_size);
   a.by_row = divisor(std::max(width / a.wide, 1));
   a.slots = packed;
