@@ -4,7 +4,8 @@
 //   o[j, h] = sum_{t <= p} w_t v[t, h / G],  w = softmax_t(scale q[j, h] . k[t, h / G]),  p = klen - qlen + j
 //
 // for token j of a sequence of qlen queries and klen keys (its last qlen tokens
-// are the queries'); a row that sees no key (p < 0) is 0.
+// are the queries'); a row that sees no key (p < 0) is 0, one whose visible
+// scores are all -inf is 0 / 0, NaN.
 //
 // Work layout.  The G query heads of a kv head share its keys, so the rows of
 // one kv head are (token, head in the group) pairs, token major: any group size
@@ -642,7 +643,7 @@ attention16_kernel(const AttnArgs a) {
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-    m_run = pos >= 0 ? -INFINITY : 0.f;  // (rows without a key would otherwise count as rising on every tile)
+    m_run = pos >= 0 ? -INFINITY : 0.f;  // 0 of a row without a key, to the end: it does not count as rising, and is told by it
     l_run = 0.f;
   };
   auto scores_step = [&](int x, const u32x4& k, floatx16& sc) {
@@ -990,7 +991,7 @@ attention16_kernel(const AttnArgs a) {
   // Rows leave through LDS, so that a store covers whole rows, and past the L2,
   // which keeps K and V (80 prompts of 100 tokens 87 us, 74 so).  Chunks are
   // swizzled by row.
-  const float inv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // (a NaN sum makes the row NaN)
+  const float inv = pos < 0 ? 0.f : 1.f / l_tot;  // (a sum of 0, all scores -inf, or a NaN one makes the row NaN)
   constexpr int kChunks = kRow / 16;  // of an output row
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
@@ -1028,6 +1029,7 @@ __global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a)
   const float* src = scratch.out + cell * D + lane * kPer;
   float m = -INFINITY, l = 0.f;
   vals o = {};
+  const bool none = ml->x == 0.f && ml->y == 0.f;  // the row sees no key: in every part a max of 0 and no sum
   for (int p0 = 0; p0 < b.parts; p0 += kBatch) {
     floatx2 x[kBatch];
     vals v[kBatch];
@@ -1055,7 +1057,7 @@ __global__ void __launch_bounds__(256) attention16_join_kernel(const AttnArgs a)
       for (int j = 0; j < kPer; ++j) o[j] = live ? fmaf(w, v[p][j], o[j]) : o[j];
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = none ? 0.f : 1.f / l;
   const int tok = divide(row, a.by_group), head = b.head * a.group + (row - tok * a.group);
   uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(b.qs + tok) * a.o_st +
                                               static_cast<int64_t>(head) * a.o_sh + lane * kPer);
