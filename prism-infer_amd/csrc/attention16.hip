@@ -16,8 +16,8 @@
 // Per tile a wave computes S^T = K Q^T with 32x32x16 MFMAs: a row is one lane
 // column from the scores to the output, so its running max, its sum and the
 // rescaling of its accumulators are lane-local.  P^T, rounded to the cache's
-// type (weights of at most 2^8 against fp32 sums), is the B operand of O^T +=
-// V^T P^T as it stands, V^T comes from ds_read_b64_tr_b16.
+// type (weights of at most 2^8, in float16 2^15, against fp32 sums), is the B
+// operand of O^T += V^T P^T as it stands, V^T comes from ds_read_b64_tr_b16.
 //
 // Bound by the MFMAs (busy 71% of the cycles) and the exponentials beside them: a
 // wave's tile is 32 MFMAs of 32 cycles and about 112 VALU instructions, 32 of
@@ -47,7 +47,6 @@ constexpr int kWaves = 4;              // per group of waves
 constexpr int kMostKeys = 0x7FFFF000;  // of a sequence: positions a few tiles further fit in 32 bits
 constexpr int kMostRows = 1 << 29;     // of a kv head: sums of blocks over 256 sequences fit in 32 bits
 constexpr int kCols = 32;              // rows per wave: the columns of a 32x32 MFMA
-constexpr float kSumLimit = 256.0f;    // largest sum of a lane's 32 weights that keeps the running max
 
 // Where keys come from: packed like the queries, pages that hold whole tiles,
 // or pages of a multiple of 16 keys.
@@ -102,18 +101,26 @@ struct SplitScratch {
 
 template <bool F16>
 struct Type;
+// kShift: weights are 2^kShift times exp(score - max) (the running max is kept less by
+// kShift, sums and outputs carry the same factor).  kSumLimit: largest sum of a
+// lane's 32 weights that keeps the running max, 8 times what the max itself allows.
 template <>
 struct Type<false> {
   typedef bf16x8 vec;
   static constexpr uint32_t kInf = 0x7F80u;
+  static constexpr float kShift = 0.f, kSumLimit = 256.f;
   static __device__ __forceinline__ floatx16 mfma(vec a, vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
+// float16 ends at 2^-24 and at 65504: the factor takes weights that small down to
+// 2^-31 of the max (40000 keys of 2^-24.6 beside one of 1 were off by half otherwise),
+// and the limit keeps every weight finite.
 template <>
 struct Type<true> {
   typedef f16x8 vec;
   static constexpr uint32_t kInf = 0x7C00u;
+  static constexpr float kShift = 7.f, kSumLimit = 32768.f;
   static __device__ __forceinline__ floatx16 mfma(vec a, vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -669,7 +676,7 @@ attention16_kernel(const AttnArgs a) {
 #pragma unroll
     for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, fmaxf(sc[0][r], sc[1][r]));
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
-    tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale;
+    tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale - T::kShift;
     const float m_new = tmax > m_run ? tmax : m_run;
     // (no key seen: keep the accumulators, all zero, from (-inf) - (-inf))
     const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
@@ -794,7 +801,7 @@ attention16_kernel(const AttnArgs a) {
       // whether that was low enough, or is no number.  Only otherwise are maxima
       // taken.  (The pins keep the weights in front of the branch.)
       asm volatile("" : "+v"(ps), "+v"(pn[0]), "+v"(pn[1]), "+v"(pn[2]), "+v"(pn[3]));
-      if (__builtin_amdgcn_ballot_w64(!(ps <= kSumLimit)) != 0) settle(sc, pn, ps);
+      if (__builtin_amdgcn_ballot_w64(!(ps <= T::kSumLimit)) != 0) settle(sc, pn, ps);
       l_run += ps;
     };
     // The step that begins iteration t of every wave: K of tile t + 1 and V of
