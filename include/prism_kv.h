@@ -316,6 +316,8 @@ int prism_device_copy(void* dst, const void* src, int64_t nbytes, int workgroups
  *              at position context_lens[i] - query_len_i + j and attends to
  *              keys 0 .. that position.
  * out        : [total_q, num_heads, head_dim] of q_dtype, strides out_strides.
+ *              Rows outside [cu_seqlens_q[0], cu_seqlens_q[batch]) become 0 over
+ *              16-bit caches and are not written over FP8 ones.
  * status     : device int32[1], set by the caller to INT32_MAX.  A sequence
  *              whose lengths are invalid (query_len <= 0, context_len <
  *              query_len, context_len > width * page_size) or whose needed

@@ -387,13 +387,13 @@ __device__ void check_metadata(const AttnArgs& a, int& first_bad) {  // (in LDS)
 // Rows outside every sequence are 0: the workgroups beyond the real blocks
 // (one per kv head at least) share them.
 template <int D>
-__device__ void zero_padding(const AttnArgs& a, int real_blocks) {
+__device__ void zero_padding(const AttnArgs& a, int checks, int real_blocks) {
   const int first = min(max(a.cu_q[0], 0), a.total_q), end = min(max(a.cu_q[a.batch], first), a.total_q);
-  const int me = static_cast<int>(blockIdx.x) - real_blocks * a.kv_heads;
-  const int64_t workers = static_cast<int64_t>(gridDim.x) - static_cast<int64_t>(real_blocks) * a.kv_heads;
+  const int64_t others = checks + static_cast<int64_t>(real_blocks) * a.kv_heads;
+  const int64_t me = blockIdx.x - others, workers = gridDim.x - others;
   const int64_t per_row = static_cast<int64_t>(a.heads) * (D / 8);
   const int64_t chunks = (first + (a.total_q - end)) * per_row;
-  for (int64_t x = static_cast<int64_t>(me) * blockDim.x + threadIdx.x; x < chunks; x += workers * blockDim.x) {
+  for (int64_t x = me * blockDim.x + threadIdx.x; x < chunks; x += workers * blockDim.x) {
     int64_t row = x / per_row;
     const int rest = static_cast<int>(x - row * per_row);
     if (row >= first) row += end - first;
@@ -450,7 +450,11 @@ attention16_kernel(const AttnArgs a) {
                      : a.batch <= 256 ? locate<SRC, kRows, 4>(a, me, first_wave, work) : locate_many<SRC, kRows>(a, me, first_wave, work);
   if (me == 0 && threadIdx.x == 0 && a.work != nullptr) *SplitScratch(a.work, a.slots, D).count = work.split * a.kv_heads;
   if (!found) {
-    if (SRC == kPacked) zero_padding<D>(a, work.total);
+    // (Its arguments are loaded anew: shared with the loop, they take scalar registers
+    // there and pages' places spill; 2 chunks behind 12000 104 us, 106 with them shared.)
+    auto* args = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    zero_padding<D>(*(const AttnArgs*)args, checks, work.total);
     return;
   }
   const int seq = uniform_int(work.seq), block = uniform_int(work.block), h = uniform_int(work.head);

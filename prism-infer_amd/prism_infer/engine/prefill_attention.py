@@ -31,8 +31,9 @@ class PagedKVPrefillAttention(PagedKVDecodeAttention):
 
         ``cached_prefix`` says whether any sequence has stored tokens in front of
         this chunk, which the host knows.  Without, the result has q's rows, zeros
-        where they are padding; with, the sequences' rows (all of q's under graph
-        capture), as ``paged_prefill_attention`` returns them.
+        where they are padding; with, the sequences' rows, or under graph capture
+        all of q's, of which padding is zeros over 16-bit caches and unspecified
+        over FP8 ones.
         """
 
         self._validate_cache_bindings()

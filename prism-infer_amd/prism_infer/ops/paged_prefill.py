@@ -21,7 +21,9 @@ cache, or a block table too short for the context.  Over FP8 caches it waits
 for the result; over 16-bit caches only until the metadata is checked, which
 the launch does first (the result is then ready in stream order, as any
 op's).  Under graph capture that check is skipped (invalid sequences then
-leave their rows unspecified).
+leave their rows unspecified) and all of q's rows are returned: those outside
+the sequences, as a batch padded to a captured size has them, are zeros over
+16-bit caches and unspecified over FP8 ones.
 
 Differences a caller can see: K/V are dequantised in fp32 (payload times
 scale applied to the fp32 scores and to the softmax weights, as the decode
