@@ -173,6 +173,10 @@ bool aligned_rows(const at::Tensor& t) {
   return true;
 }
 
+bool records_gradients(const at::Tensor* q, const at::Tensor* k, const at::Tensor* v) {
+  return c10::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad());
+}
+
 bool int32_vector(const at::Tensor& t) { return t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous(); }
 
 // A paged decode's arguments, checked: decode's of eleven (from args[0]).
@@ -341,6 +345,7 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
       bt->size(0) < batch)
     Py_RETURN_NONE;
   const bool sixteen = kc->scalar_type() == q->scalar_type();
+  if (sixteen && records_gradients(q, kc, vc)) Py_RETURN_NONE;
   if (sixteen ? (dim != 64 && dim != 128) || !aligned_rows(*q) : dim != 128) Py_RETURN_NONE;
   void* stream = current_stream(device);
   PyObject* found = by_stream(args[11], device, stream);
@@ -394,9 +399,7 @@ PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int over1 = 0, over2 = 0;
   const long heads = PyLong_AsLongAndOverflow(args[5], &over1), kv_heads = PyLong_AsLongAndOverflow(args[6], &over2);
   int device;
-  if (over1 || over2 || !on_current_device(device, q, k, v, cq, ck) ||
-      (c10::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad())))
-    Py_RETURN_NONE;
+  if (over1 || over2 || !on_current_device(device, q, k, v, cq, ck) || records_gradients(q, k, v)) Py_RETURN_NONE;
   const int type = dtype_code(q->scalar_type());
   if (q->dim() != 3 || k->dim() != 3 || k->sizes() != v->sizes() || (type != PRISM_DTYPE_BF16 && type != PRISM_DTYPE_F16) ||
       k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || !int32_vector(*cq) || !int32_vector(*ck))

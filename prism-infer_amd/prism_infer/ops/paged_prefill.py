@@ -35,7 +35,9 @@ kernels cover bf16/fp16 queries and page sizes that are multiples of 16, over
   4 or 8;
 - bf16/fp16 caches of the queries' dtype: head_dim 64 or 128, any GQA group.
 
-Other cases raise ``RuntimeError`` (no CPU fallback).
+Other cases raise ``RuntimeError`` (no CPU fallback).  There is no backward pass:
+over 16-bit caches inputs that require gradients are refused while gradients are
+recorded.
 """
 
 from __future__ import annotations
@@ -176,6 +178,9 @@ def _launch_paged_prefill(q, k_cache, v_cache, context, *, num_heads, num_kv_hea
         if q.shape[2] not in PREFILL_HEAD_DIMS_16BIT:
             raise RuntimeError("the HIP paged prefill kernel covers head_dim 64 and 128 over 16-bit caches, "
                                f"got {q.shape[2]}")
+        if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+            raise RuntimeError("paged_prefill_attention has no backward pass over 16-bit caches: "
+                               "call it without recording gradients")
     elif q.shape[2] != PREFILL_HEAD_DIM:
         raise RuntimeError(f"the HIP paged prefill kernel covers head_dim {PREFILL_HEAD_DIM}, got {q.shape[2]}")
 
