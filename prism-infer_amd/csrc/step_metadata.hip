@@ -116,6 +116,8 @@ __global__ void __launch_bounds__(kMaxThreads) step_metadata_kernel(const MetaAr
     at_b = add_sat(at_b, wave_reduce(front ? part[1][lane] : 0, AddSat()));
   }
   at_b = add_sat(at_b, max(start, 0));
+  // (a first free entry behind the free blocks is none that a request took)
+  const int last_free = min(max(a.num_free, start), kMaxInt - 1);
   int longest = 0, first_bad = kMaxInt;
   for (int i = i0; i < i1; ++i) {
     if (per > 1) r = request(a, i);
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kMaxThreads) step_metadata_kernel(const MetaAr
     at_b = add_sat(at_b, r.taken);
     const int ctx = add_sat(r.cached, r.fresh);
     longest = max(longest, ctx);
-    if (r.bad || at_n > a.num_tokens || at_b > a.num_free || start < 0) first_bad = min(first_bad, i);
+    if (r.bad || at_n > a.num_tokens || at_b > last_free || start < 0) first_bad = min(first_bad, i);
     if (blockIdx.x == 0) {
       a.cu[i + 1] = at_n;
       a.ctx[i] = ctx;
