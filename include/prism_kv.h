@@ -306,7 +306,9 @@ int prism_device_copy(void* dst, const void* src, int64_t nbytes, int workgroups
  *              q_dtype, strides k_strides / v_strides {block, token, head, dim};
  *              dim stride 1.  page_size a multiple of 16.  FP8: head_dim 128, GQA
  *              group num_heads / num_kv_heads of 1, 2, 4 or 8.  16-bit: head_dim
- *              64 or 128, any group, no scales, rows of out 16-byte aligned.
+ *              64 or 128, any group, no scales, rows of out 16-byte aligned, at
+ *              most 2^29 rows of a kv head (total_q * group) and (rows / 128
+ *              rounded up + batch + 2) * num_kv_heads workgroups below 2^24.
  * k/v_scale  : [num_blocks, page_size, num_kv_heads] fp32 or both NULL (unit
  *              scale); strides ks_strides / vs_strides.
  * block_tables, context_lens, cu_seqlens_q : int32 device arrays ([>= batch,
@@ -383,8 +385,10 @@ int prism_paged_prefill_ws(const void* q, int q_dtype, const int64_t q_strides[3
  *              Rows that see no key, and rows outside [cu_seqlens_q[0],
  *              cu_seqlens_q[batch]), are 0.  A sequence whose offsets are out of
  *              order or outside the tensors is left out, its rows unspecified;
- *              so are all rows where sequences share some.  total_q * num_heads /
- *              num_kv_heads is at most 2^29.
+ *              so are all rows where sequences share some.
+ * limits     : total_k at most 2^31 - 4096, the rows of a kv head (total_q *
+ *              num_heads / num_kv_heads) at most 2^29, and (rows / 128 rounded up +
+ *              batch + 1) * num_kv_heads workgroups below 2^24.
  * workspace  : device scratch (256-byte aligned, any contents) of at least
  *              prism_prompt_attention_workspace_bytes() bytes for the same
  *              geometry, which is 0 where none is used.  With it the keys of few,

@@ -33,7 +33,9 @@ kernels cover bf16/fp16 queries and page sizes that are multiples of 16, over
 
 - FP8 E4M3FN caches (scaled or unit-scale): head_dim 128, GQA groups of 1, 2,
   4 or 8;
-- bf16/fp16 caches of the queries' dtype: head_dim 64 or 128, any GQA group.
+- bf16/fp16 caches of the queries' dtype: head_dim 64 or 128, any GQA group, up to
+  2**29 query rows (tokens times heads per kv head) per kv head and fewer than
+  2**24 workgroups (of a kv head: one per 128 rows, one per sequence, two more).
 
 Other cases raise ``RuntimeError`` (no CPU fallback).  There is no backward pass:
 over 16-bit caches inputs that require gradients are refused while gradients are

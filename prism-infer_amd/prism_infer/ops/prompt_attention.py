@@ -17,8 +17,9 @@ when nothing is cached in front of a prompt (prism_infer/layers/attention.py:
 The offsets stay on the device and the call does not synchronise: it can be
 captured, and a replay follows the offsets of its time.  A sequence whose offsets
 are out of order or outside the tensors is left out; its rows are unspecified, and
-so are all rows where sequences share some.  A call takes up to 2**29 query rows
-per kv head and as many keys.
+so are all rows where sequences share some.  A call takes up to 2**29 keys, and of
+query rows (tokens times heads per kv head) up to 2**29 per kv head and fewer than
+2**24 workgroups: a kv head has one per 128 rows, one per sequence and one more.
 There is no backward pass: inputs that require gradients are refused while
 gradients are recorded.
 """
