@@ -348,6 +348,7 @@ int prism_paged_prefill(const void* q, int q_dtype, const int64_t q_strides[3], 
  * cu_seqlens_q[0] and cu_seqlens_q[batch].  Over FP8 caches they hold once the
  * stream is done (report[3] is not used).  Over 16-bit caches report[3], set to
  * 0 by the caller, becomes 1 once the others hold, before the attention is done.
+ * With batch or total_q 0 nothing is launched, and nothing written.
  */
 int64_t prism_paged_prefill_workspace_bytes(int batch, int total_q, int num_heads, int num_kv_heads, int page_size,
                                             int width);
@@ -425,7 +426,8 @@ int prism_prompt_attention(const void* q, const int64_t q_strides[3], const void
  *                [batch, width] block tables, -1 behind a request's last block
  * A request does not fit where a length is negative, its context exceeds width *
  * block_size, its tokens end behind num_tokens or the free blocks do not
- * suffice: what has no block gets -1.  batch is at most 8192.
+ * suffice: what has no block gets -1.  Held ids are taken as they are: tokens in
+ * a held block of -1 have slot -1 and fit.  batch is at most 8192.
  */
 int64_t prism_step_metadata_words(int batch, int width, int num_tokens);
 int prism_step_metadata(const int32_t* block_tables, const int64_t bt_strides[2], const int32_t* cached_lens,

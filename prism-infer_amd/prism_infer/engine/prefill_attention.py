@@ -30,7 +30,8 @@ class PagedKVPrefillAttention(PagedKVDecodeAttention):
         """Store the chunk's K/V ([T, kv_heads, head_dim]) and attend; q is [T, num_heads, head_dim].
 
         ``cached_prefix`` says whether any sequence has stored tokens in front of
-        this chunk, which the host knows.  Without, the result has q's rows, zeros
+        this chunk, which the host knows.  With, every sequence has new tokens (as in
+        the reference, one without is refused).  Without, the result has q's rows, zeros
         where they are padding; with, the sequences' rows, or under graph capture
         all of q's, of which padding is zeros over 16-bit caches and unspecified
         over FP8 ones.

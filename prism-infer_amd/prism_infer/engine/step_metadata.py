@@ -107,7 +107,8 @@ def build_step_metadata(
     rows get slot -1).  ``out`` is filled in place, as a captured graph's buffers are; it
     must not share memory with the inputs.  All tensors are int32 on one device.
     Nothing is synchronised: requests that do not fit get -1 where a block is
-    missing, and :meth:`StepMetadata.check` reports them.
+    missing, and :meth:`StepMetadata.check` reports them.  Held blocks are taken as
+    they are: a token in one that is -1 gets slot -1, which ``check`` does not report.
     """
 
     # calls that the native checks accept; the rest goes on below
