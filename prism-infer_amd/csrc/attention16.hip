@@ -191,10 +191,15 @@ struct Work {
 // one head's K/V.  K sequences per lane, all in registers, for batches of up to
 // 64 K: one load of the offsets, then wave reductions.
 //
-// Blocks with most keys go first, so that the launch ends on short ones: block j
-// of a sequence ends after about (level + j) ROWS / G keys, a binary search over
-// levels finds the rank's level, a scan over the sequences with a block there
-// its sequence.
+// Up to 64 sequences with more blocks than the chip holds at once: blocks with
+// most keys go first, so that the launch ends on short ones.  Block j of a
+// sequence ends after about (level + j) ROWS / G keys, a binary search over levels
+// finds the rank's level, a scan over the sequences with a block there its
+// sequence.  Otherwise sequence by sequence, in reverse.  us by levels and in
+// reverse (32 / 8 heads): 6 prompts of 61 to 1900 tokens 139.5 and 142, 20 of them
+// 182.5 and 184.5; but 4 x 2048 tokens behind 8192 1089 and 1080, 40 prompts of 500
+// to 3000 1359 and 1214, 64 of 100 to 1900 897 and 796: many sequences' blocks side by
+// side share fewer keys in the L2.
 //
 // Where blocks are few and long their keys are split: into parts of the fewest
 // tiles for which all parts fit the chip at once, if that pays.
