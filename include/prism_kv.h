@@ -35,6 +35,16 @@ extern "C" {
 #define PRISM_DTYPE_BF16 1
 #define PRISM_DTYPE_F16 2
 #define PRISM_DTYPE_FP8_E4M3FN 3
+/*
+ * The 4-bit cache format, taken by the entry points that name it: E2M1 values, two
+ * a byte (the even dim in the low half), rows of head_dim / 2 bytes, beside one
+ * power of two (E8M0: 2^(byte - 127), 255 is NaN) per 32 dims, rows of head_dim /
+ * 32 bytes.  Stores choose for each block the smallest exponent byte >= 1 with
+ * max|x| <= 7 * 2^(byte - 127) and round x / 2^(byte - 127) to the nearest value,
+ * ties to the even code, magnitudes above 6 to 6; a block with an infinity or a
+ * NaN becomes NaN (byte 255, zeros).
+ */
+#define PRISM_DTYPE_FP4_E2M1 4
 
 /* ABI version of this header (bumped on any signature change). */
 int prism_abi_version(void);
@@ -433,6 +443,85 @@ int64_t prism_step_metadata_words(int batch, int width, int num_tokens);
 int prism_step_metadata(const int32_t* block_tables, const int64_t bt_strides[2], const int32_t* cached_lens,
                         const int32_t* query_lens, const int32_t* free_blocks, int num_free, const int32_t* free_start,
                         int batch, int width, int block_size, int num_tokens, int32_t* packed, void* stream);
+
+/*
+ * Position rotation of a step's queries and keys, with the keys and values
+ * appended to a paged cache (the reference rotates in its model code and stores
+ * then: prism_infer/layers/rotary_embedding.py, prism_infer/ops/kv_cache_store.py).
+ *
+ * q          : [num_tokens, num_heads, head_dim] of in_dtype (F32/BF16/F16), strides
+ *              {token, head, dim}; dim stride 1.  num_heads 0: no queries.
+ * key, value : [num_tokens, num_kv_heads, head_dim] of in_dtype, likewise.
+ * cos_sin    : fp32 [max_positions, rotary_dim], the cosines of a position's
+ *              rotary_dim / 2 angles, then their sines.
+ * rotary_dim : how many of a head's first dims are rotated (even, 0: none).
+ *              interleaved 0: dims i and i + rotary_dim / 2 are a pair, else 2 i
+ *              and 2 i + 1.
+ * positions  : int32, num_axes rows of num_tokens, axis_stride elements apart.
+ * axes       : int32 [rotary_dim / 2], the row of positions that each angle goes
+ *              by, or NULL: row 0 for all.  An angle whose axis is outside
+ *              [0, num_axes) or position outside [0, max_positions) makes its
+ *              pair NaN.
+ * q_out      : contiguous, q rotated.  key_out: contiguous, key rotated, or NULL.
+ * k/v_cache, cache_dtype, k/v_scale, slot_mapping, num_slots : as in
+ *              prism_kv_store, or PRISM_DTYPE_FP4_E2M1 with its exponents.  What is
+ *              stored of a key is what key_out holds.  With slots < 0 and >=
+ *              num_slots only q_out and key_out are written.
+ * limits     : num_tokens * (num_heads + 2 num_kv_heads) below 2^31.
+ */
+int prism_kv_rotate_store(const void* q, const int64_t q_strides[3], const void* key, const int64_t key_strides[3],
+                          const void* value, const int64_t value_strides[3], int in_dtype, const float* cos_sin,
+                          int64_t max_positions, int rotary_dim, int interleaved, const int32_t* positions,
+                          int64_t axis_stride, int num_axes, const int32_t* axes, void* q_out, void* key_out, void* k_cache,
+                          void* v_cache, int cache_dtype, void* k_scale, void* v_scale, const int32_t* slot_mapping,
+                          int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, int64_t num_slots, void* stream);
+
+/*
+ * Rows of a cache read back: key_out and value_out, contiguous [num_tokens,
+ * num_heads, head_dim] of out_dtype (F32/BF16/F16), get what the slots hold (fp32
+ * products of payload and scale, rounded once), and zeros for slots < 0 and >=
+ * num_slots.  Caches as in prism_kv_rotate_store; head_dim a multiple of 8,
+ * buffers 16-byte aligned.
+ */
+int prism_kv_load(const void* k_cache, const void* v_cache, int cache_dtype, const void* k_scale, const void* v_scale,
+                  const int32_t* slot_mapping, void* key_out, void* value_out, int out_dtype, int64_t num_tokens,
+                  int num_heads, int head_dim, int64_t num_slots, void* stream);
+
+/*
+ * Attention over a 4-bit paged cache: one query token a sequence (cu_seqlens_q
+ * NULL, as prism_paged_decode), or a chunk of a sequence's last tokens (as
+ * prism_paged_prefill).
+ *
+ * q          : [total_q, num_heads, head_dim] of q_dtype (BF16/F16), strides
+ *              {token, head, dim}; dim stride 1, rows 16-byte aligned; head_dim 64
+ *              or 128, any group num_heads / num_kv_heads.
+ * k/v_cache  : [num_blocks, page_size, num_kv_heads, head_dim / 2] bytes, strides
+ *              {block, token, head, byte}; byte stride 1, rows 16-byte aligned;
+ *              page_size a multiple of 16, pages of less than 2^31 bytes.
+ * k/v_scale  : [num_blocks, page_size, num_kv_heads, head_dim / 32] exponent bytes,
+ *              strides likewise; byte stride 1, rows aligned to their length.
+ * block_tables, context_lens, cu_seqlens_q : as in the two entry points.
+ * max_context_len : one token a sequence: int32 [1].  Chunks: NULL.
+ * out        : [total_q, num_heads, head_dim] of q_dtype, rows 16-byte aligned.
+ *              One token a sequence: rows without a visible key are 0, blocks < 0
+ *              and >= num_blocks are skipped.  Chunks: rows outside
+ *              [cu_seqlens_q[0], cu_seqlens_q[batch]) are 0.
+ * status, report : chunks, as in prism_paged_prefill_ws over 16-bit caches.  One
+ *              token a sequence: NULL.
+ * workspace  : device scratch (256-byte aligned, any contents) of
+ *              prism_paged_fp4_workspace_bytes() bytes for the same geometry, as
+ *              much as it needs (chunks is 0 where cu_seqlens_q is NULL, else 1).
+ *              Calls that may run at once need one each.
+ */
+int64_t prism_paged_fp4_workspace_bytes(int chunks, int batch, int total_q, int num_heads, int num_kv_heads, int head_dim,
+                                        int page_size, int width);
+int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strides[3], const void* k_cache, const void* v_cache,
+                    const int64_t k_strides[4], const int64_t v_strides[4], const void* k_scale, const void* v_scale,
+                    const int64_t ks_strides[4], const int64_t vs_strides[4], const int32_t* block_tables,
+                    const int64_t bt_strides[2], const int32_t* context_lens, const int32_t* max_context_len,
+                    const int32_t* cu_seqlens_q, void* out, const int64_t out_strides[3], int batch, int total_q,
+                    int num_heads, int num_kv_heads, int head_dim, int page_size, int num_blocks, int width, float scale,
+                    int32_t* status, int32_t* report, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Test hook with no counterpart in the reference: converts n fp32 values to

@@ -65,6 +65,8 @@ int prism_preload(void) {
   if (int rc = prism::preload_paged_prefill()) return rc;
   if (int rc = prism::preload_attention16()) return rc;
   if (int rc = prism::preload_step_metadata()) return rc;
+  if (int rc = prism::preload_rotary_store()) return rc;
+  if (int rc = prism::preload_paged_fp4()) return rc;
   return prism::preload_paged_decode();
 }
 

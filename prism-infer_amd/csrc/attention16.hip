@@ -31,6 +31,7 @@
 // the last product and a division per use, 74 now).
 #include "common.h"
 #include "divide.h"
+#include "paged_chunks.h"
 #include "wave_ops.h"
 
 #include <algorithm>
@@ -140,11 +141,6 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const void* p) {
 struct Seq {
   int q0, qlen, k0, klen;
 };
-
-__device__ __forceinline__ void flag_sequence(const AttnArgs& a, int i) {
-  atomicMin(a.status, i);
-  if (a.report != nullptr) a.report[0] = 1;  // (every writer stores the same)
-}
 
 // Rows and keys of K sequences from i on; good: whether their lengths are valid
 // (packed: offsets in order and inside the tensors).  Others are out of the work.
@@ -355,57 +351,6 @@ __device__ __forceinline__ bool locate_many(const AttnArgs& a, int me, bool flag
   return false;
 }
 
-// The outcome that a host waits for, from the first workgroup alone and long
-// before the others are done: every sequence's lengths and block ids.  Threads
-// are spread over the sequences first, then over a sequence's pages.
-template <int SRC>
-__device__ void check_metadata(const AttnArgs& a, int& first_bad) {  // (in LDS)
-  constexpr int kAtOnce = 8;
-  const int tid = threadIdx.x, threads = blockDim.x;
-  if (tid == 0) first_bad = INT32_MAX;
-  __syncthreads();
-  int across = 1;  // sequences at a time
-  while (across < a.batch && across < threads) across *= 2;
-  for (int i = tid & (across - 1); i < a.batch; i += across) {
-    Seq s[1];
-    bool good[1];
-    sequences<SRC, 1>(a, i, s, good);
-    const int pages = good[0] ? (s[0].klen - 1) / a.page + 1 : 0;
-    for (int p = tid / across; p < pages; p += kAtOnce * (threads / across)) {
-      int id[kAtOnce];
-#pragma unroll
-      for (int x = 0; x < kAtOnce; ++x)
-        id[x] = a.bt[static_cast<int64_t>(i) * a.bt_sb + static_cast<int64_t>(min(p + x * (threads / across), pages - 1)) * a.bt_sn];
-#pragma unroll
-      for (int x = 0; x < kAtOnce; ++x) good[0] = good[0] && id[x] >= 0 && id[x] < a.num_blocks;
-    }
-    if (!good[0]) atomicMin(&first_bad, i);
-  }
-  __syncthreads();
-  if (tid != 0) return;
-  if (first_bad != INT32_MAX) flag_sequence(a, first_bad);
-  a.report[1] = a.cu_q[0];
-  a.report[2] = a.cu_q[a.batch];
-  __hip_atomic_store(a.report + 3, 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
-}
-
-// Rows outside every sequence are 0: the workgroups beyond the real blocks
-// (one per kv head at least) share them.
-template <int D>
-__device__ void zero_padding(const AttnArgs& a, int checks, int real_blocks) {
-  const int first = min(max(a.cu_q[0], 0), a.total_q), end = min(max(a.cu_q[a.batch], first), a.total_q);
-  const int64_t others = checks + static_cast<int64_t>(real_blocks) * a.kv_heads;
-  const int64_t me = blockIdx.x - others, workers = gridDim.x - others;
-  const int64_t per_row = static_cast<int64_t>(a.heads) * (D / 8);
-  const int64_t chunks = (first + (a.total_q - end)) * per_row;
-  for (int64_t x = me * blockDim.x + threadIdx.x; x < chunks; x += workers * blockDim.x) {
-    int64_t row = x / per_row;
-    const int rest = static_cast<int>(x - row * per_row);
-    if (row >= first) row += end - first;
-    *reinterpret_cast<u32x4*>(a.out + row * a.o_st + rest / (D / 8) * a.o_sh + rest % (D / 8) * 8) = u32x4{0, 0, 0, 0};
-  }
-}
-
 // 16-byte chunk swizzle of key t's row in LDS: chunk x holds the row's chunk
 // x ^ swz(t).  64 banks of 4 bytes; ds_read_b128 serves 16 lanes at a time,
 // ds_read_b64 (and _tr_b16) 32.  K reads (row c, chunk 2 x + g) then meet 16
@@ -446,7 +391,13 @@ attention16_kernel(const AttnArgs a) {
   const int checks = SRC != kPacked && a.report != nullptr ? a.kv_heads : 0;
   const int me = static_cast<int>(blockIdx.x) - checks;
   if (me < 0) {
-    if (blockIdx.x == 0) check_metadata<SRC>(a, *reinterpret_cast<int*>(lds));
+    if (blockIdx.x == 0)
+      check_metadata(a, *reinterpret_cast<int*>(lds), [&](int i) {
+        Seq s[1];
+        bool good[1];
+        sequences<SRC, 1>(a, i, s, good);
+        return good[0] ? s[0].klen : -1;
+      });
     return;
   }
   Work work;
@@ -459,7 +410,8 @@ attention16_kernel(const AttnArgs a) {
     // there and pages' places spill; 2 chunks behind 12000 104 us, 106 with them shared.)
     auto* args = __builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(args));
-    zero_padding<D>(*(const AttnArgs*)args, checks, work.total);
+    const int64_t others = checks + static_cast<int64_t>(work.total) * ((const AttnArgs*)args)->kv_heads;
+    zero_padding<D>(*(const AttnArgs*)args, blockIdx.x - others, gridDim.x - others);
     return;
   }
   const int seq = uniform_int(work.seq), block = uniform_int(work.block), h = uniform_int(work.head);

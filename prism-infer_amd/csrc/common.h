@@ -30,6 +30,8 @@ int preload_paged_prefill();
 int preload_paged_decode();
 int preload_attention16();
 int preload_step_metadata();
+int preload_rotary_store();
+int preload_paged_fp4();
 
 int device_cu_count();
 

@@ -23,6 +23,7 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
 DTYPE_FP8_E4M3FN = 3
+DTYPE_FP4_E2M1 = 4
 
 _TORCH_TO_CODE = {
     torch.float32: DTYPE_F32,
@@ -31,6 +32,8 @@ _TORCH_TO_CODE = {
 }
 if hasattr(torch, "float8_e4m3fn"):
     _TORCH_TO_CODE[torch.float8_e4m3fn] = DTYPE_FP8_E4M3FN
+if hasattr(torch, "float4_e2m1fn_x2"):
+    _TORCH_TO_CODE[torch.float4_e2m1fn_x2] = DTYPE_FP4_E2M1
 
 # Every symbol include/prism_kv.h declares, with (restype, argtypes).
 _I64P = ctypes.POINTER(ctypes.c_int64)
@@ -97,6 +100,18 @@ SIGNATURES: dict[str, tuple] = {
     "prism_paged_prefill_16bit_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I]),
     "prism_step_metadata_words": (_I64, [_I, _I, _I]),
     "prism_step_metadata": (_I, [_VP, _I64P, _VP, _VP, _VP, _I, _VP, _I, _I, _I, _I, _VP, _VP]),
+    "prism_kv_rotate_store": (
+        _I,
+        [_VP, _I64P, _VP, _I64P, _VP, _I64P, _I, _VP, _I64, _I, _I, _VP, _I64, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP,
+         _VP, _VP, _I64, _I, _I, _I, _I64, _VP],
+    ),
+    "prism_kv_load": (_I, [_VP, _VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _I64, _I, _I, _I64, _VP]),
+    "prism_paged_fp4_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "prism_paged_fp4": (
+        _I,
+        [_VP, _I, _I64P, _VP, _VP, _I64P, _I64P, _VP, _VP, _I64P, _I64P, _VP, _I64P, _VP, _VP, _VP, _VP, _I64P, _I, _I,
+         _I, _I, _I, _I, _I, _I, _F, _VP, _VP, _VP, _I64, _VP],
+    ),
     "prism_debug_fp8_encode": (_I, [_VP, _VP, _I64, _VP]),
 }
 
@@ -258,6 +273,7 @@ __all__ = [
     "DTYPE_BF16",
     "DTYPE_F16",
     "DTYPE_F32",
+    "DTYPE_FP4_E2M1",
     "DTYPE_FP8_E4M3FN",
     "LIB_NAME",
     "LIB_PATH",

@@ -1,4 +1,4 @@
-"""Scaled-FP8 KV format: the numeric constants and the byte arithmetic of pages.
+"""Scaled-FP8 and 4-bit KV formats: the numeric constants and the byte arithmetic of pages.
 
 The public names and values are the ones callers of
 prism_infer/engine/kv_quantization.py (:9-13, :33-107) import: an E4M3FN payload
@@ -13,6 +13,12 @@ Byte accounting, for one layer and one token:
 
 which for 8 kv heads of 128 dims in E4M3FN is 2048 + 64 = 2112 bytes. A block
 multiplies that by ``page_size * num_layers``.
+
+The 4-bit format has no counterpart in the reference: E2M1 values, two to a
+``torch.float4_e2m1fn_x2`` (the even dim in the low half), so a payload's last
+axis is ``head_dim / 2``, and one power of two (``torch.float8_e8m0fnu``) for each
+32 dims, the smallest at which the block's largest magnitude is at most 7 of it.
+A token's row of 128 dims is 64 + 4 bytes.
 """
 
 from __future__ import annotations
@@ -32,6 +38,12 @@ KV_SCALE_DTYPE = torch.float32
 KV_COMPONENT_COUNT = 2
 
 _SCALE_ITEMSIZE = 4  # bytes of one KV_SCALE_DTYPE element
+
+FP4_DTYPE = torch.float4_e2m1fn_x2
+FP4_SCALE_DTYPE = torch.float8_e8m0fnu
+FP4_SCALE_BLOCK = 32  # dims that share an exponent
+FP4_MOST = 7.0        # of a block, in units of its power of two (6 is the largest value)
+FP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)  # by code; 8 more for the sign
 
 
 class KVStorageBytes(NamedTuple):
@@ -78,6 +90,26 @@ def scale_cache_shape(payload_shape: Sequence[int]) -> tuple[int, ...]:
     return dims[:-1]
 
 
+def fp4_payload_shape(shape: Sequence[int]) -> tuple[int, ...]:
+    """Shape of the 4-bit payload that holds rows of ``shape`` ([..., kv_heads, head_dim])."""
+
+    dims = tuple(shape)
+    if len(dims) < 3 or any(not _is_count(d) or d < 1 for d in dims) or dims[-1] % FP4_SCALE_BLOCK:
+        raise ValueError(f"fp4_payload_shape: expected [..., kv_heads, head_dim] with head_dim a multiple of "
+                         f"{FP4_SCALE_BLOCK}, got {list(dims)}")
+    return (*dims[:-1], dims[-1] // 2)
+
+
+def fp4_scale_cache_shape(payload_shape: Sequence[int]) -> tuple[int, ...]:
+    """Shape of the exponents that go with a 4-bit payload ([..., kv_heads, head_dim / 2])."""
+
+    dims = tuple(payload_shape)
+    if not dims or 2 * dims[-1] % FP4_SCALE_BLOCK:
+        raise ValueError(f"fp4_scale_cache_shape: the payload's rows hold a multiple of {FP4_SCALE_BLOCK // 2} bytes, "
+                         f"got {list(dims)}")
+    return (*dims[:-1], 2 * dims[-1] // FP4_SCALE_BLOCK)
+
+
 def kv_token_layer_bytes(*, num_kv_heads: int, head_dim: int, token_head_scales: bool = True,
                          payload_itemsize: int = 1) -> int:
     """Bytes that one token occupies in one layer: K and V rows plus their scales."""
@@ -111,6 +143,9 @@ def kv_block_storage_bytes(
     if not isinstance(token_head_scales, bool):
         raise TypeError(f"token_head_scales: expected a bool, received {token_head_scales!r}")
     rows = KV_COMPONENT_COUNT * num_layers * page_size * num_kv_heads
+    if payload_dtype == FP4_DTYPE:  # exponents belong to the format
+        row = fp4_payload_shape((1, num_kv_heads, head_dim))
+        return KVStorageBytes(payload=rows * row[-1], scales=rows * fp4_scale_cache_shape(row)[-1])
     return KVStorageBytes(
         payload=rows * head_dim * payload_dtype.itemsize,
         scales=rows * _SCALE_ITEMSIZE if token_head_scales else 0,
@@ -143,12 +178,19 @@ def kv_cache_storage_bytes(payload_cache: torch.Tensor,
 
 
 __all__ = [
+    "FP4_DTYPE",
+    "FP4_MOST",
+    "FP4_SCALE_BLOCK",
+    "FP4_SCALE_DTYPE",
+    "FP4_VALUES",
     "FP8_E4M3FN_MAX",
     "FP8_E4M3FN_MIN",
     "KV_COMPONENT_COUNT",
     "KV_SCALE_DTYPE",
     "KVStorageBytes",
     "PER_TOKEN_HEAD_SCALE_FLOOR",
+    "fp4_payload_shape",
+    "fp4_scale_cache_shape",
     "kv_block_storage_bytes",
     "kv_cache_storage_bytes",
     "kv_token_layer_bytes",

@@ -11,7 +11,13 @@ libprism_mi355x.so.  Differences from the reference, all deliberate:
   always take the HIP kernels, and a missing native library raises there;
 * the scaled path is bit-exact against the eager oracle, including scales
   (the reference's Triton kernel is only checked to 1e-6 relative);
-* slots >= the cache's slot count are skipped instead of written out of bounds.
+* slots >= the cache's slot count are skipped instead of written out of bounds;
+* 4-bit caches (no counterpart in the reference): payloads of dtype
+  ``torch.float4_e2m1fn_x2`` [..., kv_heads, head_dim / 2] with exponents of dtype
+  ``torch.float8_e8m0fnu`` [..., kv_heads, head_dim / 32], head_dim a multiple of 32.
+  Each 32 dims get the smallest power of two (at least 2**-126) of which their
+  largest magnitude is at most 7, and values the nearest E2M1 multiple of it, ties
+  to the even code; a block with an infinity or a NaN becomes NaN.
 """
 
 from __future__ import annotations
@@ -20,10 +26,15 @@ import torch
 
 from prism_infer import _native, observability
 from prism_infer.engine.kv_quantization import (
+    FP4_DTYPE,
+    FP4_SCALE_BLOCK,
+    FP4_SCALE_DTYPE,
+    FP4_VALUES,
     FP8_E4M3FN_MAX,
     FP8_E4M3FN_MIN,
     KV_SCALE_DTYPE,
     PER_TOKEN_HEAD_SCALE_FLOOR,
+    fp4_scale_cache_shape,
     scale_cache_shape,
 )
 from prism_infer.observability import profile_region
@@ -52,6 +63,12 @@ def is_fp8_cache_tensor(tensor: torch.Tensor) -> bool:
     return tensor.dtype in FP8_CACHE_DTYPES
 
 
+def is_fp4_cache_tensor(tensor: torch.Tensor) -> bool:
+    """Return whether ``tensor`` is a 4-bit KV payload."""
+
+    return tensor.dtype == FP4_DTYPE
+
+
 def _validate_store_inputs(key, value, k_cache, v_cache, slot_mapping, k_scale_cache, v_scale_cache) -> bool:
     """Validate the public storage contract and return whether scales are used."""
 
@@ -73,7 +90,8 @@ def _validate_payload_store_inputs(key, value, k_cache, v_cache, slot_mapping) -
         raise ValueError("K/V payload caches must have matching shape and dtype")
     if k_cache.ndim not in SUPPORTED_KV_CACHE_RANKS:
         raise ValueError("K/V payload caches must be [slots, heads, dim] or [blocks, page, heads, dim]")
-    if tuple(k_cache.shape[-2:]) != tuple(key.shape[-2:]):
+    heads, dim = k_cache.shape[-2:]
+    if (heads, 2 * dim if is_fp4_cache_tensor(k_cache) else dim) != tuple(key.shape[-2:]):
         raise ValueError(
             "input/cache KV head shape mismatch: "
             f"input={list(key.shape[-2:])}, cache={list(k_cache.shape[-2:])}"
@@ -85,6 +103,9 @@ def _validate_payload_store_inputs(key, value, k_cache, v_cache, slot_mapping) -
 def _validate_scale_store_inputs(k_cache, k_scale_cache, v_scale_cache) -> bool:
     if (k_scale_cache is None) != (v_scale_cache is None):
         raise ValueError("K/V scale caches must be provided together")
+    if is_fp4_cache_tensor(k_cache):
+        validate_fp4_scales(k_cache, k_scale_cache, v_scale_cache)
+        return True
     if k_scale_cache is None:
         return False
     if not is_fp8_cache_tensor(k_cache):
@@ -98,6 +119,19 @@ def _validate_scale_store_inputs(k_cache, k_scale_cache, v_scale_cache) -> bool:
     if k_scale_cache.dtype != KV_SCALE_DTYPE or v_scale_cache.dtype != KV_SCALE_DTYPE:
         raise ValueError("K/V scale caches must use torch.float32")
     return True
+
+
+def validate_fp4_scales(k_cache, k_scale_cache, v_scale_cache) -> None:
+    """The exponents of a 4-bit cache."""
+
+    if k_scale_cache is None or v_scale_cache is None:
+        raise ValueError("4-bit K/V payload caches need their exponents (k_scale_cache and v_scale_cache)")
+    expected = fp4_scale_cache_shape(k_cache.shape)
+    if tuple(k_scale_cache.shape) != expected or tuple(v_scale_cache.shape) != expected:
+        raise ValueError(f"K/V scale cache shape must be one exponent per {FP4_SCALE_BLOCK} dims: expected={list(expected)}, "
+                         f"got {list(k_scale_cache.shape)} and {list(v_scale_cache.shape)}")
+    if k_scale_cache.dtype != FP4_SCALE_DTYPE or v_scale_cache.dtype != FP4_SCALE_DTYPE:
+        raise ValueError("the exponents of 4-bit K/V caches must use torch.float8_e8m0fnu")
 
 
 def _validate_device_store_layout(key, value, k_cache, v_cache, slot_mapping, k_scale_cache, v_scale_cache) -> None:
@@ -125,6 +159,8 @@ def _validate_device_store_layout(key, value, k_cache, v_cache, slot_mapping, k_
 def _store_profile_region(scaled: bool, k_cache: torch.Tensor, on_cpu: bool = False) -> str:
     if on_cpu:
         return "attention.kv_store.eager"
+    if is_fp4_cache_tensor(k_cache):
+        return "attention.kv_store.hip_fp4"
     if scaled:
         return "attention.kv_store.hip_scaled_fp8"
     if is_fp8_cache_tensor(k_cache):
@@ -163,6 +199,23 @@ def _quantize_rows(x: torch.Tensor, cache_dtype: torch.dtype) -> tuple[torch.Ten
     return payload, scale
 
 
+def _quantize_rows_fp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """[n, heads, dim] -> (E2M1 pairs, exponent bytes), both as uint8."""
+
+    blocks = x.double().unflatten(-1, (-1, FP4_SCALE_BLOCK))  # (64 bits: nothing below is rounded)
+    amax = blocks.abs().amax(-1)
+    good = torch.isfinite(amax)
+    mantissa, exponent = torch.frexp(torch.where(good, amax, 0.0))  # the mantissa is in [0.5, 1)
+    exponent = torch.where(amax > 0, torch.where(mantissa > 0.875, exponent - 2, exponent - 3), -126).clamp(min=-126)
+    units = torch.ldexp(torch.where(good[..., None], blocks, 0.0), -exponent[..., None])
+    steps = torch.tensor([(a + b) / 2 for a, b in zip(FP4_VALUES, FP4_VALUES[1:])], dtype=torch.float64)
+    size = units.abs()
+    up, down = torch.bucketize(size, steps, right=True), torch.bucketize(size, steps)  # differ at ties only
+    codes = torch.where(up % 2 == 0, up, down) + 8 * torch.signbit(units)
+    codes = codes.flatten(-2).to(torch.uint8)
+    return codes[..., 0::2] + 16 * codes[..., 1::2], torch.where(good, exponent + 127, 255).to(torch.uint8)
+
+
 def _store_kvcache_cpu(key, value, k_cache, v_cache, slot_mapping, k_scale_cache, v_scale_cache) -> None:
     """Host-tensor store: the reference's eager semantics (:183-230), vectorized
     over tokens. Payload rows and scales are written with index_copy_ on flat
@@ -171,7 +224,7 @@ def _store_kvcache_cpu(key, value, k_cache, v_cache, slot_mapping, k_scale_cache
     caches = tuple(t for t in (k_cache, v_cache, k_scale_cache, v_scale_cache) if t is not None)
     if not all(t.is_contiguous() for t in caches):
         raise RuntimeError("KV store requires contiguous KV and scale caches")
-    heads, dim = key.shape[-2], key.shape[-1]
+    heads, dim = k_cache.shape[-2:]
     flat_k = k_cache.view(-1, heads, dim)
     flat_v = v_cache.view(-1, heads, dim)
     rows, slots = _last_writer_rows(slot_mapping, flat_k.shape[0])
@@ -182,6 +235,12 @@ def _store_kvcache_cpu(key, value, k_cache, v_cache, slot_mapping, k_scale_cache
     if k_scale_cache is None:
         _index_copy_bytes(flat_k, slots, k_rows.to(k_cache.dtype))
         _index_copy_bytes(flat_v, slots, v_rows.to(v_cache.dtype))
+        return
+    if is_fp4_cache_tensor(k_cache):
+        for rows_in, flat, scales in ((k_rows, flat_k, k_scale_cache), (v_rows, flat_v, v_scale_cache)):
+            payload, exponents = _quantize_rows_fp4(rows_in)
+            _index_copy_bytes(flat, slots, payload)
+            _index_copy_bytes(scales.view(-1, heads, scales.shape[-1]), slots, exponents)
         return
     k_payload, k_scale = _quantize_rows(k_rows, k_cache.dtype)
     v_payload, v_scale = _quantize_rows(v_rows, v_cache.dtype)
@@ -226,12 +285,21 @@ def store_kvcache(
         return
     _validate_device_store_layout(key, value, k_cache, v_cache, slot_mapping, k_scale_cache, v_scale_cache)
     num_tokens, num_heads, head_dim = key.shape
-    num_slots = k_cache.numel() // (num_heads * head_dim) if k_cache.numel() else 0
+    num_slots = k_cache.numel() // (k_cache.shape[-2] * k_cache.shape[-1]) if k_cache.numel() else 0
     lib = _native.device_lib(key.device)
     with profile_region(
         _store_profile_region(scaled, k_cache),
         metadata={"cache_dtype": str(k_cache.dtype), "tokens": num_tokens},
     ), torch.cuda.device(key.device):
+        if is_fp4_cache_tensor(k_cache):
+            _native.check(lib.prism_kv_rotate_store(
+                None, None, key.data_ptr(), _native.strides(key), value.data_ptr(), _native.strides(value),
+                _native.dtype_code(key.dtype), None, 0, 0, 0, None, 0, 0, None, None, None,
+                k_cache.data_ptr(), v_cache.data_ptr(), _native.DTYPE_FP4_E2M1,
+                k_scale_cache.data_ptr(), v_scale_cache.data_ptr(), slot_mapping.data_ptr(),
+                num_tokens, 0, num_heads, head_dim, num_slots, _native.stream_handle(key.device),
+            ), "store_kvcache")
+            return
         status = lib.prism_kv_store(
             key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype),
             _native.strides(key), _native.strides(value),
@@ -251,6 +319,7 @@ __all__ = [
     "HAS_HIP_KERNELS",
     "HAS_TRITON",
     "PER_TOKEN_HEAD_SCALE_FLOOR",
+    "is_fp4_cache_tensor",
     "is_fp8_cache_tensor",
     "store_kvcache",
 ]

@@ -19,6 +19,10 @@ kernel semantics (:83-180):
 HIP kernel's tiling is its own (32-token MFMA tiles, split-K over long
 contexts), so the value does not change results.  Split-K scratch is
 allocated here from static shapes through torch's caching allocator.
+
+Over 4-bit caches (``torch.float4_e2m1fn_x2`` payloads [num_blocks, block_size,
+num_kv_heads, head_dim / 2] with their exponents, no counterpart in the reference)
+queries are bf16 or fp16, head_dim 64 or 128 and pages a multiple of 16 tokens.
 """
 
 from __future__ import annotations
@@ -26,6 +30,7 @@ from __future__ import annotations
 import torch
 
 from prism_infer import _native
+from prism_infer.ops.paged_fp4 import is_fp4, launch_fp4, validate_fp4_call, validate_fp4_devices
 
 HAS_HIP_KERNELS = _native.available()
 HAS_TRITON = HAS_HIP_KERNELS  # the reference's "kernel available" flag name
@@ -257,6 +262,25 @@ def _no_context_bound(context_lens: torch.Tensor) -> torch.Tensor:
     return cached
 
 
+def _paged_decode_fp4(q, k_cache, v_cache, block_tables, context_lens, scale, max_context_len, k_scale_cache,
+                      v_scale_cache, block_n) -> torch.Tensor:
+    what = "paged_decode_attention"
+    if block_n <= 0 or block_n & (block_n - 1):
+        raise ValueError(f"block_n must be a positive power of two, got {block_n}")
+    _validate_paged_metadata(block_tables, context_lens, max_context_len)
+    validate_fp4_call(what, q, k_cache, v_cache, k_scale_cache, v_scale_cache, block_tables)
+    batch = q.shape[0]
+    if block_tables.shape[0] < batch or context_lens.shape[0] < batch:
+        raise ValueError(
+            "block_tables/context_lens batch must cover q batch, "
+            f"got q={batch}, block_tables={block_tables.shape[0]}, context_lens={context_lens.shape[0]}"
+        )
+    validate_fp4_devices(what, q, k_cache, v_cache, k_scale_cache, v_scale_cache, block_tables, context_lens,
+                         max_context_len)
+    return launch_fp4(what, q, k_cache, v_cache, k_scale_cache, v_scale_cache, block_tables, context_lens, scale,
+                      max_context_len=max_context_len)
+
+
 def paged_decode_attention(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -270,7 +294,7 @@ def paged_decode_attention(
     max_context_len: torch.Tensor | None = None,
     block_n: int = DEFAULT_PAGED_DECODE_BLOCK_N,
 ) -> torch.Tensor:
-    """Single-query paged attention over (scaled-)FP8 or 16/32-bit KV pages."""
+    """Single-query paged attention over 4-bit, (scaled-)FP8 or 16/32-bit KV pages."""
 
     if max_context_len is None:
         max_context_len = _no_context_bound(context_lens)
@@ -281,6 +305,9 @@ def paged_decode_attention(
                            max_context_len, block_n, _WORKSPACES)
         if out is not None:
             return out
+    if is_fp4(k_cache):
+        return _paged_decode_fp4(q, k_cache, v_cache, block_tables, context_lens, scale, max_context_len,
+                                 k_scale_cache, v_scale_cache, block_n)
     scaled_kv = _validate_paged_decode_inputs(
         q, k_cache, v_cache, block_tables, context_lens, max_context_len,
         k_scale_cache=k_scale_cache, v_scale_cache=v_scale_cache, block_n=block_n,

@@ -1,4 +1,4 @@
-"""Paged prefill attention over FP8 or 16-bit pages on MI355X (HIP kernels).
+"""Paged prefill attention over 4-bit, FP8 or 16-bit pages on MI355X (HIP kernels).
 
 Drop-in for ``paged_prefill_attention_reference``
 (prism_infer/ops/paged_attention_reference.py:185-246), which
@@ -18,12 +18,12 @@ sequence) and gathers pages into dense tensors.  Here one kernel launch
 reads the pages in place, with the metadata on the device, and the host waits
 once to raise the reference's errors: invalid lengths, a block id past the
 cache, or a block table too short for the context.  Over FP8 caches it waits
-for the result; over 16-bit caches only until the metadata is checked, which
+for the result; over 16-bit and 4-bit caches only until the metadata is checked, which
 the launch does first (the result is then ready in stream order, as any
 op's).  Under graph capture that check is skipped (invalid sequences then
 leave their rows unspecified) and all of q's rows are returned: those outside
 the sequences, as a batch padded to a captured size has them, are zeros over
-16-bit caches and unspecified over FP8 ones.
+16-bit and 4-bit caches and unspecified over FP8 ones.
 
 Differences a caller can see: K/V are dequantised in fp32 (payload times
 scale applied to the fp32 scores and to the softmax weights, as the decode
@@ -33,12 +33,13 @@ kernels cover bf16/fp16 queries and page sizes that are multiples of 16, over
 
 - FP8 E4M3FN caches (scaled or unit-scale): head_dim 128, GQA groups of 1, 2,
   4 or 8;
-- bf16/fp16 caches of the queries' dtype: head_dim 64 or 128, any GQA group, up to
-  2**29 query rows (tokens times heads per kv head) per kv head and fewer than
-  2**24 workgroups (of a kv head: one per 128 rows, one per sequence, two more).
+- bf16/fp16 caches of the queries' dtype, and 4-bit caches (:mod:`.paged_fp4`):
+  head_dim 64 or 128, any GQA group, up to 2**29 query rows (tokens times heads per
+  kv head) per kv head and fewer than 2**24 workgroups (of a kv head: one per 128
+  rows, one per sequence, two more).
 
 Other cases raise ``RuntimeError`` (no CPU fallback).  There is no backward pass:
-over 16-bit caches inputs that require gradients are refused while gradients are
+over 16-bit and 4-bit caches inputs that require gradients are refused while gradients are
 recorded.
 """
 
@@ -49,6 +50,7 @@ import threading
 import torch
 
 from prism_infer import _native
+from prism_infer.ops.paged_fp4 import is_fp4, launch_fp4, validate_fp4_call, validate_fp4_devices
 
 HAS_HIP_KERNELS = _native.available()
 _HOST = _native.host_ops()
@@ -151,12 +153,50 @@ def _raise_sequence_error(seq: int, cu_seqlens_q, context_lens, block_tables, nu
     )
 
 
+def _metadata(context, device: torch.device):
+    context_lens = _int32_device(context.context_lens, device)
+    cu_seqlens_q = _int32_device(context.cu_seqlens_q, device)
+    block_tables = _int32_device(context.block_tables, device)
+    if block_tables.ndim != 2:
+        raise ValueError(f"block_tables must be two-dimensional, got {list(block_tables.shape)}")
+    batch = context_lens.numel()
+    if cu_seqlens_q.numel() < batch + 1 or block_tables.shape[0] < batch:
+        raise ValueError(
+            f"cu_seqlens_q needs {batch + 1} entries and block_tables {batch} rows, "
+            f"got {cu_seqlens_q.numel()} and {block_tables.shape[0]}"
+        )
+    return context_lens, cu_seqlens_q, block_tables, batch
+
+
+def _launch_paged_prefill_fp4(q, k_cache, v_cache, context, num_heads, num_kv_heads, scale, k_scale_cache, v_scale_cache):
+    what = "paged_prefill_attention"
+    _validate_heads(num_heads, num_kv_heads)
+    if q.ndim != 3 or q.shape[1] != num_heads:
+        raise ValueError(f"q must be [tokens, num_heads={num_heads}, head_dim], got {list(q.shape)}")
+    if k_cache.ndim != 4 or k_cache.shape[2] != num_kv_heads:
+        raise ValueError(f"4-bit K/V caches must be [num_blocks, block_size, num_kv_heads={num_kv_heads}, head_dim / 2], "
+                         f"got {list(k_cache.shape)}")
+    validate_fp4_call(what, q, k_cache, v_cache, k_scale_cache, v_scale_cache, context.block_tables)
+    validate_fp4_devices(what, q, k_cache, v_cache, k_scale_cache, v_scale_cache)
+    device = q.device
+    context_lens, cu_seqlens_q, block_tables, batch = _metadata(context, device)
+    with torch.cuda.device(device):
+        status = torch.full((1,), _STATUS_OK, dtype=torch.int32, device=device)
+    cu_seqlens_q = cu_seqlens_q.contiguous()
+    out = launch_fp4(what, q, k_cache, v_cache, k_scale_cache, v_scale_cache, block_tables, context_lens, scale,
+                     cu_seqlens_q=cu_seqlens_q, batch=batch, status=status)
+    return out, status, (context_lens, cu_seqlens_q, block_tables), batch
+
+
 def _launch_paged_prefill(q, k_cache, v_cache, context, *, num_heads, num_kv_heads, scale, k_scale_cache=None,
                           v_scale_cache=None):
     """Validate and enqueue the kernel; returns (out, status, cu_seqlens_q, batch) without synchronising."""
 
     if context.block_tables is None or context.context_lens is None or context.cu_seqlens_q is None:
         raise RuntimeError("paged prefill requires block_tables/context_lens/cu_seqlens_q")
+    if is_fp4(k_cache):
+        return _launch_paged_prefill_fp4(q, k_cache, v_cache, context, num_heads, num_kv_heads, scale, k_scale_cache,
+                                         v_scale_cache)
     scaled = _validate_caches(k_cache, v_cache, k_scale_cache, v_scale_cache)
     _validate_heads(num_heads, num_kv_heads)
     if q.ndim != 3 or q.shape[1] != num_heads:
@@ -187,17 +227,7 @@ def _launch_paged_prefill(q, k_cache, v_cache, context, *, num_heads, num_kv_hea
         raise RuntimeError(f"the HIP paged prefill kernel covers head_dim {PREFILL_HEAD_DIM}, got {q.shape[2]}")
 
     device = q.device
-    context_lens = _int32_device(context.context_lens, device)
-    cu_seqlens_q = _int32_device(context.cu_seqlens_q, device)
-    block_tables = _int32_device(context.block_tables, device)
-    if block_tables.ndim != 2:
-        raise ValueError(f"block_tables must be two-dimensional, got {list(block_tables.shape)}")
-    batch = context_lens.numel()
-    if cu_seqlens_q.numel() < batch + 1 or block_tables.shape[0] < batch:
-        raise ValueError(
-            f"cu_seqlens_q needs {batch + 1} entries and block_tables {batch} rows, "
-            f"got {cu_seqlens_q.numel()} and {block_tables.shape[0]}"
-        )
+    context_lens, cu_seqlens_q, block_tables, batch = _metadata(context, device)
     sixteen = k_cache.dtype == q.dtype
     if sixteen:
         q = _native.aligned_rows(q)
