@@ -1,9 +1,9 @@
 // Host side of the per-layer ops: argument checks and launches without
 // Python in between.
 //
-// store_kvcache, paged_decode_attention, paged_prefill_attention and
-// prompt_attention run once per layer and step, build_step_metadata once per
-// step; checked in Python and bound through ctypes, a call costs
+// store_kvcache, rotate_store_kvcache, load_kvcache, paged_decode_attention,
+// paged_prefill_attention and prompt_attention run once per layer and step,
+// build_step_metadata once per step; checked in Python and bound through ctypes, a call costs
 // the host more than the kernels of a small step take.  These functions do the
 // same checks on the tensors themselves and call the C ABI (one layer's store
 // and decode, B = 1, 1800 tokens: 41.8 us a step in Python, 16.1 here, where
@@ -49,9 +49,12 @@ int dtype_code(at::ScalarType t) {
     case at::kBFloat16: return PRISM_DTYPE_BF16;
     case at::kHalf: return PRISM_DTYPE_F16;
     case at::kFloat8_e4m3fn: return PRISM_DTYPE_FP8_E4M3FN;
+    case at::kFloat4_e2m1fn_x2: return PRISM_DTYPE_FP4_E2M1;
     default: return -1;
   }
 }
+
+bool plain_dtype(int code) { return code == PRISM_DTYPE_F32 || code == PRISM_DTYPE_BF16 || code == PRISM_DTYPE_F16; }
 
 // Every tensor on one device, which is ready and current.
 template <typename... T>
@@ -68,6 +71,18 @@ bool scale_pair(const at::Tensor& cache, const at::Tensor* ks, const at::Tensor*
   const auto want = cache.sizes().slice(0, cache.dim() - 1);
   return cache.scalar_type() == at::kFloat8_e4m3fn && ks->sizes() == want && vs->sizes() == want &&
          ks->scalar_type() == at::kFloat && vs->scalar_type() == at::kFloat;
+}
+
+// The exponents of a 4-bit cache: one per 32 dims (16 payload bytes).
+bool fp4_scale_pair(const at::Tensor& cache, const at::Tensor* ks, const at::Tensor* vs) {
+  if (!ks || !vs || cache.scalar_type() != at::kFloat4_e2m1fn_x2 || cache.dim() < 3 || cache.size(-1) <= 0 || cache.size(-1) % 16 != 0)
+    return false;
+  for (const at::Tensor* t : {ks, vs}) {
+    if (t->scalar_type() != at::kFloat8_e8m0fnu || t->dim() != cache.dim() || t->size(-1) != cache.size(-1) / 16) return false;
+    for (int64_t i = 0; i + 1 < cache.dim(); ++i)
+      if (t->size(i) != cache.size(i)) return false;
+  }
+  return true;
 }
 
 // An optional pair of arguments: both None, or both tensors.
@@ -130,12 +145,13 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t n) {
       kc->sizes() != vc->sizes() || kc->scalar_type() != vc->scalar_type())
     Py_RETURN_NONE;
   const int64_t tokens = key->size(0), heads = key->size(1), dim = key->size(2);
+  const bool four = kc->scalar_type() == at::kFloat4_e2m1fn_x2;
   if (tokens <= 0 || heads <= 0 || dim <= 0 || heads > INT32_MAX || dim > INT32_MAX || kc->size(-2) != heads ||
-      kc->size(-1) != dim || slots->dim() != 1 || slots->numel() != tokens || slots->scalar_type() != at::kInt ||
-      !slots->is_contiguous() || !scale_pair(*kc, ks, vs))
+      kc->size(-1) * (four ? 2 : 1) != dim || slots->dim() != 1 || slots->numel() != tokens || slots->scalar_type() != at::kInt ||
+      !slots->is_contiguous() || !(four ? fp4_scale_pair(*kc, ks, vs) : scale_pair(*kc, ks, vs)))
     Py_RETURN_NONE;
   const int in = dtype_code(key->scalar_type()), out = dtype_code(kc->scalar_type());
-  if (in < 0 || in == PRISM_DTYPE_FP8_E4M3FN || value->scalar_type() != key->scalar_type() || out < 0 ||
+  if (!plain_dtype(in) || value->scalar_type() != key->scalar_type() || out < 0 ||
       key->stride(2) != 1 || value->stride(2) != 1 || key->stride(1) != dim || value->stride(1) != dim ||
       !kc->is_contiguous() || !vc->is_contiguous() || (ks && (!ks->is_contiguous() || !vs->is_contiguous())))
     Py_RETURN_NONE;
@@ -144,11 +160,17 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int rc;
   {
     WithoutGil released;
-    rc = prism_kv_store(key->data_ptr(), value->data_ptr(), in, kst, vst, kc->data_ptr(), vc->data_ptr(), out,
-                        ks ? static_cast<float*>(ks->data_ptr()) : nullptr,
-                        vs ? static_cast<float*>(vs->data_ptr()) : nullptr,
-                        static_cast<const int32_t*>(slots->data_ptr()), tokens, static_cast<int>(heads),
-                        static_cast<int>(dim), kc->numel() / (heads * dim), current_stream(device));
+    if (four)
+      rc = prism_kv_rotate_store(nullptr, nullptr, key->data_ptr(), kst, value->data_ptr(), vst, in, nullptr, 0, 0, 0, nullptr, 0, 0,
+                                 nullptr, nullptr, nullptr, kc->data_ptr(), vc->data_ptr(), out, ks->data_ptr(), vs->data_ptr(),
+                                 static_cast<const int32_t*>(slots->data_ptr()), tokens, 0, static_cast<int>(heads),
+                                 static_cast<int>(dim), kc->numel() / (heads * kc->size(-1)), current_stream(device));
+    else
+      rc = prism_kv_store(key->data_ptr(), value->data_ptr(), in, kst, vst, kc->data_ptr(), vc->data_ptr(), out,
+                          ks ? static_cast<float*>(ks->data_ptr()) : nullptr,
+                          vs ? static_cast<float*>(vs->data_ptr()) : nullptr,
+                          static_cast<const int32_t*>(slots->data_ptr()), tokens, static_cast<int>(heads),
+                          static_cast<int>(dim), kc->numel() / (heads * dim), current_stream(device));
   }
   if (rc != PRISM_OK) Py_RETURN_NONE;
   Py_RETURN_TRUE;
@@ -178,6 +200,181 @@ bool records_gradients(const at::Tensor* q, const at::Tensor* k, const at::Tenso
 }
 
 bool int32_vector(const at::Tensor& t) { return t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous(); }
+
+PyObject* pair(at::Tensor&& a, at::Tensor&& b) {
+  PyObject* first = THPVariable_Wrap(std::move(a));
+  PyObject* second = first ? THPVariable_Wrap(std::move(b)) : nullptr;
+  if (second == nullptr) {
+    Py_XDECREF(first);
+    return nullptr;
+  }
+  return Py_BuildValue("(NN)", first, second);
+}
+
+// rotate_store(q, key, value, cos_sin, positions, k_cache, v_cache, slot_mapping, k_scale, v_scale, position_axes,
+//              interleaved, return_key) -> rotated q, (rotated q, rotated key) or None
+PyObject* rotate_store(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 13 || !PyBool_Check(args[11]) || !PyBool_Check(args[12])) Py_RETURN_NONE;
+  const at::Tensor *q = tensor(args[0]), *key = tensor(args[1]), *value = tensor(args[2]), *table = tensor(args[3]),
+                   *at = tensor(args[4]), *kc = tensor(args[5]), *vc = tensor(args[6]), *slots = tensor(args[7]), *ks, *vs,
+                   *axes = args[10] == Py_None ? nullptr : tensor(args[10]);
+  if (!q || !key || !value || !table || !at || !kc || !vc || !slots || !optional_pair(args[8], args[9], ks, vs) ||
+      (!axes && args[10] != Py_None))
+    Py_RETURN_NONE;
+  int device;
+  if (!on_current_device(device, q, key, value, table, at, kc, vc, slots, ks, vs, axes) || records_gradients(q, key, value) ||
+      (c10::GradMode::is_enabled() && table->requires_grad()))
+    Py_RETURN_NONE;
+  if (q->dim() != 3 || key->dim() != 3 || key->sizes() != value->sizes() || (kc->dim() != 3 && kc->dim() != 4) ||
+      kc->sizes() != vc->sizes() || kc->scalar_type() != vc->scalar_type() || table->dim() != 2 || slots->dim() != 1)
+    Py_RETURN_NONE;
+  const int64_t tokens = key->size(0), heads = key->size(1), dim = key->size(2), q_heads = q->size(1), rotary = table->size(1);
+  const bool four = kc->scalar_type() == at::kFloat4_e2m1fn_x2;
+  const int in = dtype_code(q->scalar_type()), out = dtype_code(kc->scalar_type());
+  if (tokens <= 0 || heads <= 0 || dim <= 0 || q_heads <= 0 || q_heads > INT32_MAX || heads > INT32_MAX || dim > INT32_MAX ||
+      q->size(0) != tokens || q->size(2) != dim || kc->size(-2) != heads || kc->size(-1) * (four ? 2 : 1) != dim ||
+      !(four ? fp4_scale_pair(*kc, ks, vs) : scale_pair(*kc, ks, vs)) || !plain_dtype(in) || out < 0 ||
+      key->scalar_type() != q->scalar_type() || value->scalar_type() != q->scalar_type() || q->stride(2) != 1 ||
+      key->stride(2) != 1 || value->stride(2) != 1 || !kc->is_contiguous() || !vc->is_contiguous() ||
+      (ks && (!ks->is_contiguous() || !vs->is_contiguous())) || slots->numel() != tokens || !int32_vector(*slots) ||
+      rotary <= 0 || rotary % 2 != 0 || rotary > dim || table->scalar_type() != at::kFloat || !table->is_contiguous() ||
+      at->scalar_type() != at::kInt || !at->is_contiguous())
+    Py_RETURN_NONE;
+  if (axes ? at->dim() != 2 || at->size(0) < 1 || at->size(0) > INT32_MAX || at->size(1) != tokens || !int32_vector(*axes) ||
+                 axes->numel() != rotary / 2
+           : at->dim() != 1 || at->numel() != tokens)
+    Py_RETURN_NONE;
+  at::Tensor q_out, key_out;
+  int rc;
+  {
+    WithoutGil released;
+    q_out = at::empty(q->sizes(), q->options());
+    if (args[12] == Py_True) key_out = at::empty(key->sizes(), key->options());
+    const Strides sq(q, true), sk(key, true), sv(value, true);
+    rc = prism_kv_rotate_store(
+        q->data_ptr(), sq.v, key->data_ptr(), sk.v, value->data_ptr(), sv.v, in, static_cast<const float*>(table->data_ptr()),
+        table->size(0), static_cast<int>(rotary), args[11] == Py_True, static_cast<const int32_t*>(at->data_ptr()), tokens,
+        axes ? static_cast<int>(at->size(0)) : 1, axes ? static_cast<const int32_t*>(axes->data_ptr()) : nullptr,
+        q_out.data_ptr(), key_out.defined() ? key_out.data_ptr() : nullptr, kc->data_ptr(), vc->data_ptr(), out,
+        ks ? ks->data_ptr() : nullptr, vs ? vs->data_ptr() : nullptr, static_cast<const int32_t*>(slots->data_ptr()), tokens,
+        static_cast<int>(q_heads), static_cast<int>(heads), static_cast<int>(dim),
+        kc->numel() / (heads * kc->size(-1)), current_stream(device));
+  }
+  if (rc != PRISM_OK) Py_RETURN_NONE;
+  if (!key_out.defined()) return THPVariable_Wrap(std::move(q_out));
+  return pair(std::move(q_out), std::move(key_out));
+  END_HANDLE_TH_ERRORS
+}
+
+// load(k_cache, v_cache, slot_mapping, k_scale, v_scale, dtype code) -> (key, value) or None
+PyObject* load(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !PyLong_CheckExact(args[5])) Py_RETURN_NONE;
+  const at::Tensor *kc = tensor(args[0]), *vc = tensor(args[1]), *slots = tensor(args[2]), *ks, *vs;
+  if (!kc || !vc || !slots || !optional_pair(args[3], args[4], ks, vs)) Py_RETURN_NONE;
+  const long to = PyLong_AsLong(args[5]);
+  int device;
+  if (!on_current_device(device, kc, vc, slots, ks, vs) || (kc->dim() != 3 && kc->dim() != 4) || kc->sizes() != vc->sizes() ||
+      kc->scalar_type() != vc->scalar_type() || !int32_vector(*slots) || (to < 0 || !plain_dtype(static_cast<int>(to))))
+    Py_RETURN_NONE;
+  const bool four = kc->scalar_type() == at::kFloat4_e2m1fn_x2;
+  const int from = dtype_code(kc->scalar_type());
+  const int64_t tokens = slots->numel(), heads = kc->size(-2), row = kc->size(-1), dim = four ? 2 * row : row;
+  if (from < 0 || !(four ? fp4_scale_pair(*kc, ks, vs) : scale_pair(*kc, ks, vs)) || tokens <= 0 || heads <= 0 || row <= 0 ||
+      heads > INT32_MAX || dim > INT32_MAX || !kc->is_contiguous() || !vc->is_contiguous() ||
+      (ks && (!ks->is_contiguous() || !vs->is_contiguous())))
+    Py_RETURN_NONE;
+  at::Tensor key, value;
+  int rc;
+  {
+    WithoutGil released;
+    const auto options = kc->options().dtype(to == PRISM_DTYPE_F32 ? at::kFloat : to == PRISM_DTYPE_BF16 ? at::kBFloat16 : at::kHalf);
+    key = at::empty({tokens, heads, dim}, options);
+    value = at::empty({tokens, heads, dim}, options);
+    rc = prism_kv_load(kc->data_ptr(), vc->data_ptr(), from, ks ? ks->data_ptr() : nullptr, vs ? vs->data_ptr() : nullptr,
+                       static_cast<const int32_t*>(slots->data_ptr()), key.data_ptr(), value.data_ptr(), static_cast<int>(to),
+                       tokens, static_cast<int>(heads), static_cast<int>(dim), kc->numel() / (heads * row), current_stream(device));
+  }
+  if (rc != PRISM_OK) Py_RETURN_NONE;
+  return pair(std::move(key), std::move(value));
+  END_HANDLE_TH_ERRORS
+}
+
+// A call over a 4-bit cache: what decode and prefill check alike.
+struct Fp4Call {
+  const at::Tensor *q, *kc, *vc, *ks, *vs, *bt, *ctx;
+  int device, qd;
+  int64_t total, heads, dim, blocks, page, kv_heads, width;
+  void* stream;
+};
+
+bool exponent_rows(const at::Tensor& t) {
+  const int64_t row = t.size(-1);
+  if (t.stride(-1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % row != 0) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) != 1 && t.stride(i) % row != 0) return false;
+  return true;
+}
+
+bool check_fp4(Fp4Call& d) {
+  const at::Tensor &q = *d.q, &kc = *d.kc;
+  if (!on_current_device(d.device, d.q, d.kc, d.vc, d.ks, d.vs, d.bt, d.ctx) || q.dim() != 3 || kc.dim() != 4 ||
+      kc.sizes() != d.vc->sizes() || d.vc->scalar_type() != kc.scalar_type() || !fp4_scale_pair(kc, d.ks, d.vs) || d.bt->dim() != 2 ||
+      d.bt->scalar_type() != at::kInt || !int32_vector(*d.ctx) || (c10::GradMode::is_enabled() && q.requires_grad()))
+    return false;
+  d.qd = dtype_code(q.scalar_type());
+  d.total = q.size(0), d.heads = q.size(1), d.dim = q.size(2);
+  d.blocks = kc.size(0), d.page = kc.size(1), d.kv_heads = kc.size(2), d.width = d.bt->size(1);
+  if ((d.qd != PRISM_DTYPE_BF16 && d.qd != PRISM_DTYPE_F16) || (d.dim != 64 && d.dim != 128) || kc.size(3) * 2 != d.dim ||
+      d.total <= 0 || d.total > INT32_MAX || d.heads <= 0 || d.heads > INT32_MAX || d.kv_heads <= 0 || d.heads % d.kv_heads != 0 ||
+      d.page <= 0 || d.page % 16 != 0 || d.page > INT32_MAX || d.blocks > INT32_MAX || d.width > INT32_MAX || !aligned_rows(q) ||
+      !aligned_rows(kc) || !aligned_rows(*d.vc) || !exponent_rows(*d.ks) || !exponent_rows(*d.vs))
+    return false;
+  d.stream = current_stream(d.device);
+  return true;
+}
+
+// The launch, with its scratch (which the stream's order keeps until it is done).
+int launch_fp4(const Fp4Call& d, const at::Tensor* max_ctx, const at::Tensor* cu, int64_t batch, float scale, int32_t* status,
+               int32_t* report, at::Tensor& out) {
+  out = at::empty(d.q->sizes(), d.q->options());
+  const int64_t need = prism_paged_fp4_workspace_bytes(cu != nullptr, static_cast<int>(batch), static_cast<int>(d.total),
+                                                       static_cast<int>(d.heads), static_cast<int>(d.kv_heads),
+                                                       static_cast<int>(d.dim), static_cast<int>(d.page), static_cast<int>(d.width));
+  const at::Tensor ws = at::empty({need}, d.q->options().dtype(at::kByte));
+  const Strides sq(d.q, true), sk(d.kc, true), sv(d.vc, true), sks(d.ks, true), svs(d.vs, true), sbt(d.bt), so(&out);
+  return prism_paged_fp4(
+      d.q->data_ptr(), d.qd, sq.v, d.kc->data_ptr(), d.vc->data_ptr(), sk.v, sv.v, d.ks->data_ptr(), d.vs->data_ptr(), sks.v, svs.v,
+      static_cast<const int32_t*>(d.bt->data_ptr()), sbt.v, static_cast<const int32_t*>(d.ctx->data_ptr()),
+      max_ctx ? static_cast<const int32_t*>(max_ctx->data_ptr()) : nullptr, cu ? static_cast<const int32_t*>(cu->data_ptr()) : nullptr,
+      out.data_ptr(), so.v, static_cast<int>(batch), static_cast<int>(d.total), static_cast<int>(d.heads),
+      static_cast<int>(d.kv_heads), static_cast<int>(d.dim), static_cast<int>(d.page), static_cast<int>(d.blocks),
+      static_cast<int>(d.width), scale, status, report, ws.data_ptr(), need, d.stream);
+}
+
+// decode's call over a 4-bit cache
+PyObject* decode_fp4(PyObject* const* args) {
+  Fp4Call d{tensor(args[0]), tensor(args[1]), tensor(args[2]), nullptr, nullptr, tensor(args[3]), tensor(args[4])};
+  const at::Tensor* max_ctx = tensor(args[8]);
+  if (!d.q || !d.vc || !d.bt || !d.ctx || !max_ctx || !optional_pair(args[6], args[7], d.ks, d.vs) || !d.ks ||
+      !PyFloat_CheckExact(args[5]) || !PyLong_CheckExact(args[9]))
+    Py_RETURN_NONE;
+  int overflow = 0;
+  const long block_n = PyLong_AsLongAndOverflow(args[9], &overflow);
+  if (overflow || block_n <= 0 || (block_n & (block_n - 1)) || !check_fp4(d) || !max_ctx->is_cuda() ||
+      max_ctx->get_device() != d.device || max_ctx->numel() != 1 || max_ctx->scalar_type() != at::kInt || d.bt->size(0) < d.total ||
+      d.ctx->numel() < d.total)
+    Py_RETURN_NONE;
+  at::Tensor out;
+  int rc;
+  {
+    WithoutGil released;
+    rc = launch_fp4(d, max_ctx, nullptr, d.total, static_cast<float>(PyFloat_AS_DOUBLE(args[5])), nullptr, nullptr, out);
+  }
+  if (rc != PRISM_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
 
 // A paged decode's arguments, checked: decode's of eleven (from args[0]).
 struct DecodeCall {
@@ -211,7 +408,7 @@ bool check_decode(PyObject* const* args, DecodeCall& d) {
   d.batch = q.size(0), d.heads = q.size(1), d.dim = q.size(2);
   d.blocks = kc.size(0), d.page = kc.size(1), d.kv_heads = kc.size(2), d.width = d.bt->size(1);
   d.qd = dtype_code(q.scalar_type()), d.cd = dtype_code(kc.scalar_type());
-  if (d.qd < 0 || d.qd == PRISM_DTYPE_FP8_E4M3FN || d.cd < 0 || d.batch <= 0 || d.heads <= 0 || d.dim <= 0 ||
+  if (!plain_dtype(d.qd) || d.cd < 0 || d.cd == PRISM_DTYPE_FP4_E2M1 || d.batch <= 0 || d.heads <= 0 || d.dim <= 0 ||
       d.dim > 256 || kc.size(3) != d.dim || d.page <= 0 || d.kv_heads <= 0 || d.heads % d.kv_heads != 0 ||
       d.bt->size(0) < d.batch || d.ctx->size(0) < d.batch || kc.stride(3) != 1 || d.batch > INT32_MAX ||
       d.heads > INT32_MAX || d.page > INT32_MAX || d.width > INT32_MAX)
@@ -243,7 +440,9 @@ const float* scales(const at::Tensor* t) { return t ? static_cast<const float*>(
 PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   DecodeCall d;
-  if (n != 11 || !check_decode(args, d)) Py_RETURN_NONE;
+  if (n != 11) Py_RETURN_NONE;
+  if (const at::Tensor* kc = tensor(args[1]); kc && kc->scalar_type() == at::kFloat4_e2m1fn_x2) return decode_fp4(args);
+  if (!check_decode(args, d)) Py_RETURN_NONE;
   at::Tensor out;
   int rc;
   {
@@ -311,6 +510,44 @@ bool outcome_known(const int32_t* word, void* stream) {
   }
 }
 
+// A call's result from the words that its launch wrote: (out, first bad sequence, first row, end row), or None where there is no outcome.
+PyObject* outcome(int rc, bool known, at::Tensor&& out, const at::Tensor& status, const volatile int32_t* r) {
+  if (rc != PRISM_OK || !known) Py_RETURN_NONE;
+  const int row0 = r[1], row1 = r[2];
+  const int bad = r[0] == 0 ? INT32_MAX : status.item<int32_t>();
+  PyObject* wrapped = THPVariable_Wrap(std::move(out));
+  if (wrapped == nullptr) return nullptr;
+  return Py_BuildValue("(Niii)", wrapped, bad, row0, row1);
+}
+
+// prefill's call over a 4-bit cache
+PyObject* prefill_fp4(const at::Tensor* q, const at::Tensor* kc, const at::Tensor* vc, const at::Tensor* ks, const at::Tensor* vs,
+                      const at::Tensor* bt, const at::Tensor* ctx, const at::Tensor* cu, long heads, long kv_heads, double scale,
+                      PyObject* buffers) {
+  if (ks == nullptr) Py_RETURN_NONE;
+  Fp4Call d{q, kc, vc, ks, vs, bt, ctx};
+  const int64_t batch = ctx->numel();
+  if (!check_fp4(d) || d.heads != heads || d.kv_heads != kv_heads || batch <= 0 || batch > INT32_MAX || !int32_vector(*cu) ||
+      cu->numel() < batch + 1 || bt->size(0) < batch)
+    Py_RETURN_NONE;
+  PyObject* found = by_stream(buffers, d.device, d.stream);
+  if (found == nullptr || !PyTuple_CheckExact(found) || PyTuple_GET_SIZE(found) != 2) Py_RETURN_NONE;
+  const at::Tensor *status = tensor(PyTuple_GET_ITEM(found, 0)), *report = tensor(PyTuple_GET_ITEM(found, 1));
+  if (!status || !report) Py_RETURN_NONE;
+  int32_t* words = static_cast<int32_t*>(report->data_ptr());
+  words[0] = words[3] = 0;  // (the thread's previous call on this stream has its outcome: nothing writes them any more)
+  at::Tensor out;
+  int rc;
+  {
+    WithoutGil released;
+    rc = launch_fp4(d, nullptr, cu, batch, static_cast<float>(scale), static_cast<int32_t*>(status->data_ptr()), words, out);
+    if (rc == PRISM_OK && (!outcome_known(words + 3, d.stream) || *static_cast<volatile int32_t*>(words) != 0))
+      C10_HIP_CHECK(hipStreamSynchronize(static_cast<hipStream_t>(d.stream)));
+  }
+  const volatile int32_t* r = words;
+  return outcome(rc, r[3] != 0, std::move(out), *status, r);
+}
+
 // prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, num_heads, num_kv_heads, scale, k_scale,
 //         v_scale, buffers) -> (out, first bad sequence, first row, end row) or None
 //
@@ -330,6 +567,7 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const double scale = PyFloat_AS_DOUBLE(args[8]);
   int device;
   if (over1 || over2 || !on_current_device(device, q, kc, vc, bt, ctx, cu, ks, vs) || capturing()) Py_RETURN_NONE;
+  if (kc->scalar_type() == at::kFloat4_e2m1fn_x2) return prefill_fp4(q, kc, vc, ks, vs, bt, ctx, cu, heads, kv_heads, scale, args[11]);
   if (q->dim() != 3 || kc->dim() != 4 || kc->sizes() != vc->sizes() || bt->dim() != 2 ||
       (kc->scalar_type() != at::kFloat8_e4m3fn && kc->scalar_type() != q->scalar_type()) ||
       vc->scalar_type() != kc->scalar_type() || !scale_pair(*kc, ks, vs) ||
@@ -378,12 +616,7 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
       C10_HIP_CHECK(hipStreamSynchronize(static_cast<hipStream_t>(stream)));
   }
   const volatile int32_t* r = words;
-  if (rc != PRISM_OK || (sixteen && r[3] == 0)) Py_RETURN_NONE;
-  const int row0 = r[1], row1 = r[2];
-  const int bad = r[0] == 0 ? INT32_MAX : status->item<int32_t>();
-  PyObject* wrapped = THPVariable_Wrap(std::move(out));
-  if (wrapped == nullptr) return nullptr;
-  return Py_BuildValue("(Niii)", wrapped, bad, row0, row1);
+  return outcome(rc, !sixteen || r[3] != 0, std::move(out), *status, r);
   END_HANDLE_TH_ERRORS
 }
 
@@ -504,6 +737,8 @@ PyObject* step_metadata(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"mark_ready", mark_ready, METH_O, nullptr},
+    {"rotate_store", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rotate_store)), METH_FASTCALL, nullptr},
+    {"load", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(load)), METH_FASTCALL, nullptr},
     {"store", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(store)), METH_FASTCALL, nullptr},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(decode)), METH_FASTCALL, nullptr},
     {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(step)), METH_FASTCALL, nullptr},

@@ -19,6 +19,7 @@ from prism_infer.ops.kv_cache_store import (
 )
 
 HAS_HIP_KERNELS = _native.available()
+_HOST = _native.host_ops()
 
 LOAD_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -38,6 +39,11 @@ def load_kvcache(
     negative or behind the cache.  head_dim is a multiple of 8.
     """
 
+    # calls that the native checks accept; the rest goes on below
+    if _HOST is not None and dtype in LOAD_DTYPES:
+        out = _HOST.load(k_cache, v_cache, slot_mapping, k_scale_cache, v_scale_cache, _native.dtype_code(dtype))
+        if out is not None:
+            return out
     if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError("K/V payload caches must have matching shape and dtype")
     if k_cache.ndim not in SUPPORTED_KV_CACHE_RANKS:

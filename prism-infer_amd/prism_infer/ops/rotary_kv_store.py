@@ -32,6 +32,7 @@ from prism_infer import _native
 from prism_infer.ops.kv_cache_store import _validate_store_inputs
 
 HAS_HIP_KERNELS = _native.available()
+_HOST = _native.host_ops()
 
 ROTARY_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -75,6 +76,12 @@ def rotate_store_kvcache(
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """Rotate q and key by their positions, store key and value; returns the rotated q (and key, with ``return_key``)."""
 
+    # calls that the native checks accept; the rest goes on below
+    if _HOST is not None:
+        out = _HOST.rotate_store(q, key, value, cos_sin, positions, k_cache, v_cache, slot_mapping, k_scale_cache,
+                                 v_scale_cache, position_axes, interleaved, return_key)
+        if out is not None:
+            return out
     scaled = _validate_store_inputs(key, value, k_cache, v_cache, slot_mapping, k_scale_cache, v_scale_cache)
     _validate_rotation(q, key, cos_sin, positions, position_axes)
     if q.dtype not in ROTARY_DTYPES or key.dtype != q.dtype or value.dtype != q.dtype:
