@@ -31,6 +31,7 @@
 // the last product and a division per use, 74 now).
 #include "common.h"
 #include "divide.h"
+#include "fp4.h"
 #include "paged_chunks.h"
 #include "wave_ops.h"
 
@@ -50,15 +51,18 @@ constexpr int kMostRows = 1 << 29;     // of a kv head: sums of blocks over 256 
 constexpr int kCols = 32;              // rows per wave: the columns of a 32x32 MFMA
 
 // Where keys come from: packed like the queries, pages that hold whole tiles,
-// or pages of a multiple of 16 keys.
-enum Source { kPacked, kPages, kSmallPages };
+// or pages of a multiple of 16 keys; of 16 bits, or of 4 (fp4.h), which become 16 on
+// their way to LDS.
+enum Source { kPacked, kPages, kSmallPages, kPages4, kSmallPages4 };
+constexpr bool small_pages(int src) { return src == kSmallPages || src == kSmallPages4; }
+constexpr bool four_bits(int src) { return src >= kPages4; }
 
 struct AttnArgs {
   const uint16_t* q;
   int64_t q_st, q_sh;  // strides in elements (dim stride 1)
   const uint16_t* k;
   const uint16_t* v;
-  int64_t k_sn, k_st, k_sh, v_sn, v_st, v_sh;  // page, token, head
+  int64_t k_sn, k_st, k_sh, v_sn, v_st, v_sh;  // page, token, head (also where keys have 4 bits: in units of two bytes)
   const int32_t* bt;
   int64_t bt_sb, bt_sn;
   const int32_t* ctx;   // paged: keys of each sequence
@@ -75,6 +79,11 @@ struct AttnArgs {
   int slots;      // workgroups that the chip holds at once
   int room;       // of one kv head
   uint8_t* work;  // scratch of split blocks (SplitScratch), or null: no block is split
+  const uint8_t* ks;  // exponents of 4-bit keys and values, strides in bytes
+  const uint8_t* vs;
+  int64_t ks_sn, ks_st, ks_sh, vs_sn, vs_st, vs_sh;
+  Divisor by_page;    // where they lie in small pages
+  bool four;
 };
 
 // A block whose keys are split: its rows, and where its parts are.
@@ -369,6 +378,22 @@ __device__ __forceinline__ uint32_t pack(float lo, float up) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, up}, bf16x2));
 }
 
+// Eight 4-bit values times a power of two -> 16-bit ones: exact, but that float16
+// ends at 65504 and at 2^-24, as it does where a cache holds it.
+template <bool F16>
+__device__ __forceinline__ u32x4 widen8(uint32_t w, float scale) {
+  if constexpr (F16)
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
+  else
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+}
+
 template <bool F16, int D, int SRC, int GROUPS>
 __global__ void __launch_bounds__(64 * kWaves * GROUPS) __attribute__((amdgpu_waves_per_eu(2)))
 attention16_kernel(const AttnArgs a) {
@@ -458,7 +483,7 @@ attention16_kernel(const AttnArgs a) {
   const int32_t* bt_row = SRC == kPacked ? nullptr : a.bt + static_cast<int64_t>(seq) * a.bt_sb;
   auto load_ids = [&](int base) { return bt_row[static_cast<int64_t>(min(base + lane, a.width - 1)) * a.bt_sn]; };
   // The table is walked tile by tile; 64 consecutive entries sit in one register.
-  constexpr int kGroups = SRC == kSmallPages ? kKeys / 16 : 1;  // entries per tile
+  constexpr int kGroups = SRC == kSmallPages4 ? (D == 128 ? 1 : 2) : small_pages(SRC) ? kKeys / 16 : 1;  // entries per tile; of 4 bits, a wave's
   struct Place {
     int blk[kGroups];  // pages, per 16 keys where a tile may lie in several (-1: not needed)
     int row;           // of the first key in its page
@@ -473,15 +498,33 @@ attention16_kernel(const AttnArgs a) {
       ids = load_ids(page);
     }
   };
-  auto look_up = [&](int t) {
+  auto look_up = [&](int t) __attribute__((always_inline)) {
     Place p;
     p.ok = true;
-    if constexpr (SRC != kPacked) {
+    if constexpr (SRC == kSmallPages4) {
+#pragma unroll
+      for (int x = 0; x < kGroups; ++x) {
+        const int key = t * kKeys + 16 * ((D == 128 ? wave : 2 * (wave % 2)) + x);
+        p.blk[x] = -1;
+        if (x == 0) p.row = 0;
+        if (key < kend) {
+          const int at = divide(key, a.by_page);
+          if (at >= ids_base + 64) {
+            ids_base = at;
+            ids = load_ids(at);
+          }
+          p.blk[x] = __builtin_amdgcn_readlane(ids, at - ids_base);
+          p.ok = p.ok && p.blk[x] >= 0 && p.blk[x] < a.num_blocks;
+          if (x == 0) p.row = key - at * a.page;
+        }
+      }
+      if (!p.ok && lane == 0) flag_sequence(a, seq);
+    } else if constexpr (SRC != kPacked) {
       p.row = page_row;
 #pragma unroll
       for (int x = 0; x < kGroups; ++x) {
         p.blk[x] = -1;
-        if (SRC == kPages || t * kKeys + x * 16 < kend) {  // groups past the keys needed are not looked up
+        if (!small_pages(SRC) || t * kKeys + x * 16 < kend) {  // groups past the keys needed are not looked up
           if (page >= ids_base + 64) {
             ids_base = page;
             ids = load_ids(page);
@@ -507,7 +550,75 @@ attention16_kernel(const AttnArgs a) {
   const uint32_t lds0 = lds_address(share);
   // Starts the loads of K or V of tile t into LDS offset `stage`.  (A tile that
   // cannot be loaded leaves the stage as it was: its sequence is flagged.)
+  // 4-bit keys: a lane has the 16 bytes of one exponent, 32 dims of a key.  With 128
+  // dims a wave has 16 keys and their values, with 64 two waves have 32 keys each, the
+  // others the values.  The bytes come to LDS behind the stages (their queries are in
+  // registers by then), from where the same lane widens them into their stage a tile
+  // later; the exponent waits in a register.  (All in registers over a tile, 23 of
+  // them spilled.)  The rows of 16 lanes are those whose swizzles differ.
+  struct Fours {
+    u32x4 w;
+    uint32_t e;
+  };
+  constexpr uint32_t kRaw = 4 * kPayload, kHalf = 5120;  // K and V: 4 kB and 1 kB
+  static_assert(2 * kHalf <= 2 * kCols * kRow || D == 64, "the bytes fit behind the stages");
+  const bool values4 = D == 64 && wave >= 2;  // 64 dims: which of the two the wave has
+  auto row4 = [&](int l) __attribute__((always_inline)) {
+    return D == 128 ? 16 * wave + 4 * (l / 4 % 4) + l / 16
+                    : 32 * (wave % 2) + l / 2 % 2 + 4 * (l / 4 % 2) + 8 * (l / 8 % 2) + 2 * (l / 16 % 2) + 16 * (l / 32);
+  };
+  auto block4 = [&](int l) { return D == 128 ? l % 4 : l % 2; };
+  // (recomputed each time: kept, what depends on the lane takes registers that the loop needs)
+  auto fresh_lane = [&]() {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  auto place4 = [&](const Place& place, bool isv, int l, const uint8_t*& bytes, const uint8_t*& exponent) __attribute__((always_inline)) {
+    int b = place.blk[0], p = place.row + (small_pages(SRC) ? row4(l) % 16 : row4(l));
+    if constexpr (SRC == kSmallPages4 && D == 64) {
+      int next = place.row + 16;
+      if (next >= a.page) next -= a.page;
+      if (l >= 32) b = place.blk[kGroups - 1], p = next + row4(l) % 16;
+    }
+    bytes = (isv ? v_head : k_head) + b * ((isv ? a.v_sn : a.k_sn) * 2) + static_cast<int64_t>(p) * (isv ? v_st : k_st) + block4(l) * 16;
+    exponent = (isv ? a.vs + h * a.vs_sh : a.ks + h * a.ks_sh) + b * (isv ? a.vs_sn : a.ks_sn) + p * (isv ? a.vs_st : a.ks_st) + block4(l);
+    return b >= 0;
+  };
+  auto fetch = [&](const Place& place, bool isv, Fours& f) __attribute__((always_inline)) {  // into registers
+    const uint8_t *bytes, *exponent;
+    if (!place.ok || (D == 64 && isv != values4) || !place4(place, isv, lane, bytes, exponent)) return;
+    f.w = *reinterpret_cast<const u32x4*>(bytes);
+    f.e = *exponent;
+  };
+  auto put = [&](const Fours& f, uint32_t stage) __attribute__((always_inline)) {
+    const int l = fresh_lane(), r = row4(l);
+    const float e = f.e == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(f.e << 23);
+    const uint32_t at = stage + r * kRow + (((4 * block4(l)) ^ swz<D>(r)) << 4);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) *reinterpret_cast<u32x4*>(share + (at ^ (x << 4))) = widen8<F16>(f.w[x], e);
+  };
+  uint32_t exp4 = 0;  // 64 dims; with 128 a key's four come to LDS behind the bytes, by lanes' rows
+  auto fetch_raw = [&](const Place& place, bool isv) __attribute__((always_inline)) {
+    const uint8_t *bytes, *exponent;
+    const int l = fresh_lane();
+    if (!place.ok || (D == 64 && isv != values4) || !place4(place, isv, l, bytes, exponent)) return;
+    const uint32_t raw = lds0 + kRaw + (D == 128 && isv ? kHalf : 0u);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 : : "v"(bytes), "s"(uniform_int(raw + static_cast<uint32_t>(wave) * 1024u)) : "memory", "m0");
+    if constexpr (D == 64) exp4 = *exponent;
+    else if (l % 4 == 0)
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+                   : : "v"(exponent), "s"(uniform_int(raw + 4096u + static_cast<uint32_t>(wave) * 256u)) : "memory", "m0");
+  };
+  auto put_raw = [&](bool isv, uint32_t stage) __attribute__((always_inline)) {
+    if (D == 64 && isv != values4) return;
+    const int l = fresh_lane();
+    const uint8_t* raw = share + kRaw + (D == 128 && isv ? kHalf : 0u);
+    put(Fours{*reinterpret_cast<const u32x4*>(raw + wave * 1024 + l * 16), D == 64 ? exp4 : raw[4096 + wave * 256 + l / 4 * 16 + l % 4]}, stage);
+  };
   auto issue = [&](int t, const Place& place, bool isv, uint32_t stage) {
+    if constexpr (four_bits(SRC)) return fetch_raw(place, isv);
     if (!place.ok) return;
     const int st_bytes = isv ? v_st : k_st;
     const uint8_t* head_base = isv ? v_head : k_head;
@@ -521,14 +632,14 @@ attention16_kernel(const AttnArgs a) {
         base = head_base + static_cast<int64_t>(t * kKeys) * st_bytes;
         r = min(lrow + tr, klen - 1 - t * kKeys);  // (rows past the last key repeat it)
       } else {
-        const int x = SRC == kPages ? 0 : uniform_int((tr + wave * kLoadRows) / 16);
+        const int x = !small_pages(SRC) ? 0 : uniform_int((tr + wave * kLoadRows) / 16);
         int b = place.blk[0], p = place.row + 16 * x;
 #pragma unroll
         for (int y = 1; y < kGroups; ++y) {
           if (x == y) b = place.blk[y];
           if (p >= a.page) p -= a.page;
         }
-        if (SRC == kSmallPages && b < 0) continue;
+        if (small_pages(SRC) && b < 0) continue;
         p += tr - 16 * x;
         base = head_base + b * page_bytes + static_cast<int64_t>(p) * st_bytes;
         r = lrow;
@@ -540,14 +651,21 @@ attention16_kernel(const AttnArgs a) {
 
   // the first tiles' loads, then the queries'
   Place place[3] = {};  // of tiles t, t + 1 and t + 2
+  Fours first[3] = {};  // 4-bit: K and V of the first tile, K of the second
   if (t0 < t1) {
     start_walk();
     place[0] = look_up(t0);
-    issue(t0, place[0], false, 0);
-    issue(t0, place[0], true, kV + kPayload);
+    if constexpr (four_bits(SRC)) {
+      fetch(place[0], false, first[0]);
+      fetch(place[0], true, first[1]);
+    } else {
+      issue(t0, place[0], false, 0);
+      issue(t0, place[0], true, kV + kPayload);
+    }
     if (t0 + 1 < t1) {
       place[1] = look_up(t0 + 1);
-      issue(t0 + 1, place[1], false, kPayload);
+      if constexpr (four_bits(SRC)) fetch(place[1], false, first[2]);
+      else issue(t0 + 1, place[1], false, kPayload);
     }
   }
 
@@ -675,6 +793,11 @@ attention16_kernel(const AttnArgs a) {
   reset();
   {
     uint32_t k_next = kPayload, v_prev = kV;  // stages of K of tile t + 1 and V of tile t - 1
+    if constexpr (four_bits(SRC)) {
+      if (D == 128 || !values4) put(first[0], 0);
+      if (D == 128 || values4) put(first[1], kV + kPayload);
+      if (D == 128 || !values4) put(first[2], kPayload);
+    }
     landed();
     barrier();
 #pragma unroll
@@ -768,8 +891,12 @@ attention16_kernel(const AttnArgs a) {
     // The step that begins iteration t of every wave: K of tile t + 1 and V of
     // tile t - 1 have landed for all; K of tile t + 2 and V of tile t go where K
     // of tile t and V of tile t - 2 were, which every wave is done with.
-    auto begin = [&](int t) {
+    auto begin = [&](int t) __attribute__((always_inline)) {
       landed();
+      if constexpr (four_bits(SRC)) {  // (their stages' last readers are past the barrier before)
+        if (t > t0 && t + 1 < t1) put_raw(false, k_next);
+        if (t > t0 + 1 && t - 1 < t1) put_raw(true, v_prev);
+      }
       barrier();
       if (t + 2 < t1) {
         place[2] = look_up(t + 2);
@@ -835,6 +962,12 @@ attention16_kernel(const AttnArgs a) {
     for (int r = 0; r < 16; ++r) check = fmaf(acc[d][r], 0.f, check);
   if (__builtin_amdgcn_ballot_w64(check != 0.f) != 0 && (SRC == kPacked || a.num_blocks > 0)) {
     reset();
+    // eight dims of a 4-bit row, and one
+    auto exponent_row = [&](bool isv, int key) {
+      key = min(key, kend - 1);
+      const int page = key / a.page, blk = min(max(bt_row[static_cast<int64_t>(page) * a.bt_sn], 0), a.num_blocks - 1), r = key - page * a.page;
+      return isv ? a.vs + h * a.vs_sh + blk * a.vs_sn + r * a.vs_st : a.ks + h * a.ks_sh + blk * a.ks_sn + r * a.ks_st;
+    };
     auto key_row = [&](const uint8_t* head, int64_t page_bytes, int st_bytes, int key) {
       key = min(key, kend - 1);
       if constexpr (SRC == kPacked) return head + static_cast<int64_t>(key) * st_bytes;
@@ -849,23 +982,31 @@ attention16_kernel(const AttnArgs a) {
       float ps;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const uint8_t* row = key_row(k_head, a.k_sn * 2, k_st, key0 + 32 * b + c) + 16 * g;
+        const uint8_t* row = key_row(k_head, a.k_sn * 2, k_st, key0 + 32 * b + c);
+        if constexpr (four_bits(SRC)) {
+          const uint8_t* exponents = exponent_row(false, key0 + 32 * b + c);
 #pragma unroll
-        for (int x = 0; x < kSteps; ++x) scores_step(x, *reinterpret_cast<const u32x4*>(row + 32 * x), sc[b]);
+          for (int x = 0; x < kSteps; ++x)
+            scores_step(x, widen8<F16>(*reinterpret_cast<const uint32_t*>(row + 8 * x + 4 * g), e8m0_value(exponents[x / 2])), sc[b]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < kSteps; ++x) scores_step(x, *reinterpret_cast<const u32x4*>(row + 16 * g + 32 * x), sc[b]);
+        }
       }
       mask(key0, sc);
       settle(sc, pa, ps);
       l_run += ps;
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        const uint8_t* row[8];
+        const uint8_t *row[8], *exponents[8];
         u32x4 seen;  // 1 where the lane's row sees the key of the slot
         constexpr uint32_t kOne = F16 ? 0x3C00u : 0x3F80u;
         const int first = key0 + 16 * m + 4 * g;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = first + 8 * (j / 4) + j % 4;
-          row[j] = key_row(v_head, a.v_sn * 2, v_st, key) + 2 * c;
+          row[j] = key_row(v_head, a.v_sn * 2, v_st, key);
+          if constexpr (four_bits(SRC)) exponents[j] = exponent_row(true, key);
           const uint32_t bit = key <= pos ? kOne : 0u;
           seen[j / 2] = j % 2 ? seen[j / 2] | (bit << 16) : bit;
         }
@@ -875,7 +1016,10 @@ attention16_kernel(const AttnArgs a) {
           uint32_t value[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            value[j] = *reinterpret_cast<const uint16_t*>(row[j] + 64 * n);
+            if constexpr (four_bits(SRC))
+              value[j] = widen8<F16>(row[j][16 * n + c / 2] >> (c % 2 * 4), e8m0_value(exponents[j][n]))[0] & 0xFFFFu;
+            else
+              value[j] = *reinterpret_cast<const uint16_t*>(row[j] + 2 * c + 64 * n);
             const uint32_t finite = (value[j] & T::kInf) == T::kInf ? 0u : value[j];
             clean[j / 2] = j % 2 ? clean[j / 2] | (finite << 16) : finite;
           }
@@ -1084,6 +1228,7 @@ int launch(const AttnArgs& a, hipStream_t stream) {
 template <bool F16, int D, int GROUPS>
 int by_source(const AttnArgs& a, hipStream_t stream) {
   if (a.cu_k != nullptr) return launch<F16, D, kPacked, GROUPS>(a, stream);  // (a table without columns has no address)
+  if (a.four) return a.page % kKeys == 0 ? launch<F16, D, kPages4, GROUPS>(a, stream) : launch<F16, D, kSmallPages4, GROUPS>(a, stream);
   return a.page % kKeys == 0 ? launch<F16, D, kPages, GROUPS>(a, stream) : launch<F16, D, kSmallPages, GROUPS>(a, stream);
 }
 
@@ -1120,6 +1265,7 @@ int dispatch(AttnArgs a, int dtype, int head_dim, const Layout& layout, void* wo
   a.room = a.slots / a.kv_heads;
   a.by_group = divisor(a.group);
   a.by_kv_heads = divisor(a.kv_heads);
+  a.by_page = divisor(std::max(a.page, 1));
   if (dtype == PRISM_DTYPE_F16)
     return head_dim == 128 ? by_groups<true, 128>(a, groups, stream) : by_groups<true, 64>(a, groups, stream);
   return head_dim == 128 ? by_groups<false, 128>(a, groups, stream) : by_groups<false, 64>(a, groups, stream);
@@ -1188,6 +1334,40 @@ int paged_prefill16(const void* q, const int64_t* qs, const void* k, const void*
   a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
   a.k_sn = ks[0], a.k_st = ks[1], a.k_sh = ks[2];
   a.v_sn = vs[0], a.v_st = vs[1], a.v_sh = vs[2];
+  a.bt = bt;
+  a.bt_sb = bts[0], a.bt_sn = bts[1];
+  a.ctx = ctx;
+  a.cu_q = cu_q;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_st = os[0], a.o_sh = os[1];
+  a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+  a.page = page, a.num_blocks = num_blocks, a.width = width, a.total_q = total_q;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.status = status;
+  a.report = report;
+  return dispatch(a, dtype, head_dim, paged_layout(batch, total_q, heads, kv_heads, page, width), workspace, workspace_bytes, stream);
+}
+
+// prism_paged_fp4's chunks; what it checks is checked.  Strides of K and V in bytes.
+int64_t paged_prefill4_workspace_bytes(int batch, int total_q, int heads, int kv_heads, int head_dim, int page, int width) {
+  return paged_layout(batch, total_q, heads, kv_heads, page, width).scratch(head_dim);
+}
+
+int paged_prefill4(const void* q, const int64_t* qs, const void* k, const void* v, int dtype, const int64_t* ks, const int64_t* vs,
+                   const void* ke, const void* ve, const int64_t* kes, const int64_t* ves, const int32_t* bt, const int64_t* bts,
+                   const int32_t* ctx, const int32_t* cu_q, void* out, const int64_t* os, int batch, int total_q, int heads,
+                   int kv_heads, int head_dim, int page, int num_blocks, int width, float scale, int32_t* status, void* workspace,
+                   int64_t workspace_bytes, int32_t* report, hipStream_t stream) {
+  AttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = qs[0], a.q_sh = qs[1];
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.k_sn = ks[0] / 2, a.k_st = ks[1] / 2, a.k_sh = ks[2] / 2;
+  a.v_sn = vs[0] / 2, a.v_st = vs[1] / 2, a.v_sh = vs[2] / 2;
+  a.four = true;  // (an empty cache has no exponents)
+  a.ks = static_cast<const uint8_t*>(ke), a.vs = static_cast<const uint8_t*>(ve);
+  a.ks_sn = kes[0], a.ks_st = kes[1], a.ks_sh = kes[2];
+  a.vs_sn = ves[0], a.vs_st = ves[1], a.vs_sh = ves[2];
   a.bt = bt;
   a.bt_sb = bts[0], a.bt_sn = bts[1];
   a.ctx = ctx;

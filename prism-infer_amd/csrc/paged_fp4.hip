@@ -37,6 +37,15 @@
 #include <algorithm>
 
 namespace prism {
+
+// Chunks in blocks of 128 rows (attention16.hip).
+int64_t paged_prefill4_workspace_bytes(int batch, int total_q, int heads, int kv_heads, int head_dim, int page, int width);
+int paged_prefill4(const void* q, const int64_t* qs, const void* k, const void* v, int dtype, const int64_t* ks, const int64_t* vs,
+                   const void* ke, const void* ve, const int64_t* kes, const int64_t* ves, const int32_t* bt, const int64_t* bts,
+                   const int32_t* ctx, const int32_t* cu_q, void* out, const int64_t* os, int batch, int total_q, int heads,
+                   int kv_heads, int head_dim, int page, int num_blocks, int width, float scale, int32_t* status, void* workspace,
+                   int64_t workspace_bytes, int32_t* report, hipStream_t stream);
+
 namespace {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
@@ -598,6 +607,12 @@ int64_t scratch_bytes(bool chunks, int group, int kv_heads, int head_dim) {
   return Scratch<128, 16>::head(shares) + ((static_cast<int64_t>(2 * shares) << heads_log2(kv_heads)) * (r * head_dim + 2 * r)) * 4;
 }
 
+// Chunks of more than this many rows of a kv head go to blocks of 128 rows.
+#ifndef WIDE_ROWS
+#define WIDE_ROWS 16
+#endif
+bool wide_chunks(int batch, int total_q, int group) { return static_cast<int64_t>(total_q) * group > static_cast<int64_t>(WIDE_ROWS) * batch; }
+
 template <bool F16, int D, int R, bool CHUNK>
 int launch(const Fp4Args& a, hipStream_t stream) {
   const int others = CHUNK ? kPadding + (a.report != nullptr ? 1 : 0) : 0;
@@ -633,6 +648,8 @@ extern "C" int64_t prism_paged_fp4_workspace_bytes(int chunks, int batch, int to
   if (batch <= 0 || total_q <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
       page_size <= 0 || width < 0)
     return 0;
+  if (chunks != 0 && prism::wide_chunks(batch, total_q, num_heads / num_kv_heads))
+    return prism::paged_prefill4_workspace_bytes(batch, total_q, num_heads, num_kv_heads, head_dim, page_size, width);
   return prism::scratch_bytes(chunks != 0, num_heads / num_kv_heads, num_kv_heads, head_dim);
 }
 
@@ -694,10 +711,15 @@ extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strid
       return PRISM_ERR_LAYOUT;
     }
   const int64_t need = prism_paged_fp4_workspace_bytes(chunks, batch, total_q, num_heads, num_kv_heads, head_dim, page_size, width);
-  if (workspace_bytes < need || !workspace || !aligned(workspace, 256)) {
+  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 256)))) {
     set_error("%s: the workspace needs %lld bytes, 256-byte aligned", what, static_cast<long long>(need));
     return PRISM_ERR_INVALID;
   }
+  if (chunks && wide_chunks(batch, total_q, num_heads / num_kv_heads))
+    return paged_prefill4(q, q_strides, k_cache, v_cache, q_dtype, k_strides, v_strides, k_scale, v_scale, ks_strides, vs_strides,
+                          block_tables, bt_strides, context_lens, cu_seqlens_q, out, out_strides, batch, total_q, num_heads,
+                          num_kv_heads, head_dim, page_size, num_blocks, width, scale, status, workspace, need, report,
+                          static_cast<hipStream_t>(stream_ptr));
   Fp4Args a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_st = q_strides[0], a.q_sh = q_strides[1];
