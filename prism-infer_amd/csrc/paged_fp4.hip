@@ -1,40 +1,41 @@
-// Attention over a paged cache of 4-bit keys and values: one query token a
-// sequence, and short chunks of a sequence's last tokens.
+// Attention over a paged cache of 4-bit keys and values, one query token a sequence
+// (chunks of tokens: attention16.hip).
 //
-//   o[j, h] = sum_t w_t v[t, h / G],  w = softmax_t(scale q[j, h] . k[t, h / G]),
-//   k[t] = 2^ek[t, d / 32] E2M1(k4[t, d]), v likewise,
-//
-// over the keys that token j sees.
+//   o[h] = sum_t w_t v[t, h / G],  w = softmax_t(scale q[h] . k[t, h / G]),
+//   k[t, d] = 2^ek[t, d / 32] E2M1(k4[t, d]), v likewise.
 //
 // Per 64 keys of a kv head a wave takes S^T = K Q^T with 16x16x32 bf16 MFMAs.  The
 // order of the contraction is free: lane group g of the operand has the 16 bytes of
 // a key that it loads, in a product for each eight dims, so that a lane's values
 // have one exponent and become bf16 with it, exactly.  (The block-scaled MFMA takes
 // the bytes as they are, but aligns products to the largest with few bits: sums were
-// off by up to 2^-11 of the largest product.)  Queries are bf16; float16 ones, of 11
-// bits, are the sum of two.  A row of scores is one lane column.  P^T is
+// off by up to 2^-11 of the largest product.)  Float16 queries meet float16 keys,
+// 2^-4 of them, which ends at keys of 2^20.  A row of scores is one lane column.  P^T is
 // the B operand of O^T += V^T P^T as it stands; V^T comes from
 // ds_read_b64_tr_b4, 16 keys of a dim at a time, and becomes bf16 exactly.  Values'
 // exponents are by key and 32 dims: they go into the weights.  With R rows a 16-row
 // operand has room for 16 / R of these: column group x holds the weights for the
 // x-th block of dims, and the output of other blocks' columns is dropped.  Weights
-// are rounded to bf16 against fp32 sums.
+// are rounded to bf16 against fp32 sums; for float16 queries they are the sum of two
+// bf16 numbers, whose 16 bits leave the output's 11.
 //
 // Bound by HBM: 2 (D / 2 + D / 32) bytes of a key and head.
 //
-// Work layout.  A workgroup's waves are kv heads, and parts of the keys where there
-// are fewer heads, so that the rows of a token are read together.  A step is 64 keys
-// of each wave.  All sequences' steps are one list, of which a workgroup has an equal
+// Work layout.  A workgroup's four waves are kv heads, and parts of the keys where
+// there are fewer heads.  A step is 64 keys of each wave, which they load together,
+// 16 keys of all their heads each (with a wave's loads its own head's alone, 64 bytes
+// of a key, half lines, the same work stayed at 4.6 TB/s whatever else it did).  All
+// sequences' steps are one list, of which a workgroup has an equal
 // share: parts of a sequence that lies in several shares are joined by a second
 // kernel.
 #include "common.h"
 #include "divide.h"
 #include "fp4.h"
 #include "fp8_mfma.h"
-#include "paged_chunks.h"
 #include "wave_ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace prism {
 
@@ -51,10 +52,8 @@ namespace {
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
-constexpr int kWaves = 8;
+constexpr int kWavesLog2 = 2, kWaves = 1 << kWavesLog2;
 constexpr int kTile = 64;        // keys of a wave's step
-constexpr int kPadding = 64;     // workgroups for rows outside the sequences
-constexpr int kMinSteps = 1;     // of a share
 constexpr int kMostKeys = 0x7FFFF000;  // of a sequence: positions a few steps further fit in 32 bits
 
 struct Fp4Args {
@@ -70,24 +69,24 @@ struct Fp4Args {
   const int32_t* bt;
   int64_t bt_sb, bt_sn;
   const int32_t* ctx;
-  const int32_t* max_ctx;  // one token a sequence
-  const int32_t* cu_q;     // chunks
+  const int32_t* max_ctx;
   uint16_t* out;
   int64_t o_st, o_sh;
-  int batch, heads, kv_heads, group, page, num_blocks, width, total_q;
+  int batch, heads, kv_heads, group, page, num_blocks, width;
   float scale_log2;
-  int* status;
-  int* report;
   int heads_log2;  // of the kv heads of a workgroup
   int shares;      // workgroups
+  int splits;      // descriptions
+  bool by_number;
   uint8_t* work;
-  Divisor by_group, by_page;
+  Divisor by_page;
 };
 
-// A sequence's part of the list that begins in share w and ends in a later one:
-// description w.  Parts: slot 2 w + 1, then slots 2 (w + 1), 2 (w + 2), ...
+// A sequence's part of the list (of a block of rows and a group of kv heads): how many
+// shares it lies in, from share w on.  Parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2),
+// ...  Described by its number where there are as many shares, else by w.
 struct Split {
-  int parts, seq, head, row0, rows, q0;
+  int parts, share, seq, head, row0;
 };
 
 template <int D, int R>
@@ -105,6 +104,13 @@ __device__ __forceinline__ int64_t uniform_int64(int64_t v) {
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
+// The lane, as a value that is not known to be the same one: what is computed from it
+// is computed where it stands, and does not take registers over the whole kernel.
+__device__ __forceinline__ uint32_t fresh(uint32_t lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // LDS writes of a wave are read by its other lanes: program order is enough for the
 // hardware, the compiler has to be told.
 __device__ __forceinline__ void wave_lds_order() {
@@ -113,29 +119,10 @@ __device__ __forceinline__ void wave_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A sequence: its queries, keys, blocks of rows, and steps of a block.
-struct Seq {
-  int q0, qlen, klen, blocks, steps;
-};
-
-template <int R, bool CHUNK>
-__device__ __forceinline__ Seq sequence(const Fp4Args& a, int i, int step_log2) {
-  Seq s{i, 1, a.ctx[i], 0, 0};
+// A sequence's keys.
+__device__ __forceinline__ int keys_of(const Fp4Args& a, int i) {
   const int64_t room = min(static_cast<int64_t>(a.width) * a.page, static_cast<int64_t>(kMostKeys));
-  bool good = true;
-  if (CHUNK) {
-    s.q0 = a.cu_q[i];
-    const int end = a.cu_q[i + 1];
-    good = s.q0 >= 0 && end > s.q0 && end <= a.total_q && s.klen >= end - s.q0 && s.klen <= room;
-    s.qlen = end - s.q0;
-  } else {
-    s.klen = static_cast<int>(min(static_cast<int64_t>(max(min(s.klen, *a.max_ctx), 0)), room));
-  }
-  if (good) {
-    s.blocks = (s.qlen * a.group + R - 1) / R * (a.kv_heads >> a.heads_log2);
-    s.steps = max((s.klen + (1 << step_log2) - 1) >> step_log2, 1);
-  }
-  return s;
+  return static_cast<int>(min(static_cast<int64_t>(max(min(a.ctx[i], *a.max_ctx), 0)), room));
 }
 
 // Two fp32 values -> two bf16 ones, to nearest even.
@@ -150,12 +137,30 @@ __device__ __forceinline__ uint32_t pack_out(float lo, float up) {
 }
 
 // Eight E2M1 codes times a power of two -> bf16, exact.
+constexpr uint32_t kKeyShift = 4;  // float16 keys are 2^-4 of themselves: 65504 rounds to 65536, no float16 number
 __device__ __forceinline__ bf16x8 fp4x8_to_bf16x8(uint32_t w, float scale = 1.0f) {
   const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
   return __builtin_bit_cast(bf16x8, r);
+}
+
+// ... times 2^(e - 127) of an exponent byte, as the scores' operand.
+template <bool F16>
+__device__ __forceinline__ u32x4 widen_key(uint32_t w, uint32_t e) {
+  if constexpr (!F16) return __builtin_bit_cast(u32x4, fp4x8_to_bf16x8(w, __uint_as_float(e << 23)));
+  const float scale = __uint_as_float((max(e, kKeyShift + 1u) - kKeyShift) << 23);
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
+}
+
+template <bool F16>
+__device__ __forceinline__ floatx4 score_product(const u32x4& k, const u32x4& q, floatx4 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
 }
 
 __device__ __forceinline__ float sum_across_groups(float v) {
@@ -178,63 +183,63 @@ struct Shape {
 };
 
 template <bool F16, int D, int R>
-__device__ __forceinline__ void write_row(const Fp4Args& a, const floatx4 (&o)[Shape<D, R>::kVecs], float l, int q0, int head, int row, int lane) {
+__device__ __forceinline__ void write_row(const Fp4Args& a, const floatx4 (&o)[Shape<D, R>::kVecs], float l, int seq, int head, int row, int lane) {
   const float inv = l == 0.f ? 0.f : 1.f / l;  // (no visible key: zeros; a NaN sum goes through)
-  const int tok = divide(row, a.by_group);
-  uint16_t* dst = a.out + static_cast<int64_t>(q0 + tok) * a.o_st + static_cast<int64_t>(head * a.group + row - tok * a.group) * a.o_sh;
+  uint16_t* dst = a.out + static_cast<int64_t>(seq) * a.o_st + static_cast<int64_t>(head * a.group + row) * a.o_sh;
 #pragma unroll
   for (int x = 0; x < Shape<D, R>::kVecs; ++x)
     *reinterpret_cast<u32x2*>(dst + Shape<D, R>::dim(x, lane)) =
         u32x2{pack_out<F16>(o[x][0] * inv, o[x][1] * inv), pack_out<F16>(o[x][2] * inv, o[x][3] * inv)};
 }
 
-template <bool F16, int D, int R, bool CHUNK>
-__global__ void __launch_bounds__(64 * kWaves) paged_fp4_kernel(const Fp4Args a) {
-  constexpr int kRow = D / 2;             // bytes of a key
-  constexpr int kChunks = kRow / 16;
-  constexpr int kVLoads = kTile * kRow / 1024;
-  constexpr int kVKeys = 64 / kChunks;    // keys of a load of values
-  constexpr int kPer = Shape<D, R>::kPer, kSets = Shape<D, R>::kSets, kVecs = Shape<D, R>::kVecs;
-  constexpr int kTerms = F16 ? 2 : 1;     // bf16 terms of a query
-  constexpr int kWords = kRow / 16;       // of a key in a lane: products of the scores
-  constexpr int kStage = kTile * kRow + 2 * kTile * 4;
-  constexpr int kJoin = kVecs * 1024 + 512;
-  constexpr int kShare = (kStage > kJoin ? kStage : kJoin);
-  __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * kShare];
+// Partial results of the same rows together: a part without keys has max -inf and
+// zeros, one whose scores are all NaN max -inf and a NaN sum.
+template <int N>
+__device__ __forceinline__ void join(float& m, float& l, floatx4 (&o)[N], float m1, float l1, const floatx4 (&o1)[N]) {
+  const float top = fmaxf(m, m1);
+  const float w0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - top);
+  l = l != l || l1 != l1 ? __uint_as_float(0x7FC00000u) : l * w0 + l1 * w1;
+#pragma unroll
+  for (int x = 0; x < N; ++x) o[x] = o[x] * w0 + o1[x] * w1;
+  m = top;
+}
 
-  const int lane = threadIdx.x % 64, wave = uniform_int(threadIdx.x / 64);
-  const int n = lane % 16, g = lane / 16;
-  const int wg_heads = 1 << a.heads_log2, subs_log2 = 3 - a.heads_log2;
-  const int my_head = wave & (wg_heads - 1), sub = wave >> a.heads_log2;
+template <bool F16, int D, int R, bool ONE>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3))) paged_fp4_kernel(const Fp4Args a) {
+  constexpr int kRow = D / 2;             // bytes of a key
+  constexpr int kChunks = kRow / 16, kChunksLog2 = D == 128 ? 2 : 1;
+  constexpr int kLoads = kTile * kRow / 1024;  // of a wave, of K and of V
+  constexpr int kPer = Shape<D, R>::kPer, kSets = Shape<D, R>::kSets, kVecs = Shape<D, R>::kVecs;
+  constexpr int kTerms = F16 ? 2 : 1;     // bf16 terms of a weight
+  constexpr int kWords = kRow / 16;       // of a key in a lane: products of the scores
+  // a wave's share of LDS: K, V, their exponents, V's as numbers, by 32 dims; then joined parts
+  constexpr int kKeyExps = 2 * kTile * kRow, kValueExps = kKeyExps + kTile * 4, kNumbers = kValueExps + kTile * 4;
+  constexpr int kStage = kNumbers + kTile * D / 8, kJoin = kVecs * 1024 + 512;
+  constexpr int kShare = (kStage > kJoin ? kStage : kJoin) + 64;  // (heads' rows a quarter of the banks apart)
+  static_assert(kShare % 256 == 64, "rows of four heads meet different banks");
+  __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * kShare];
+  __shared__ int absent[kWaves * 4];  // by 16 keys of a step: 1 where they have no block
+
+  const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
+  const int wave = uniform_int(threadIdx.x / 64);
+  const int heads_log2 = ONE ? kWavesLog2 : a.heads_log2;  // ONE: a wave is a head
+  const int subs_log2 = kWavesLog2 - heads_log2;
+  const int my_head = wave & ((1 << heads_log2) - 1), sub = wave >> heads_log2;
   const int step_log2 = 6 + subs_log2;
-  int me = static_cast<int>(blockIdx.x);
+  const int me = static_cast<int>(blockIdx.x);
   const Scratch<D, R> scratch(a.work, a.shares);
-  if constexpr (CHUNK) {  // the first workgroup may be the check's, the last ones are the padding's
-    if (a.report != nullptr && me == 0) {
-      check_metadata(a, *reinterpret_cast<int*>(lds), [&](int i) {
-        const Seq s = sequence<R, CHUNK>(a, i, step_log2);
-        return s.steps > 0 ? s.klen : -1;
-      });
-      return;
-    }
-    me -= a.report != nullptr ? 1 : 0;
-    if (me >= a.shares) {
-      zero_padding<D>(a, me - a.shares, kPadding);
-      return;
-    }
-  }
+  // a sequence's blocks: of R rows, for each group of kv heads
+  const int head_groups = a.kv_heads >> heads_log2, blocks = head_groups * ((a.group + R - 1) / R);
+  auto steps_of = [&](int keys) { return max((keys + (1 << step_log2) - 1) >> step_log2, 1); };
 
   // ---- this workgroup's share of the list.  A lane has `each` sequences.
   const int each = (a.batch + 63) / 64;
   int64_t mine = 0;
   for (int j = 0; j < each; ++j) {
     const int i = lane * each + j;
-    if (i < a.batch) {
-      const Seq s = sequence<R, CHUNK>(a, i, step_log2);
-      mine += static_cast<int64_t>(s.blocks) * s.steps;
-      if (CHUNK && s.steps == 0 && me == 0 && threadIdx.x < 64) flag_sequence(a, i);
-    }
+    if (i < a.batch) mine += steps_of(keys_of(a, i));
   }
+  mine *= blocks;
   int64_t incl = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -242,302 +247,350 @@ __global__ void __launch_bounds__(64 * kWaves) paged_fp4_kernel(const Fp4Args a)
     incl += lane >= d ? x : 0;
   }
   const int64_t total = uniform_int64(__shfl(incl, 63));
-  const int64_t share = max((total + a.shares - 1) / a.shares, static_cast<int64_t>(kMinSteps));
-  int64_t left_from = me * share;
-  const int64_t left_to = min(left_from + share, total);
-  if (threadIdx.x == 0) scratch.splits[me].parts = 0;
-  if (left_from >= left_to) return;
+  const int64_t share = (total + a.shares - 1) / a.shares;
+  const int64_t from = me * share;
+  int64_t left = min(share, total - from);
+  if (!a.by_number && threadIdx.x == 0) scratch.splits[me].parts = 0;
+  if (left <= 0) return;
   int seq;
   int64_t offset;  // in the sequence
   {
-    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > left_from));
-    offset = left_from - uniform_int64(__shfl(incl - mine, l));
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > from));
+    offset = from - uniform_int64(__shfl(incl - mine, l));
     seq = l * each;
   }
-  int64_t left = left_to - left_from;
 
   uint8_t* const stage = lds + wave * kShare;
-  uint8_t* const v_stage = stage;
-  uint32_t* const ks_stage = reinterpret_cast<uint32_t*>(stage + kTile * kRow);
-  uint32_t* const vs_stage = ks_stage + kTile;
-  const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+  uint8_t* const v_stage = stage + kTile * kRow;
+  uint32_t* const ks_stage = reinterpret_cast<uint32_t*>(stage + kKeyExps);
+  uint32_t* const vs_stage = reinterpret_cast<uint32_t*>(stage + kValueExps);
+  float* const numbers = reinterpret_cast<float*>(stage + kNumbers);
+  const float scale = (a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2)) * (F16 ? static_cast<float>(1u << kKeyShift) : 1.f);
 
   while (left > 0) {
-    Seq s = sequence<R, CHUNK>(a, seq, step_log2);
-    const int64_t all = static_cast<int64_t>(s.blocks) * s.steps;
+    const int klen = uniform_int(keys_of(a, seq)), seq_steps = uniform_int(steps_of(klen));
+    const int64_t all = static_cast<int64_t>(blocks) * seq_steps;
     if (offset >= all) {
       offset -= all;
       ++seq;
       continue;
     }
-    s.q0 = uniform_int(s.q0), s.qlen = uniform_int(s.qlen), s.klen = uniform_int(s.klen), s.steps = uniform_int(s.steps);
-    const int at = uniform_int(static_cast<int>(offset / s.steps));
-    const int step0 = uniform_int(static_cast<int>(offset - static_cast<int64_t>(at) * s.steps));
-    const int steps = uniform_int(static_cast<int>(min(static_cast<int64_t>(s.steps - step0), left)));
-    const int head_groups = a.kv_heads >> a.heads_log2;
+    const int at = uniform_int(static_cast<int>(offset / seq_steps));
+    const int step0 = uniform_int(static_cast<int>(offset - static_cast<int64_t>(at) * seq_steps));
+    const int steps = uniform_int(static_cast<int>(min(static_cast<int64_t>(seq_steps - step0), left)));
     const int row_block = at / head_groups;
-    const int h = ((at - row_block * head_groups) << a.heads_log2) + my_head;
-    const int row0 = row_block * R, rows = s.qlen * a.group;
+    const int h0 = (at - row_block * head_groups) << heads_log2, h = h0 + my_head;
+    const int my_row = row_block * R + n % R;
+    const bool real = my_row < a.group;
 
     // ---- the queries
-    const int my_row = row0 + n % R;
-    const bool real = my_row < rows;
-    const int tok = CHUNK ? divide(min(my_row, rows - 1), a.by_group) : 0;
-    const int first_seen = CHUNK ? s.klen - s.qlen + divide(row0, a.by_group) + 1 : s.klen;  // keys that every row sees
-    const int kend = CHUNK ? s.klen - s.qlen + divide(min(row0 + R, rows) - 1, a.by_group) + 1 : s.klen;
-    const int seen = CHUNK ? s.klen - s.qlen + tok + 1 : s.klen;
-    bf16x8 qop[kTerms][kWords];
+    u32x4 qop[kWords];
     {
-      const uint16_t* src = a.q + static_cast<int64_t>(s.q0 + tok) * a.q_st +
-                            static_cast<int64_t>(h * a.group + min(my_row, rows - 1) - tok * a.group) * a.q_sh;
+      const uint16_t* src = a.q + static_cast<int64_t>(seq) * a.q_st + static_cast<int64_t>(h * a.group + min(my_row, a.group - 1)) * a.q_sh;
       const uint32_t keep = !real || a.scale_log2 == 0.f ? 0u : ~0u, flip = a.scale_log2 < 0.f ? 0x80008000u & keep : 0u;
 #pragma unroll
       for (int x = 0; x < kWords; ++x) {
-        u32x4 w = *reinterpret_cast<const u32x4*>(src + (g * kWords + x) * 8);
+        qop[x] = *reinterpret_cast<const u32x4*>(src + (g * kWords + x) * 8);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = (w[j] & keep) ^ flip;
-          if constexpr (F16) {
-            const float lo = f16_bits_to_f32(w[j] & 0xFFFFu), hi = f16_bits_to_f32(w[j] >> 16);
-            const uint32_t first = pack_bf16(lo, hi);
-            w[j] = first;
-            u32x4 rest = __builtin_bit_cast(u32x4, qop[kTerms - 1][x]);
-            rest[j] = pack_bf16(lo - __uint_as_float(first << 16), hi - __uint_as_float(first & 0xFFFF0000u));
-            qop[kTerms - 1][x] = __builtin_bit_cast(bf16x8, rest);
-          }
-        }
-        qop[0][x] = __builtin_bit_cast(bf16x8, w);
+        for (int j = 0; j < 4; ++j) qop[x][j] = (qop[x][j] & keep) ^ flip;
       }
     }
 
-    // ---- the wave's tiles: t0, t0 + subs, ... below t1
+    // ---- loads of a step: 16 subs keys of all heads.  Keys and values past the L2
+    // (16 x 32768 keys: 120 us, 99 so); exponents of other heads share lines.
     const int subs = 1 << subs_log2;
-    const int need = (kend + kTile - 1) / kTile;
-    int t = (step0 << subs_log2) + sub;
-    const int t1 = min((step0 + steps) << subs_log2, need);
-    const uint8_t* const k_head = a.k + h * a.k_sh;
-    const uint8_t* const v_head = a.v + h * a.v_sh;
-    const uint8_t* const ks_head = a.ks + h * a.ks_sh;
-    const uint8_t* const vs_head = a.vs + h * a.vs_sh;
+    const uint8_t* const k_head = a.k + h0 * a.k_sh;
+    const uint8_t* const v_head = a.v + h0 * a.v_sh;
+    const uint8_t* const ks_head = a.ks + h0 * a.ks_sh;
+    const uint8_t* const vs_head = a.vs + h0 * a.vs_sh;
     const int32_t* bt_row = a.bt + static_cast<int64_t>(seq) * a.bt_sb;
     int ids_base = 0, ids = 0;
     auto load_ids = [&](int base) {
       ids_base = base;
-      ids = bt_row[static_cast<int64_t>(min(base + lane, a.width - 1)) * a.bt_sn];
+      ids = bt_row[static_cast<int64_t>(min(base + static_cast<int>(lane), a.width - 1)) * a.bt_sn];
     };
+    auto first_key = [&](int step) { return (step << step_log2) + (wave << (4 + subs_log2)); };
 
-    typedef uint32_t k_words __attribute__((ext_vector_type(kWords)));
-    k_words kw[4];
-    u32x4 vw[kVLoads];
+    u32x4 kw[kLoads], vw[kLoads];
     uint32_t ksw = 0, vsw = 0;
-    int missing = 0;  // bit x: the x-th 16 keys of the tile are not there
-    auto issue = [&](int tile) {
+    int missing = 0;  // bit x: the x-th 16 keys of the wave's loads are not there
+    typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type exponents;
+    auto issue = [&](int step) {
+      constexpr int kGroups = ONE ? 1 : 4;
       missing = 0;
-      int blk[4], row[4];
+      int blk[kGroups], row[kGroups];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int key = tile * kTile + 16 * x;
+      for (int x = 0; x < kGroups; ++x) {
+        const int key = first_key(step) + 16 * x;
         blk[x] = row[x] = 0;
-        if (key >= kend) {
+        if (x >= subs || key >= klen) {  // (nobody's keys: any bytes of the cache)
           missing |= 1 << x;
           continue;
         }
         const int p = divide(key, a.by_page);
         row[x] = key - p * a.page;
         if (p >= ids_base + 64) load_ids(p);
-        blk[x] = __builtin_amdgcn_readlane(ids, p - ids_base);
+        blk[x] = uniform_int(__builtin_amdgcn_readlane(ids, p - ids_base));
         if (blk[x] < 0 || blk[x] >= a.num_blocks) {
-          if (CHUNK && lane == 0) flag_sequence(a, seq);
           missing |= 1 << x;
           blk[x] = row[x] = 0;
         }
       }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint8_t* base = k_head + blk[x] * a.k_sn + static_cast<int64_t>(row[x]) * a.k_st;
-        kw[x] = *reinterpret_cast<const k_words*>(base + (n * a.k_st + g * 4 * kWords));
-      }
-      {
-        const int x = lane / 16;
-        const int b = x == 0 ? blk[0] : x == 1 ? blk[1] : x == 2 ? blk[2] : blk[3];
-        const int r = (x == 0 ? row[0] : x == 1 ? row[1] : x == 2 ? row[2] : row[3]) + n;
-        const uint8_t* kp = ks_head + b * a.ks_sn + static_cast<int64_t>(r) * a.ks_st;
-        const uint8_t* vp = vs_head + b * a.vs_sn + static_cast<int64_t>(r) * a.vs_st;
-        if constexpr (D == 128) {
-          ksw = *reinterpret_cast<const uint32_t*>(kp);
-          vsw = *reinterpret_cast<const uint32_t*>(vp);
+      // a lane's rows: `key` of the wave's, in the page of its 16
+      auto at = [&](const uint8_t* head, int64_t sn, int st, uint32_t key, uint32_t offset) {
+        if constexpr (ONE) {  // a uniform base, 32-bit offsets of the lanes
+          return head + blk[0] * sn + static_cast<int64_t>(row[0]) * st + (key * st + offset);
         } else {
-          ksw = *reinterpret_cast<const uint16_t*>(kp);
-          vsw = *reinterpret_cast<const uint16_t*>(vp);
-        }
-      }
+          int b = blk[0], r = row[0];
 #pragma unroll
-      for (int x = 0; x < kVLoads; ++x) {
-        int b = blk[x * kVKeys / 16], r = row[x * kVKeys / 16];
-        if (kVKeys == 32 && lane >= 32) b = blk[2 * x + 1], r = row[2 * x + 1];
-        const uint8_t* base = v_head + b * a.v_sn + static_cast<int64_t>(r) * a.v_st;
-        vw[x] = *reinterpret_cast<const u32x4*>(base + (lane / kChunks % 16 * a.v_st + lane % kChunks * 16));
+          for (int x = 1; x < kGroups; ++x) {
+            const int bx = uniform_int(blk[x]), rx = uniform_int(row[x]);  // (as an element by number the table goes to memory)
+            if (key / 16 == x) b = bx, r = rx;
+          }
+          return head + b * sn + (static_cast<int64_t>(r) + key % 16) * st + offset;
+        }
+      };
+      const uint32_t l = fresh(lane), heads = 1u << heads_log2;
+      {
+        const uint32_t key = l >> heads_log2, head = l & (heads - 1);
+        ksw = *reinterpret_cast<const exponents*>(at(ks_head, a.ks_sn, a.ks_st, key, head * static_cast<uint32_t>(a.ks_sh)));
+        vsw = *reinterpret_cast<const exponents*>(at(vs_head, a.vs_sn, a.vs_st, key, head * static_cast<uint32_t>(a.vs_sh)));
+      }
+      const int per = heads_log2 + kChunksLog2;  // lanes of a key
+      const uint32_t head = l / kChunks & (heads - 1), chunk = l % kChunks;
+#pragma unroll
+      for (int x = 0; x < kLoads; ++x) {
+        const uint32_t key = (x << (6 - per)) + (l >> per);
+        kw[x] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at(k_head, a.k_sn, a.k_st, key, head * static_cast<uint32_t>(a.k_sh) + chunk * 16)));
+        vw[x] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at(v_head, a.v_sn, a.v_st, key, head * static_cast<uint32_t>(a.v_sh) + chunk * 16)));
       }
     };
+    // ... to the shares of the waves that compute with them
+    auto deliver = [&]() {
+      const uint32_t l = fresh(lane), heads = 1u << heads_log2;
+      const uint32_t before = (wave & (kWaves - 1)) << (4 + subs_log2);  // keys of the step
+      const int per = heads_log2 + kChunksLog2;
+      const uint32_t head = l / kChunks & (heads - 1), chunk = l % kChunks;
+#pragma unroll
+      for (int x = 0; x < kLoads; ++x) {
+        const uint32_t all = before | x << (6 - per) | l >> per, key = all % kTile;
+        uint8_t* to = lds + (head + (all / kTile << heads_log2)) * kShare + key * kRow;
+        *reinterpret_cast<u32x4*>(to + ((chunk ^ (key / 4 % kChunks)) << 4)) = kw[x];
+        *reinterpret_cast<u32x4*>(to + kTile * kRow + ((chunk ^ (key / 16 % kChunks)) << 4)) = vw[x];
+      }
+      const uint32_t all = before | l >> heads_log2, key = all % kTile;
+      uint32_t* to = reinterpret_cast<uint32_t*>(lds + ((l & (heads - 1)) + (all / kTile << heads_log2)) * kShare + kKeyExps) + key;
+      to[0] = ksw;
+      to[kTile] = vsw;
+      if (l < subs) absent[(wave << subs_log2) + l] = missing >> l & 1;
+    };
+    // (what is in flight to registers stays so)
+    auto meet = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); };
 
+    typedef uint32_t k_words __attribute__((ext_vector_type(kWords)));
     floatx4 acc[D / 16];
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) acc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;
+    int nan_blocks = 0;  // bit x: a key has a NaN exponent for values' 32 dims x; the last one: for its own
 
-    if (t < t1) {
-      load_ids(uniform_int(divide(t * kTile, a.by_page)));
-      issue(t);
+    const int end = klen > 0 ? step0 + steps : step0;  // (without keys there may be no cache)
+    if (step0 < end) {
+      if (first_key(step0) < klen) load_ids(uniform_int(divide(first_key(step0), a.by_page)));
+      issue(step0);
     }
-    for (; t < t1; t += subs) {
-      const int key0 = t * kTile, gone = missing;
-      // ---- values and exponents to LDS, scores
-#pragma unroll
-      for (int x = 0; x < kVLoads; ++x) {
-        const int key = x * kVKeys + lane / kChunks;
-        *reinterpret_cast<u32x4*>(v_stage + key * kRow + ((lane % kChunks ^ (key / 16 % kChunks)) << 4)) = vw[x];
+    for (int step = step0; step < end; ++step) {
+      deliver();
+      meet();
+      if (step + 1 < end) issue(step + 1);
+      const int key0 = (step << step_log2) + sub * kTile;
+      if (key0 >= klen) {
+        meet();
+        continue;
       }
-      ks_stage[lane] = ksw;
-      vs_stage[lane] = vsw;
-      const bool nan_block = (((vsw & 0x7F7F7F7Fu) + 0x01010101u) & vsw & 0x80808080u) != 0;
-      const bool special = __builtin_amdgcn_ballot_w64(nan_block) != 0 || gone != 0 || key0 + kTile > first_seen;
+      const uint32_t lw = fresh(lane);
+      const u32x4 none = *reinterpret_cast<const u32x4*>(absent + 4 * sub);
+      const int gone = uniform_int(static_cast<int>(none[0] | none[1] << 1 | none[2] << 2 | none[3] << 3));
+      const bool partial = gone != 0 || key0 + kTile > klen;
+      uint32_t kx = ks_stage[lw], vx = vs_stage[lw];
+      if (partial && (static_cast<int>(key0 + lw) >= klen || (gone >> (lw / 16) & 1))) kx = vx = 0;  // nobody's: 0 times anything finite
+      auto has_nan = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & w & 0x80808080u; };
+      if (__builtin_amdgcn_ballot_w64((has_nan(kx) | has_nan(vx)) != 0) != 0) {
+        if (has_nan(kx) != 0) nan_blocks |= 1 << (D / 32);
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+          if ((vx >> (8 * x) & 0xFFu) == 0xFFu) vx &= ~(0xFFu << (8 * x)), nan_blocks |= 1 << x;
+      }
+      if (partial) ks_stage[lw] = kx;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) numbers[x * kTile + lw] = __uint_as_float((vx >> (8 * x) & 0xFFu) << 23);
       wave_lds_order();
       floatx4 sc[4];
+      auto scores = [&]() __attribute__((always_inline)) {
+        const uint32_t k_rd = n * kRow + (((D == 128 ? g : g / 2) ^ (n / 4 % kChunks)) << 4) + (D == 128 ? 0 : g % 2 * 8);
+        auto read_k = [&](int x) { return *reinterpret_cast<const k_words*>(stage + k_rd + 16 * x * kRow); };
+        auto read_ke = [&](int x) { return static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(ks_stage)[(16 * x + n) * 4 + (D == 128 ? g : g / 2)]); };
+        k_words w[4];
+        uint32_t ke[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint32_t e = reinterpret_cast<const uint8_t*>(ks_stage)[(16 * x + n) * 4 + (D == 128 ? g : g / 2)];
-        const float ke = e == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(e << 23);
-        sc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int y = 0; y < kWords; ++y) {
-          const bf16x8 key = fp4x8_to_bf16x8(kw[x][y], ke);
-#pragma unroll
-          for (int term = kTerms - 1; term >= 0; --term) sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, qop[term][y], sc[x], 0, 0, 0);
+        for (int x = 0; x < 4; ++x) {
+          w[x] = read_k(x);
+          ke[x] = read_ke(x);
+          sc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
-      }
-      u32x4 ve[4];
+        // (four products that do not wait for each other)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) ve[x] = *reinterpret_cast<const u32x4*>(vs_stage + 16 * x + 4 * g);
-      if (t + subs < t1) issue(t + subs);
+        for (int y = 0; y < kWords; ++y)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[x] = score_product<F16>(widen_key<F16>(w[x][y], ke[x]), qop[y], sc[x]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (partial) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int left_keys = gone >> x & 1 ? 0 : klen - key0 - 16 * x - 4 * static_cast<int>(g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[x][i] = i < left_keys ? sc[x][i] : -INFINITY;
+          }
+        }
+      };
+      scores();
 
-      // ---- softmax
-      if (special) {
+      // ---- softmax.  Weights against the running max as it stands; their sum tells
+      // whether that is high enough (2^8 leaves them finite), or is no number, as
+      // before the first: only then the scores are taken once more, and their max.
+      auto weights = [&](float m) __attribute__((always_inline)) {
+        float sum = 0.f;
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sc[x][i] = key0 + 16 * x + 4 * g + i < seen && !(gone >> x & 1) ? sc[x][i] : -INFINITY;
-      }
-      float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+          for (int i = 0; i < 4; ++i) {
+            sc[x][i] = __builtin_amdgcn_exp2f(fmaf(sc[x][i], scale, -m));
+            sum += sc[x][i];
+          }
+        return sum;
+      };
+      float sum = weights(m_run);
+      if (__builtin_amdgcn_ballot_w64(!(sum <= 256.f)) != 0) {
+        scores();
+        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
 #pragma unroll
-      for (int x = 1; x < 4; ++x) top = fmaxf(top, fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])));
-      top = wave_max_across_groups(top) * scale;
-      const float m_new = fmaxf(m_run, top);
-      if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
+        for (int x = 1; x < 4; ++x) top = fmaxf(top, fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])));
+        top = wave_max_across_groups(top) * scale;
+        const float m_new = fmaxf(m_run, top);
         const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
         l_run *= alpha;
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) acc[x] *= alpha;
         m_run = m_new;
+        sum = weights(m_run == -INFINITY ? 0.f : m_run);
       }
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
-      float p[4][4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[x][i] = __builtin_amdgcn_exp2f(fmaf(sc[x][i], scale, -m_use));
-          l_run += p[x][i];
-        }
+      l_run += sum;
+      __builtin_amdgcn_sched_barrier(0);
 
-      // ---- output
+      // ---- output.  (The lane's place anew: kept, its eight forms take registers.)
+      const uint32_t l = fresh(lane);
+      const uint32_t v_rd = (16 * (l / 4 % 4) + 4 * (l / 16) + l % 4) * kRow + ((l / 4 % 4 % kChunks) << 4);
 #pragma unroll
       for (int set = 0; set < kSets; ++set) {
-        const int shift = 8 * (set * kPer + n / R);
-        u32x4 pw[2];
+        u32x4 pw[kTerms][2];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          float w[4];
+          floatx4 w = sc[x] * *reinterpret_cast<const floatx4*>(numbers + (set * kPer + n / R) * kTile + 16 * x + 4 * g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t e = (ve[x][i] >> shift) & 0xFFu;
-            w[i] = p[x][i] * __uint_as_float(e << 23);
-            if (special) {
-              const bool sees = key0 + 16 * x + 4 * g + i < seen && !(gone >> x & 1);
-              w[i] = !sees ? 0.f : e == 255u ? __uint_as_float(0x7FC00000u) : w[i];
+          for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t two = pack_bf16(w[2 * i], w[2 * i + 1]);
+              pw[term][x / 2][x % 2 * 2 + i] = two;
+              w[2 * i] -= __uint_as_float(two << 16);
+              w[2 * i + 1] -= __uint_as_float(two & 0xFFFF0000u);
+            }
+        }
+        auto read_v = [&](int m) {  // 16 dims of 64 keys
+          return __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(v_stage + ((v_rd ^ (m / 2 << 4)) + m % 2 * 8)));
+        };
+        i32x2 next[2] = {read_v(set * 2 * kPer), read_v(set * 2 * kPer + 1)};
+#pragma unroll
+        for (int y = 0; y < 2 * kPer; y += 2) {
+          const int m = set * 2 * kPer + y;
+          const i32x2 w0 = next[0], w1 = next[1];
+          if (y + 2 < 2 * kPer) next[0] = read_v(m + 2), next[1] = read_v(m + 3);
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const bf16x8 v0 = fp4x8_to_bf16x8(w0[z]), v1 = fp4x8_to_bf16x8(w1[z]);
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term) {
+              acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, __builtin_bit_cast(bf16x8, pw[term][z]), acc[m], 0, 0, 0);
+              acc[m + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, __builtin_bit_cast(bf16x8, pw[term][z]), acc[m + 1], 0, 0, 0);
             }
           }
-          pw[x / 2][x % 2 * 2] = pack_bf16(w[0], w[1]);
-          pw[x / 2][x % 2 * 2 + 1] = pack_bf16(w[2], w[3]);
-        }
-#pragma unroll
-        for (int y = 0; y < 2 * kPer; ++y) {
-          const int m = set * 2 * kPer + y;  // 16 dims
-          const int key = 16 * (n / 4) + 4 * g + n % 4;
-          const uint8_t* src = v_stage + key * kRow + (((m / 2) ^ (n / 4 % kChunks)) << 4) + m % 2 * 8;
-          const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)(src));
-          acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4x8_to_bf16x8(w[0]), __builtin_bit_cast(bf16x8, pw[0]), acc[m], 0, 0, 0);
-          acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4x8_to_bf16x8(w[1]), __builtin_bit_cast(bf16x8, pw[1]), acc[m], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-      wave_lds_order();
+      meet();
     }
 
     // ---- the columns' own blocks
     float l_tot = sum_across_groups(l_run);
+    if (__builtin_amdgcn_ballot_w64(nan_blocks != 0) != 0) {
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x)
+        if (__builtin_amdgcn_ballot_w64(nan_blocks >> x & 1) != 0)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) acc[2 * x][y] = acc[2 * x + 1][y] = __uint_as_float(0x7FC00000u);
+      if (__builtin_amdgcn_ballot_w64(nan_blocks >> (D / 32)) != 0) l_tot = __uint_as_float(0x7FC00000u);
+    }
     floatx4 o[kVecs];
+    const uint32_t le = fresh(lane);
 #pragma unroll
     for (int x = 0; x < kVecs; ++x) {
       o[x] = acc[x / 2 * 2 * kPer + x % 2];
 #pragma unroll
       for (int y = 1; y < kPer; ++y)
-        if (n / R == y) o[x] = acc[(x / 2 * kPer + y) * 2 + x % 2];
+        if (le % 16 / R == y) o[x] = acc[(x / 2 * kPer + y) * 2 + x % 2];
     }
     if (subs > 1) {  // parts of the keys in other waves
       floatx4* own = reinterpret_cast<floatx4*>(stage);
       floatx2* own_ml = reinterpret_cast<floatx2*>(stage + kVecs * 1024);
       if (sub > 0) {
 #pragma unroll
-        for (int x = 0; x < kVecs; ++x) own[x * 64 + lane] = o[x];
-        own_ml[lane] = floatx2{m_run, l_tot};
+        for (int x = 0; x < kVecs; ++x) own[x * 64 + le] = o[x];
+        own_ml[le] = floatx2{m_run, l_tot};
       }
       __syncthreads();
       if (sub == 0) {
         for (int y = 1; y < subs; ++y) {
-          const uint8_t* theirs = lds + (my_head + (y << a.heads_log2)) * kShare;
-          const floatx2 ml = reinterpret_cast<const floatx2*>(theirs + kVecs * 1024)[lane];
-          const float m = fmaxf(m_run, ml[0]);
-          const float w0 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m), w1 = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
-          // (a part without keys has max -inf and zeros; one whose scores are all NaN has max -inf and a NaN sum)
-          l_tot = l_tot != l_tot || ml[1] != ml[1] ? __uint_as_float(0x7FC00000u) : l_tot * w0 + ml[1] * w1;
+          const uint8_t* theirs = lds + (my_head + (y << heads_log2)) * kShare;
+          const floatx2 ml = reinterpret_cast<const floatx2*>(theirs + kVecs * 1024)[le];
+          floatx4 o1[kVecs];
 #pragma unroll
-          for (int x = 0; x < kVecs; ++x) o[x] = o[x] * w0 + reinterpret_cast<const floatx4*>(theirs)[x * 64 + lane] * w1;
-          m_run = m;
+          for (int x = 0; x < kVecs; ++x) o1[x] = reinterpret_cast<const floatx4*>(theirs)[x * 64 + le];
+          join(m_run, l_tot, o, ml[0], ml[1], o1);
         }
       }
       __syncthreads();
     }
-    const bool begins = step0 == 0, ends = step0 + steps == s.steps;
+    const bool begins = step0 == 0, ends = step0 + steps == seq_steps;
     if (begins && ends) {
-      if (sub == 0 && real) write_row<F16, D, R>(a, o, l_tot, s.q0, h, my_row, lane);
+      if (sub == 0 && real) write_row<F16, D, R>(a, o, l_tot, seq, h, row_block * R + le % R, le);
     } else if (sub == 0) {
-      float* part = scratch.parts + (((static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) << a.heads_log2) + my_head) * Scratch<D, R>::kPart;
+      float* part = scratch.parts + (((static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) << heads_log2) + my_head) * Scratch<D, R>::kPart;
 #pragma unroll
-      for (int x = 0; x < kVecs; ++x) reinterpret_cast<floatx4*>(part)[x * 64 + lane] = o[x];
-      if (lane < R) reinterpret_cast<floatx2*>(part + R * D)[lane] = floatx2{m_run, l_tot};
-      if (begins && threadIdx.x == 0) {
-        const int64_t more = (s.steps - steps + share - 1) / share;
-        scratch.splits[me] = Split{1 + static_cast<int>(more), seq, h, row0, rows, s.q0};
-      }
+      for (int x = 0; x < kVecs; ++x) reinterpret_cast<floatx4*>(part)[x * 64 + le] = o[x];
+      if (le < R) reinterpret_cast<floatx2*>(part + R * D)[le] = floatx2{m_run, l_tot};
+    }
+    if (begins && threadIdx.x == 0 && (a.by_number || !ends)) {
+      const int64_t more = (seq_steps - steps + share - 1) / share;
+      scratch.splits[a.by_number ? seq * blocks + at : me] = Split{ends ? 0 : 1 + static_cast<int>(more), me, seq, h, row_block * R};
     }
     left -= steps;
     offset += steps;
   }
 }
 
-// Joins the parts of a split sequence: a workgroup per share that one begins in
-// and head, its waves taking parts in turn.
-constexpr int kJoinWaves = 4;
+// Joins the parts of split sequences: a workgroup per description and head, its waves
+// taking parts in turn.
+constexpr int kJoinWaves = 8;
 
 template <bool F16, int D, int R>
 __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const Fp4Args a) {
@@ -545,22 +598,14 @@ __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const F
   __shared__ floatx4 rows[kJoinWaves][kVecs * 64];
   __shared__ floatx2 stats[kJoinWaves][64];
   const Scratch<D, R> scratch(a.work, a.shares);
-  const int me = static_cast<int>(blockIdx.x) >> a.heads_log2, my_head = static_cast<int>(blockIdx.x) & ((1 << a.heads_log2) - 1);
-  const Split s = scratch.splits[me];
+  const int my_head = static_cast<int>(blockIdx.x) & ((1 << a.heads_log2) - 1);
+  const Split s = scratch.splits[blockIdx.x >> a.heads_log2];
   if (s.parts == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   float m_run = -INFINITY, l_run = 0.f;
   floatx4 o[kVecs];
 #pragma unroll
   for (int x = 0; x < kVecs; ++x) o[x] = floatx4{0.f, 0.f, 0.f, 0.f};
-  auto join = [&](float m1, float l1, const floatx4 (&v)[kVecs]) {
-    const float m = fmaxf(m_run, m1);
-    const float w0 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m), w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
-    l_run = l_run != l_run || l1 != l1 ? __uint_as_float(0x7FC00000u) : l_run * w0 + l1 * w1;
-#pragma unroll
-    for (int x = 0; x < kVecs; ++x) o[x] = o[x] * w0 + v[x] * w1;
-    m_run = m;
-  };
   constexpr int kAtOnce = kVecs <= 2 ? 4 : 2;
   for (int p0 = wave * kAtOnce; p0 < s.parts; p0 += kJoinWaves * kAtOnce) {
     floatx4 v[kAtOnce][kVecs];
@@ -568,7 +613,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const F
 #pragma unroll
     for (int y = 0; y < kAtOnce; ++y) {
       const int p = min(p0 + y, s.parts - 1);
-      const int64_t slot = p == 0 ? 2 * static_cast<int64_t>(me) + 1 : 2 * (static_cast<int64_t>(me) + p);
+      const int64_t slot = p == 0 ? 2 * static_cast<int64_t>(s.share) + 1 : 2 * (static_cast<int64_t>(s.share) + p);
       const float* part = scratch.parts + ((slot << a.heads_log2) + my_head) * kPart;
 #pragma unroll
       for (int x = 0; x < kVecs; ++x) v[y][x] = reinterpret_cast<const floatx4*>(part)[x * 64 + lane];
@@ -576,7 +621,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const F
     }
 #pragma unroll
     for (int y = 0; y < kAtOnce; ++y)
-      if (p0 + y < s.parts) join(ml[y][0], ml[y][1], v[y]);
+      if (p0 + y < s.parts) join(m_run, l_run, o, ml[y][0], ml[y][1], v[y]);
   }
 #pragma unroll
   for (int x = 0; x < kVecs; ++x) rows[wave][x * 64 + lane] = o[x];
@@ -587,58 +632,48 @@ __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const F
     floatx4 v[kVecs];
 #pragma unroll
     for (int x = 0; x < kVecs; ++x) v[x] = rows[y][x * 64 + lane];
-    join(stats[y][lane][0], stats[y][lane][1], v);
+    join(m_run, l_run, o, stats[y][lane][0], stats[y][lane][1], v);
   }
   const int row = s.row0 + lane % R;
-  if (row < s.rows) write_row<F16, D, R>(a, o, l_run, s.q0, s.head + my_head, row, lane);
+  if (row < a.group) write_row<F16, D, R>(a, o, l_run, s.seq, s.head + my_head, row, lane);
 }
 
-int heads_log2(int kv_heads) { return kv_heads % 8 == 0 ? 3 : kv_heads % 4 == 0 ? 2 : kv_heads % 2 == 0 ? 1 : 0; }
+int heads_log2(int kv_heads) { return kv_heads % 4 == 0 ? 2 : kv_heads % 2 == 0 ? 1 : 0; }
 
-int row_block(bool chunks, int group, int head_dim) {
-  if (chunks || group > 8) return 16;
-  return group > 4 || head_dim == 64 ? 8 : 4;
-}
+// Rows of an operand: a kv head's group, rounded up.
+int row_block(int group, int head_dim) { return group > 8 ? 16 : group > 4 || head_dim == 64 ? 8 : 4; }
 
-int share_count() { return 2 * device_cu_count(); }
+int share_count() { return 3 * device_cu_count(); }
 
-int64_t scratch_bytes(bool chunks, int group, int kv_heads, int head_dim) {
-  const int r = row_block(chunks, group, head_dim), shares = share_count();
+int64_t scratch_bytes(int group, int kv_heads, int head_dim) {
+  const int r = row_block(group, head_dim), shares = share_count();
   return Scratch<128, 16>::head(shares) + ((static_cast<int64_t>(2 * shares) << heads_log2(kv_heads)) * (r * head_dim + 2 * r)) * 4;
 }
 
-// Chunks of more than this many rows of a kv head go to blocks of 128 rows.
-#ifndef WIDE_ROWS
-#define WIDE_ROWS 16
-#endif
-bool wide_chunks(int batch, int total_q, int group) { return static_cast<int64_t>(total_q) * group > static_cast<int64_t>(WIDE_ROWS) * batch; }
-
-template <bool F16, int D, int R, bool CHUNK>
+template <bool F16, int D, int R>
 int launch(const Fp4Args& a, hipStream_t stream) {
-  const int others = CHUNK ? kPadding + (a.report != nullptr ? 1 : 0) : 0;
-  hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, CHUNK>), dim3(a.shares + others), dim3(64 * kWaves), 0, stream, a);
+  if (a.heads_log2 == kWavesLog2)
+    hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, true>), dim3(a.shares), dim3(64 * kWaves), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, false>), dim3(a.shares), dim3(64 * kWaves), 0, stream, a);
   if (int rc = check_launch("paged_fp4_kernel launch")) return rc;
-  hipLaunchKernelGGL((paged_fp4_join_kernel<F16, D, R>), dim3(a.shares << a.heads_log2), dim3(64 * kJoinWaves), 0, stream, a);
+  hipLaunchKernelGGL((paged_fp4_join_kernel<F16, D, R>), dim3(a.splits << a.heads_log2), dim3(64 * kJoinWaves), 0, stream, a);
   return check_launch("paged_fp4_join_kernel launch");
 }
 
 template <bool F16>
 int dispatch(const Fp4Args& a, int head_dim, hipStream_t stream) {
-  const bool chunks = a.cu_q != nullptr;
-  const int r = row_block(chunks, a.group, head_dim);
-  if (head_dim == 128) {
-    if (chunks) return launch<F16, 128, 16, true>(a, stream);
-    return r == 4 ? launch<F16, 128, 4, false>(a, stream) : r == 8 ? launch<F16, 128, 8, false>(a, stream) : launch<F16, 128, 16, false>(a, stream);
-  }
-  if (chunks) return launch<F16, 64, 16, true>(a, stream);
-  return r == 8 ? launch<F16, 64, 8, false>(a, stream) : launch<F16, 64, 16, false>(a, stream);
+  const int r = row_block(a.group, head_dim);
+  if (head_dim == 128)
+    return r == 4 ? launch<F16, 128, 4>(a, stream) : r == 8 ? launch<F16, 128, 8>(a, stream) : launch<F16, 128, 16>(a, stream);
+  return r == 8 ? launch<F16, 64, 8>(a, stream) : launch<F16, 64, 16>(a, stream);
 }
 
 }  // namespace
 
 int preload_paged_fp4() {
   hipFuncAttributes attr;
-  return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&paged_fp4_kernel<false, 128, 4, false>)), "preload_paged_fp4");
+  return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&paged_fp4_kernel<false, 128, 4, true>)), "preload_paged_fp4");
 }
 
 }  // namespace prism
@@ -648,9 +683,9 @@ extern "C" int64_t prism_paged_fp4_workspace_bytes(int chunks, int batch, int to
   if (batch <= 0 || total_q <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
       page_size <= 0 || width < 0)
     return 0;
-  if (chunks != 0 && prism::wide_chunks(batch, total_q, num_heads / num_kv_heads))
+  if (chunks != 0)
     return prism::paged_prefill4_workspace_bytes(batch, total_q, num_heads, num_kv_heads, head_dim, page_size, width);
-  return prism::scratch_bytes(chunks != 0, num_heads / num_kv_heads, num_kv_heads, head_dim);
+  return prism::scratch_bytes(num_heads / num_kv_heads, num_kv_heads, head_dim);
 }
 
 extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strides[3], const void* k_cache, const void* v_cache,
@@ -706,8 +741,8 @@ extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strid
     return PRISM_ERR_LAYOUT;
   }
   for (const int64_t* s : {k_strides, v_strides, ks_strides, vs_strides})
-    if (s[1] < 0 || s[1] > INT32_MAX / page_size) {
-      set_error("%s: a page must span less than 2 GiB", what);
+    if (s[1] < 0 || s[1] > INT32_MAX / 2 / page_size || s[2] < 0 || s[2] > INT32_MAX / 8) {
+      set_error("%s: a page must span less than 1 GiB, and eight heads less than 2", what);
       return PRISM_ERR_LAYOUT;
     }
   const int64_t need = prism_paged_fp4_workspace_bytes(chunks, batch, total_q, num_heads, num_kv_heads, head_dim, page_size, width);
@@ -715,7 +750,7 @@ extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strid
     set_error("%s: the workspace needs %lld bytes, 256-byte aligned", what, static_cast<long long>(need));
     return PRISM_ERR_INVALID;
   }
-  if (chunks && wide_chunks(batch, total_q, num_heads / num_kv_heads))
+  if (chunks)
     return paged_prefill4(q, q_strides, k_cache, v_cache, q_dtype, k_strides, v_strides, k_scale, v_scale, ks_strides, vs_strides,
                           block_tables, bt_strides, context_lens, cu_seqlens_q, out, out_strides, batch, total_q, num_heads,
                           num_kv_heads, head_dim, page_size, num_blocks, width, scale, status, workspace, need, report,
@@ -733,19 +768,18 @@ extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strid
   a.bt_sb = bt_strides[0], a.bt_sn = bt_strides[1];
   a.ctx = context_lens;
   a.max_ctx = max_context_len;
-  a.cu_q = cu_seqlens_q;
   a.out = static_cast<uint16_t*>(out);
   a.o_st = out_strides[0], a.o_sh = out_strides[1];
   a.batch = batch, a.heads = num_heads, a.kv_heads = num_kv_heads, a.group = num_heads / num_kv_heads;
-  a.page = page_size, a.num_blocks = num_blocks, a.total_q = total_q;
+  a.page = page_size, a.num_blocks = num_blocks;
   a.width = num_blocks > 0 ? width : 0;  // (without pages nothing is read)
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.status = status;
-  a.report = report;
   a.heads_log2 = heads_log2(num_kv_heads);
   a.shares = share_count();
+  const int64_t numbers = static_cast<int64_t>(batch) * (num_kv_heads >> a.heads_log2) * ceil_div(a.group, row_block(a.group, head_dim));
+  a.by_number = numbers <= a.shares;
+  a.splits = a.by_number ? static_cast<int>(numbers) : a.shares;
   a.work = static_cast<uint8_t*>(workspace);
-  a.by_group = divisor(a.group);
   a.by_page = divisor(page_size);
   hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
   return q_dtype == PRISM_DTYPE_F16 ? dispatch<true>(a, head_dim, stream) : dispatch<false>(a, head_dim, stream);

@@ -58,11 +58,11 @@ def empty_cache(shape, device="cuda", fill=0x55, exponent=127):
     return payload, scales
 
 
-def attend(q, k, v, scale, visible):
+def attend(q, k, v, scale, visible, weight=2.0 ** -8):
     """q [rows, dim], k and v [keys, dim] in 64 bits, visible [rows, keys] -> (output, bound on the kernel's error).
 
     The bound counts, per row, with w the weights and A = sum w |v|:
-      2^-8 A          weights times exponents rounded to bf16;
+      weight A        weights times exponents rounded: 2^-8 to bf16, 2^-11 to float16, 2^-16 to two bf16 numbers;
       2 ds A          weights off because scores are off by up to ds (numerator and denominator);
       2^-18 A         fp32 sums of weights and outputs, parts joined (a few hundred roundings of 2^-24);
       2^-126 sum (|v| + 6)  weights (the largest is 1), and weights times exponents, below the smallest normal number
@@ -82,7 +82,9 @@ def attend(q, k, v, scale, visible):
     ds = torch.where(visible, ds, 0.0).amax(1, keepdim=True)
     at = w @ v.abs()
     lost = 2.0 ** -126 * (visible.double() @ (v.abs() + 6.0))
-    return w @ v, (2.0 ** -8 + 2 * ds + 2.0 ** -18) * at + lost
+    if weight == 2.0 ** -11:  # float16 weights, 2^7 times exp(score - max), end at half of 2^-24
+        lost = lost + 2.0 ** -32 * (visible.double() @ v.abs())
+    return w @ v, (weight + 2 * ds + 2.0 ** -18) * at + lost
 
 
 def check(got: torch.Tensor, want: torch.Tensor, bound: torch.Tensor, label="") -> None:
@@ -140,6 +142,7 @@ class Pool:
 def decode_reference(pool: Pool, q, scale, limit=None):
     """Expected decode output and bound, [batch, heads, dim]."""
 
+    weight = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -16
     q = q.double().cpu()
     out, bound = torch.zeros_like(q), torch.zeros_like(q)
     for i in range(q.shape[0]):
@@ -150,13 +153,14 @@ def decode_reference(pool: Pool, q, scale, limit=None):
         group = q.shape[1] // k.shape[1]
         for h in range(k.shape[1]):
             rows = slice(h * group, (h + 1) * group)
-            out[i, rows], bound[i, rows] = attend(q[i, rows], k[:, h], v[:, h], scale, torch.ones(group, keep.numel(), dtype=torch.bool))
+            out[i, rows], bound[i, rows] = attend(q[i, rows], k[:, h], v[:, h], scale, torch.ones(group, keep.numel(), dtype=torch.bool), weight)
     return out, bound
 
 
 def chunk_reference(pool: Pool, q, cu, scale):
     """Expected chunk output and bound, with q's rows (zeros outside the sequences)."""
 
+    weight = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11
     q = q.double().cpu()
     out, bound = torch.zeros_like(q), torch.zeros_like(q)
     for i, (a, b) in enumerate(zip(cu, cu[1:])):
@@ -166,5 +170,5 @@ def chunk_reference(pool: Pool, q, cu, scale):
         for h in range(k.shape[1]):
             for j in range(h * group, (h + 1) * group):
                 seen = keep[None, :] <= (m - n + torch.arange(n))[:, None]
-                out[a:b, j], bound[a:b, j] = attend(q[a:b, j], k[:, h], v[:, h], scale, seen)
+                out[a:b, j], bound[a:b, j] = attend(q[a:b, j], k[:, h], v[:, h], scale, seen, weight)
     return out, bound
