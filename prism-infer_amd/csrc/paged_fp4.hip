@@ -73,13 +73,14 @@ struct Fp4Args {
   uint16_t* out;
   int64_t o_st, o_sh;
   int batch, heads, kv_heads, group, page, num_blocks, width;
+  int room;  // keys that a block table holds
   float scale_log2;
   int heads_log2;  // of the kv heads of a workgroup
   int shares;      // workgroups
   int splits;      // descriptions
   bool by_number;
   uint8_t* work;
-  Divisor by_page;
+  Divisor by_page, by_shares;
 };
 
 // A sequence's part of the list (of a block of rows and a group of kv heads): how many
@@ -98,12 +99,6 @@ struct Scratch {
   static __host__ __device__ int64_t head(int shares) { return (static_cast<int64_t>(shares) * sizeof(Split) + 255) / 256 * 256; }
 };
 
-__device__ __forceinline__ int64_t uniform_int64(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-
 // The lane, as a value that is not known to be the same one: what is computed from it
 // is computed where it stands, and does not take registers over the whole kernel.
 __device__ __forceinline__ uint32_t fresh(uint32_t lane) {
@@ -120,10 +115,7 @@ __device__ __forceinline__ void wave_lds_order() {
 }
 
 // A sequence's keys.
-__device__ __forceinline__ int keys_of(const Fp4Args& a, int i) {
-  const int64_t room = min(static_cast<int64_t>(a.width) * a.page, static_cast<int64_t>(kMostKeys));
-  return static_cast<int>(min(static_cast<int64_t>(max(min(a.ctx[i], *a.max_ctx), 0)), room));
-}
+__device__ __forceinline__ int keys_of(const Fp4Args& a, int i) { return min(max(min(a.ctx[i], *a.max_ctx), 0), a.room); }
 
 // Two fp32 values -> two bf16 ones, to nearest even.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float up) {
@@ -234,29 +226,23 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 
   // ---- this workgroup's share of the list.  A lane has `each` sequences.
   const int each = (a.batch + 63) / 64;
-  int64_t mine = 0;
+  int mine = 0;
   for (int j = 0; j < each; ++j) {
-    const int i = lane * each + j;
+    const int i = static_cast<int>(lane) * each + j;
     if (i < a.batch) mine += steps_of(keys_of(a, i));
   }
   mine *= blocks;
-  int64_t incl = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t x = __shfl_up(incl, d);
-    incl += lane >= d ? x : 0;
-  }
-  const int64_t total = uniform_int64(__shfl(incl, 63));
-  const int64_t share = (total + a.shares - 1) / a.shares;
-  const int64_t from = me * share;
-  int64_t left = min(share, total - from);
+  const int incl = wave_scan(mine, Add());
+  const int total = __builtin_amdgcn_readlane(incl, 63);
+  const int share = divide(total - 1, a.by_shares) + 1;
+  const int from = me * share;
+  int left = min(share, total - from);
   if (!a.by_number && threadIdx.x == 0) scratch.splits[me].parts = 0;
   if (left <= 0) return;
-  int seq;
-  int64_t offset;  // in the sequence
+  int seq, offset;  // in the sequence
   {
     const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > from));
-    offset = from - uniform_int64(__shfl(incl - mine, l));
+    offset = from - __builtin_amdgcn_readlane(incl - mine, l);
     seq = l * each;
   }
 
@@ -269,15 +255,14 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 
   while (left > 0) {
     const int klen = uniform_int(keys_of(a, seq)), seq_steps = uniform_int(steps_of(klen));
-    const int64_t all = static_cast<int64_t>(blocks) * seq_steps;
+    const int all = blocks * seq_steps;
     if (offset >= all) {
       offset -= all;
       ++seq;
       continue;
     }
-    const int at = uniform_int(static_cast<int>(offset / seq_steps));
-    const int step0 = uniform_int(static_cast<int>(offset - static_cast<int64_t>(at) * seq_steps));
-    const int steps = uniform_int(static_cast<int>(min(static_cast<int64_t>(seq_steps - step0), left)));
+    const int at = uniform_int(static_cast<uint32_t>(offset) / static_cast<uint32_t>(seq_steps));
+    const int step0 = uniform_int(offset - at * seq_steps), steps = uniform_int(min(seq_steps - step0, left));
     const int row_block = at / head_groups;
     const int h0 = (at - row_block * head_groups) << heads_log2, h = h0 + my_head;
     const int my_row = row_block * R + n % R;
@@ -580,8 +565,8 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
       if (le < R) reinterpret_cast<floatx2*>(part + R * D)[le] = floatx2{m_run, l_tot};
     }
     if (begins && threadIdx.x == 0 && (a.by_number || !ends)) {
-      const int64_t more = (seq_steps - steps + share - 1) / share;
-      scratch.splits[a.by_number ? seq * blocks + at : me] = Split{ends ? 0 : 1 + static_cast<int>(more), me, seq, h, row_block * R};
+      scratch.splits[a.by_number ? seq * blocks + at : me] =
+          Split{ends ? 0 : 1 + (seq_steps - steps + share - 1) / share, me, seq, h, row_block * R};
     }
     left -= steps;
     offset += steps;
@@ -773,10 +758,17 @@ extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strid
   a.batch = batch, a.heads = num_heads, a.kv_heads = num_kv_heads, a.group = num_heads / num_kv_heads;
   a.page = page_size, a.num_blocks = num_blocks;
   a.width = num_blocks > 0 ? width : 0;  // (without pages nothing is read)
+  a.room = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.width) * page_size, kMostKeys));
   a.scale_log2 = scale * 1.4426950408889634f;
   a.heads_log2 = heads_log2(num_kv_heads);
   a.shares = share_count();
   const int64_t numbers = static_cast<int64_t>(batch) * (num_kv_heads >> a.heads_log2) * ceil_div(a.group, row_block(a.group, head_dim));
+  // (the steps of the list, and a share beyond it, in 32 bits)
+  if (numbers * (static_cast<int64_t>(a.room) / kTile + 1) > (1 << 30)) {
+    set_error("%s: %lld blocks of rows of up to %d keys are too many steps for one launch", what, static_cast<long long>(numbers), a.room);
+    return PRISM_ERR_INVALID;
+  }
+  a.by_shares = divisor(a.shares);
   a.by_number = numbers <= a.shares;
   a.splits = a.by_number ? static_cast<int>(numbers) : a.shares;
   a.work = static_cast<uint8_t*>(workspace);
