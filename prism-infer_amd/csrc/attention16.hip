@@ -561,64 +561,81 @@ attention16_kernel(const AttnArgs a) {
     uint32_t e;
   };
   constexpr uint32_t kRaw = 4 * kPayload, kHalf = 5120;  // K and V: 4 kB and 1 kB
-  static_assert(2 * kHalf <= 2 * kCols * kRow || D == 64, "the bytes fit behind the stages");
+  constexpr uint32_t kLanes = kRaw + 2 * kHalf;          // with 128 dims: 16 and 8 bytes a lane
+  static_assert((D == 128 ? 2 * kHalf + 6144 : 4096) <= 2 * kCols * kRow, "the bytes fit behind the stages");
   const bool values4 = D == 64 && wave >= 2;  // 64 dims: which of the two the wave has
-  auto row4 = [&](int l) __attribute__((always_inline)) {
-    return D == 128 ? 16 * wave + 4 * (l / 4 % 4) + l / 16
-                    : 32 * (wave % 2) + l / 2 % 2 + 4 * (l / 4 % 2) + 8 * (l / 8 % 2) + 2 * (l / 16 % 2) + 16 * (l / 32);
+  // A lane's place in its wave's rows: byte offsets from the first of them in the
+  // caches, and where its values go in a stage.
+  struct Lane4 {
+    u32x4 from;   // K, V, their exponents
+    u32x2 to;     // values in a stage, with 128 dims its exponent in `raw`
   };
-  auto block4 = [&](int l) { return D == 128 ? l % 4 : l % 2; };
-  // (recomputed each time: kept, what depends on the lane takes registers that the loop needs)
-  auto fresh_lane = [&]() {
-    int l = lane;
+  auto row4 = [](uint32_t l) __attribute__((always_inline)) {
+    return D == 128 ? 4 * (l / 4 % 4) + l / 16 : l / 2 % 2 + 4 * (l / 4 % 2) + 8 * (l / 8 % 2) + 2 * (l / 16 % 2) + 16 * (l / 32);
+  };
+  auto lane4 = [&]() __attribute__((always_inline)) {
+    const uint32_t l = lane, r = row4(l), block = D == 128 ? l % 4 : l % 2;
+    const uint32_t in_page = small_pages(SRC) ? r % 16 : r;
+    return Lane4{{in_page * static_cast<uint32_t>(k_st) + block * 16, in_page * static_cast<uint32_t>(v_st) + block * 16,
+                  in_page * static_cast<uint32_t>(a.ks_st) + block, in_page * static_cast<uint32_t>(a.vs_st) + block},
+                 {r * kRow + (((4 * block) ^ static_cast<uint32_t>(swz<D>(r))) << 4), 4096 + l / 4 * 16 + l % 4}};
+  };
+  // (what depends on the lane anew each time: kept, it takes registers that the loop needs)
+  auto fresh_lane = [&]() __attribute__((always_inline)) {
+    uint32_t l = lane;
     asm volatile("" : "+v"(l));
     return l;
   };
-  auto place4 = [&](const Place& place, bool isv, int l, const uint8_t*& bytes, const uint8_t*& exponent) __attribute__((always_inline)) {
-    int b = place.blk[0], p = place.row + (small_pages(SRC) ? row4(l) % 16 : row4(l));
+  Lane4 kept;  // 64 dims; with 128, whose loop has no register left, in LDS
+  auto from4 = [&]() __attribute__((always_inline)) {
+    if constexpr (D == 64) return kept.from;
+    else return *reinterpret_cast<const u32x4*>(share + kLanes + wave * 1024 + fresh_lane() * 16);
+  };
+  auto to4 = [&]() __attribute__((always_inline)) {
+    if constexpr (D == 64) return kept.to;
+    else return *reinterpret_cast<const u32x2*>(share + kLanes + 4096 + wave * 512 + fresh_lane() * 8);
+  };
+  // the wave's first row of a tile in the caches, and the lane's bytes from there
+  auto place4 = [&](const Place& place, bool isv, const u32x4& from, const uint8_t*& bytes, const uint8_t*& exponent) __attribute__((always_inline)) {
+    int b = uniform_int(place.blk[0]), p = place.row + (small_pages(SRC) ? 0 : D == 128 ? 16 * wave : 32 * (wave % 2));
     if constexpr (SRC == kSmallPages4 && D == 64) {
-      int next = place.row + 16;
-      if (next >= a.page) next -= a.page;
-      if (l >= 32) b = place.blk[kGroups - 1], p = next + row4(l) % 16;
+      const int next = place.row + 16, b1 = uniform_int(place.blk[kGroups - 1]);
+      if (lane >= 32) b = b1, p = next >= a.page ? next - a.page : next;
     }
-    bytes = (isv ? v_head : k_head) + b * ((isv ? a.v_sn : a.k_sn) * 2) + static_cast<int64_t>(p) * (isv ? v_st : k_st) + block4(l) * 16;
-    exponent = (isv ? a.vs + h * a.vs_sh : a.ks + h * a.ks_sh) + b * (isv ? a.vs_sn : a.ks_sn) + p * (isv ? a.vs_st : a.ks_st) + block4(l);
+    bytes = (isv ? v_head : k_head) + b * ((isv ? a.v_sn : a.k_sn) * 2) + static_cast<int64_t>(p) * (isv ? v_st : k_st) + (isv ? from[1] : from[0]);
+    exponent = (isv ? a.vs + h * a.vs_sh : a.ks + h * a.ks_sh) + b * (isv ? a.vs_sn : a.ks_sn) + p * (isv ? a.vs_st : a.ks_st) + (isv ? from[3] : from[2]);
     return b >= 0;
   };
   auto fetch = [&](const Place& place, bool isv, Fours& f) __attribute__((always_inline)) {  // into registers
     const uint8_t *bytes, *exponent;
-    if (!place.ok || (D == 64 && isv != values4) || !place4(place, isv, lane, bytes, exponent)) return;
+    if (!place.ok || (D == 64 && isv != values4) || !place4(place, isv, kept.from, bytes, exponent)) return;
     f.w = *reinterpret_cast<const u32x4*>(bytes);
     f.e = *exponent;
   };
-  auto put = [&](const Fours& f, uint32_t stage) __attribute__((always_inline)) {
-    const int l = fresh_lane(), r = row4(l);
+  auto put = [&](const Fours& f, uint32_t to, uint32_t stage) __attribute__((always_inline)) {
     const float e = f.e == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(f.e << 23);
-    const uint32_t at = stage + r * kRow + (((4 * block4(l)) ^ swz<D>(r)) << 4);
+    const uint32_t at = to + stage + (D == 128 ? 16 * wave : 32 * (wave % 2)) * kRow;
 #pragma unroll
     for (int x = 0; x < 4; ++x) *reinterpret_cast<u32x4*>(share + (at ^ (x << 4))) = widen8<F16>(f.w[x], e);
   };
   uint32_t exp4 = 0;  // 64 dims; with 128 a key's four come to LDS behind the bytes, by lanes' rows
-  auto fetch_raw = [&](const Place& place, bool isv) __attribute__((always_inline)) {
+  auto fetch_raw = [&](const Place& place, bool isv, const u32x4& from) __attribute__((always_inline)) {
     const uint8_t *bytes, *exponent;
-    const int l = fresh_lane();
-    if (!place.ok || (D == 64 && isv != values4) || !place4(place, isv, l, bytes, exponent)) return;
+    if (!place.ok || (D == 64 && isv != values4) || !place4(place, isv, from, bytes, exponent)) return;
     const uint32_t raw = lds0 + kRaw + (D == 128 && isv ? kHalf : 0u);
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  : : "v"(bytes), "s"(uniform_int(raw + static_cast<uint32_t>(wave) * 1024u)) : "memory", "m0");
     if constexpr (D == 64) exp4 = *exponent;
-    else if (l % 4 == 0)
+    else if (fresh_lane() % 4 == 0)
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                    : : "v"(exponent), "s"(uniform_int(raw + 4096u + static_cast<uint32_t>(wave) * 256u)) : "memory", "m0");
   };
-  auto put_raw = [&](bool isv, uint32_t stage) __attribute__((always_inline)) {
+  auto put_raw = [&](bool isv, uint32_t stage, const u32x2& to) __attribute__((always_inline)) {
     if (D == 64 && isv != values4) return;
-    const int l = fresh_lane();
     const uint8_t* raw = share + kRaw + (D == 128 && isv ? kHalf : 0u);
-    put(Fours{*reinterpret_cast<const u32x4*>(raw + wave * 1024 + l * 16), D == 64 ? exp4 : raw[4096 + wave * 256 + l / 4 * 16 + l % 4]}, stage);
+    put(Fours{*reinterpret_cast<const u32x4*>(raw + wave * 1024 + fresh_lane() * 16), D == 64 ? exp4 : raw[wave * 256 + to[1]]}, to[0], stage);
   };
   auto issue = [&](int t, const Place& place, bool isv, uint32_t stage) {
-    if constexpr (four_bits(SRC)) return fetch_raw(place, isv);
     if (!place.ok) return;
     const int st_bytes = isv ? v_st : k_st;
     const uint8_t* head_base = isv ? v_head : k_head;
@@ -651,6 +668,7 @@ attention16_kernel(const AttnArgs a) {
 
   // the first tiles' loads, then the queries'
   Place place[3] = {};  // of tiles t, t + 1 and t + 2
+  if constexpr (four_bits(SRC)) kept = lane4();
   Fours first[3] = {};  // 4-bit: K and V of the first tile, K of the second
   if (t0 < t1) {
     start_walk();
@@ -794,14 +812,19 @@ attention16_kernel(const AttnArgs a) {
   {
     uint32_t k_next = kPayload, v_prev = kV;  // stages of K of tile t + 1 and V of tile t - 1
     if constexpr (four_bits(SRC)) {
-      if (D == 128 || !values4) put(first[0], 0);
-      if (D == 128 || values4) put(first[1], kV + kPayload);
-      if (D == 128 || !values4) put(first[2], kPayload);
+      if (D == 128 || !values4) put(first[0], kept.to[0], 0);
+      if (D == 128 || values4) put(first[1], kept.to[0], kV + kPayload);
+      if (D == 128 || !values4) put(first[2], kept.to[0], kPayload);
     }
     landed();
     barrier();
 #pragma unroll
     for (int x = 0; x < kSteps; ++x) qop[x] = __builtin_bit_cast(vec, *reinterpret_cast<const u32x4*>(share + ((q_lds + k_rd) ^ (x << 5))));
+    if constexpr (four_bits(SRC) && D == 128) {
+      barrier();  // (every wave has its queries)
+      *reinterpret_cast<u32x4*>(share + kLanes + tid * 16) = kept.from;
+      *reinterpret_cast<u32x2*>(share + kLanes + 4096 + tid * 8) = kept.to;
+    }
     // The exponent's scale is positive, so that a masked score is -inf: a negative
     // one is the queries' sign, and with 0 all queries are 0, as they are without a row.
     if (a.scale_log2 <= 0.f || row0 + kCols > rows) {
@@ -894,15 +917,25 @@ attention16_kernel(const AttnArgs a) {
     auto begin = [&](int t) __attribute__((always_inline)) {
       landed();
       if constexpr (four_bits(SRC)) {  // (their stages' last readers are past the barrier before)
-        if (t > t0 && t + 1 < t1) put_raw(false, k_next);
-        if (t > t0 + 1 && t - 1 < t1) put_raw(true, v_prev);
+        const u32x2 to = to4();
+        if (t > t0 && t + 1 < t1) put_raw(false, k_next, to);
+        if (t > t0 + 1 && t - 1 < t1) put_raw(true, v_prev, to);
       }
       barrier();
-      if (t + 2 < t1) {
-        place[2] = look_up(t + 2);
-        issue(t + 2, place[2], false, k_next ^ kPayload);
+      if constexpr (four_bits(SRC)) {
+        const u32x4 from = from4();
+        if (t + 2 < t1) {
+          place[2] = look_up(t + 2);
+          fetch_raw(place[2], false, from);
+        }
+        if (t > t0 && t < t1) fetch_raw(place[0], true, from);
+      } else {
+        if (t + 2 < t1) {
+          place[2] = look_up(t + 2);
+          issue(t + 2, place[2], false, k_next ^ kPayload);
+        }
+        if (t > t0 && t < t1) issue(t, place[0], true, v_prev ^ kPayload);  // (the first is under way)
       }
-      if (t > t0 && t < t1) issue(t, place[0], true, v_prev ^ kPayload);  // (the first is under way)
       place[0] = place[1];
       place[1] = place[2];
     };

@@ -108,7 +108,7 @@ template <int IN>
 __device__ __forceinline__ void store8(char* p, const Raw8<IN>& r) {
 #pragma unroll
   for (int i = 0; i < Raw8<IN>::kWords; i += 4)
-    *(reinterpret_cast<u32x4*>(p) + i / 4) = u32x4{r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]};
+    __builtin_nontemporal_store(u32x4{r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]}, reinterpret_cast<u32x4*>(p) + i / 4);
 }
 
 // Products and their sum, each rounded (no fused step, which would round once).
@@ -379,9 +379,15 @@ int launch_passes(RotateArgs& a, hipStream_t stream) {
   return check_launch("rotate_store_kernel launch");
 }
 
+// A wave's passes share a token's cosines and sines: as many as leave the chip 16
+// waves a CU.  One, two, four, six and twelve passes, us: 8192 tokens of three axes
+// (32 / 8 heads of 128 dims, with the rows read back from a 4-bit cache) -, 66, 55,
+// 49 and 48; 777 tokens (16 / 4 heads of 64) -, 6.2, 6.8, 7.2 and 8.5.
 template <int IN, int LANES>
 int launch_lanes(RotateArgs& a, hipStream_t stream) {
-  return a.tokens >= 512 ? launch_passes<IN, LANES, 4>(a, stream) : launch_passes<IN, LANES, 1>(a, stream);
+  const int64_t passes = ceil_div(a.q_heads + 2 * a.heads, 64 / LANES), enough = 16 * device_cu_count();
+  if (a.tokens * ceil_div(passes, 6) >= enough) return launch_passes<IN, LANES, 6>(a, stream);
+  return a.tokens * ceil_div(passes, 2) >= enough ? launch_passes<IN, LANES, 2>(a, stream) : launch_passes<IN, LANES, 1>(a, stream);
 }
 
 template <int IN>
@@ -400,23 +406,24 @@ struct LoadArgs {
   const uint8_t* scale[2];
   char* out[2];
   const int32_t* slots;
-  int64_t units, num_slots;  // units: of eight values, K then V
+  int64_t num_slots;
+  int units;  // of eight values, of K and of V
   int per_row, heads, kind, cache_dtype, out_dtype;
+  Divisor by_token, by_row;
 };
 
 __global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs a) {
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (unit >= 2 * a.units) return;
-  const int which = unit >= a.units;
-  const int64_t i = unit - which * a.units;
-  const int64_t per_token = static_cast<int64_t>(a.heads) * a.per_row;
-  const int64_t token = i / per_token;
-  const int rest = static_cast<int>(i - token * per_token);
+  const int which = blockIdx.y;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= a.units) return;
+  const int per_token = a.heads * a.per_row;
+  const int token = divide(static_cast<int>(i), a.by_token);
+  const int rest = static_cast<int>(i) - token * per_token;
   const int32_t slot = a.slots[token];
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (slot >= 0 && slot < a.num_slots) {
-    const int64_t at = slot * per_token + rest;  // in eights
-    const int64_t row = static_cast<int64_t>(slot) * a.heads + rest / a.per_row;
+    const int64_t at = static_cast<int64_t>(slot) * per_token + rest;  // in eights
+    const int64_t row = static_cast<int64_t>(slot) * a.heads + divide(rest, a.by_row);
     if (a.kind == kCacheFp4) {
       fp4_decode8(reinterpret_cast<const uint32_t*>(a.cache[which])[at], e8m0_value(a.scale[which][at / 4]), x);
     } else if (a.kind == kCachePlain) {
@@ -445,7 +452,7 @@ __global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs a) {
     u32x4 r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = pack16(a.out_dtype, x[2 * j], x[2 * j + 1]);
-    *(reinterpret_cast<u32x4*>(a.out[which]) + i) = r;
+    __builtin_nontemporal_store(r, reinterpret_cast<u32x4*>(a.out[which]) + i);
   }
 }
 
@@ -608,13 +615,15 @@ extern "C" int prism_kv_load(const void* k_cache, const void* v_cache, int cache
   a.per_row = head_dim / 8;
   a.heads = num_heads;
   a.num_slots = num_slots;
-  a.units = num_tokens * num_heads * a.per_row;
-  a.kind = kind, a.cache_dtype = cache_dtype, a.out_dtype = out_dtype;
-  const int64_t blocks = ceil_div(2 * a.units, 256);
-  if (blocks * 256 > UINT32_MAX) {
+  const int64_t per_token = static_cast<int64_t>(num_heads) * a.per_row;
+  if (per_token > INT32_MAX || num_tokens > INT32_MAX / per_token) {
     set_error("%s: too many rows for one launch", what);
     return PRISM_ERR_INVALID;
   }
-  hipLaunchKernelGGL(kv_load_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  a.units = static_cast<int>(num_tokens * per_token);
+  a.by_token = divisor(static_cast<int>(per_token));
+  a.by_row = divisor(a.per_row);
+  a.kind = kind, a.cache_dtype = cache_dtype, a.out_dtype = out_dtype;
+  hipLaunchKernelGGL(kv_load_kernel, dim3(static_cast<unsigned>(ceil_div(a.units, 256)), 2), dim3(256), 0, static_cast<hipStream_t>(stream), a);
   return check_launch("kv_load_kernel launch");
 }
