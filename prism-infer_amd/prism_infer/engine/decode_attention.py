@@ -1,4 +1,4 @@
-"""One attention layer's decode step on the scaled-FP8 paged KV cache.
+"""One attention layer's decode step on the paged KV cache.
 
 Restates the decode branch of the reference's ``Attention`` layer
 (prism_infer/layers/attention.py:85-111 routing, :115-156 cache-binding
@@ -25,6 +25,7 @@ import torch
 from prism_infer import _native, observability
 from prism_infer.ops.kv_cache_store import store_kvcache
 from prism_infer.ops.paged_decode import _WORKSPACES, DEFAULT_PAGED_DECODE_BLOCK_N, paged_decode_attention
+from prism_infer.ops.rotary_kv_store import rotate_store_kvcache
 
 _HOST = _native.host_ops()
 
@@ -91,12 +92,18 @@ def pack_decode_metadata(slot_mapping, context_lens, block_tables, *, logical_co
 
 
 class PagedKVDecodeAttention:
-    """Decode attention of one layer over its (scaled-)FP8 paged KV cache.
+    """Decode attention of one layer over its paged KV cache.
 
     Bind the layer's caches to ``k_cache`` / ``v_cache`` ([blocks, page,
     kv_heads, head_dim]) and, for the scaled format, ``k_scale_cache`` /
     ``v_scale_cache`` ([blocks, page, kv_heads] fp32), as the reference's
-    model runner does (model_runner.py:817-837).
+    model runner does (model_runner.py:817-837).  A 4-bit cache has payloads
+    [blocks, page, kv_heads, head_dim / 2] and exponents [..., head_dim / 32].
+
+    With ``cos_sin_cache`` bound (fp32 [max_positions, rotary_dim], and
+    ``position_axes`` and ``interleaved_rotary`` as ``rotate_store_kvcache`` has
+    them), queries and keys arrive unrotated: the store is then
+    ``rotate_store_kvcache``, and the rotated queries attend.
     """
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, scale: float):
@@ -110,6 +117,21 @@ class PagedKVDecodeAttention:
         self.v_cache = torch.tensor([])
         self.k_scale_cache: torch.Tensor | None = None
         self.v_scale_cache: torch.Tensor | None = None
+        self.cos_sin_cache: torch.Tensor | None = None
+        self.position_axes: torch.Tensor | None = None
+        self.interleaved_rotary = False
+
+    def _rotate_and_store(self, q, k, v, metadata, positions, return_key: bool = False):
+        """The step's rotated queries (and keys, with ``return_key``); rotated keys and values are stored."""
+
+        if positions is None:
+            positions = getattr(metadata, "positions", None)
+        if positions is None:
+            raise RuntimeError("a bound cos_sin_cache requires the step's positions")
+        return rotate_store_kvcache(q, k, v, self.cos_sin_cache, positions, self.k_cache, self.v_cache,
+                                    metadata.slot_mapping, self.k_scale_cache, self.v_scale_cache,
+                                    position_axes=self.position_axes, interleaved=self.interleaved_rotary,
+                                    return_key=return_key)
 
     def _validate_cache_bindings(self) -> None:
         """The reference's binding checks (attention.py:115-140)."""
@@ -124,12 +146,22 @@ class PagedKVDecodeAttention:
         if self.k_scale_cache is not None and (not self.k_scale_cache.numel() or not self.v_scale_cache.numel()):
             raise RuntimeError("bound K/V scale caches must not be empty")
 
-    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, metadata: DecodeMetadata) -> torch.Tensor:
-        """Store the step's K/V ([B, kv_heads, head_dim]) and attend; q is [B, num_heads, head_dim]."""
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, metadata: DecodeMetadata,
+                positions: torch.Tensor | None = None) -> torch.Tensor:
+        """Store the step's K/V ([B, kv_heads, head_dim]) and attend; q is [B, num_heads, head_dim].
+
+        ``positions`` (default: the metadata's own) are read where a
+        ``cos_sin_cache`` is bound, and refused where none is.
+        """
 
         self._validate_cache_bindings()
         if metadata.slot_mapping is None:
             raise RuntimeError("bound KV cache requires slot_mapping")
+        if self.cos_sin_cache is not None:
+            q = self._rotate_and_store(q, k, v, metadata, positions)
+            return self._attend(q, metadata)
+        if positions is not None:
+            raise RuntimeError("positions need a bound cos_sin_cache")
         # both ops in one native call, and for small batches in one launch; what
         # it does not take, and every call while a profiling provider is
         # installed, goes through the two ops
@@ -141,6 +173,9 @@ class PagedKVDecodeAttention:
                 return out
         store_kvcache(k, v, self.k_cache, self.v_cache, metadata.slot_mapping, self.k_scale_cache,
                       self.v_scale_cache)
+        return self._attend(q, metadata)
+
+    def _attend(self, q: torch.Tensor, metadata: DecodeMetadata) -> torch.Tensor:
         return paged_decode_attention(
             q, self.k_cache, self.v_cache, metadata.block_tables, metadata.context_lens, self.scale,
             k_scale_cache=self.k_scale_cache, v_scale_cache=self.v_scale_cache,

@@ -12,7 +12,8 @@ arguments instead of reading them from a runner:
   cache (``swap_blocks``, :1001-1031).
 
 Payload caches are ``[2, layers, blocks, block_size, kv_heads, head_dim]``;
-token-head scale caches ``[2, layers, blocks, block_size, kv_heads]`` fp32.
+token-head scale caches ``[2, layers, blocks, block_size, kv_heads]`` fp32.  4-bit
+payloads hold ``head_dim / 2`` bytes a row and their exponents ``head_dim / 32``.
 
 On the device, a batch of block or row moves is one launch of the slot
 compaction kernels (``compact_kv_slots``) per cache instead of one torch copy
@@ -31,6 +32,8 @@ import math
 import torch
 
 from prism_infer import _native
+from prism_infer.engine.kv_quantization import fp4_scale_cache_shape
+from prism_infer.ops.kv_cache_store import is_fp4_cache_tensor
 from prism_infer.ops.kv_compaction import compact_kv_slots
 
 PAYLOAD_CACHE_RANK = 6
@@ -43,7 +46,14 @@ def _check_pair(kv_cache: torch.Tensor, scale_cache: torch.Tensor | None) -> Non
             "KV cache must be [2, layers, blocks, block_size, kv_heads, head_dim], "
             f"got {list(kv_cache.shape)}"
         )
-    if scale_cache is not None and tuple(scale_cache.shape) != tuple(kv_cache.shape[:-1]):
+    if is_fp4_cache_tensor(kv_cache):
+        expected = fp4_scale_cache_shape(kv_cache.shape)
+        if scale_cache is not None and tuple(scale_cache.shape) != expected:
+            raise ValueError(
+                "KV scale cache shape must hold one exponent per 32 dims of a 4-bit payload: "
+                f"payload={list(kv_cache.shape)}, scales={list(scale_cache.shape)}"
+            )
+    elif scale_cache is not None and tuple(scale_cache.shape) != tuple(kv_cache.shape[:-1]):
         raise ValueError(
             "KV scale cache shape must equal the payload shape without head_dim: "
             f"payload={list(kv_cache.shape)}, scales={list(scale_cache.shape)}"
@@ -97,7 +107,7 @@ def copy_kv_block_prefixes(kv_cache: torch.Tensor, copies, scale_cache: torch.Te
     slots = num_blocks * block_size
     compact_kv_slots(kv_cache.view(kv, layers, slots, *kv_cache.shape[4:]), src, dst)
     if scale_cache is not None:
-        compact_kv_slots(scale_cache.view(kv, layers, slots, scale_cache.shape[4]), src, dst)
+        compact_kv_slots(scale_cache.view(kv, layers, slots, *scale_cache.shape[4:]), src, dst)
 
 
 def _copy_blocks(dst: torch.Tensor, src: torch.Tensor, dst_ids: list[int], src_ids: list[int], stream) -> None:

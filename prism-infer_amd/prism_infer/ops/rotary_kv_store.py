@@ -28,8 +28,9 @@ from __future__ import annotations
 
 import torch
 
-from prism_infer import _native
-from prism_infer.ops.kv_cache_store import _validate_store_inputs
+from prism_infer import _native, observability
+from prism_infer.observability import profile_region
+from prism_infer.ops.kv_cache_store import _store_profile_region, _validate_store_inputs
 
 HAS_HIP_KERNELS = _native.available()
 _HOST = _native.host_ops()
@@ -76,8 +77,9 @@ def rotate_store_kvcache(
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """Rotate q and key by their positions, store key and value; returns the rotated q (and key, with ``return_key``)."""
 
-    # calls that the native checks accept; the rest goes on below
-    if _HOST is not None:
+    # calls that the native checks accept; the rest, and every call while a
+    # profiling provider is installed, goes on below
+    if _HOST is not None and observability._region_provider is None:
         out = _HOST.rotate_store(q, key, value, cos_sin, positions, k_cache, v_cache, slot_mapping, k_scale_cache,
                                  v_scale_cache, position_axes, interleaved, return_key)
         if out is not None:
@@ -111,19 +113,22 @@ def rotate_store_kvcache(
         q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
         key_out = torch.empty(key.shape, dtype=q.dtype, device=device) if return_key else None
         if tokens > 0:
-            rc = lib.prism_kv_rotate_store(
-                q.data_ptr(), _native.row_strides(q), key.data_ptr(), _native.row_strides(key), value.data_ptr(),
-                _native.row_strides(value), _native.dtype_code(q.dtype), cos_sin.data_ptr(), cos_sin.shape[0],
-                cos_sin.shape[1], int(bool(interleaved)), positions.data_ptr(), tokens,
-                1 if position_axes is None else positions.shape[0],
-                None if position_axes is None else position_axes.data_ptr(), q_out.data_ptr(),
-                None if key_out is None else key_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                _native.dtype_code(k_cache.dtype), k_scale_cache.data_ptr() if scaled else None,
-                v_scale_cache.data_ptr() if scaled else None, slot_mapping.data_ptr(), tokens, q.shape[1], heads, dim,
-                k_cache.numel() // (k_cache.shape[-2] * k_cache.shape[-1]) if k_cache.numel() else 0,
-                _native.stream_handle(device),
-            )
-            _native.check(rc, "rotate_store_kvcache")
+            with profile_region(
+                _store_profile_region(scaled, k_cache), metadata={"cache_dtype": str(k_cache.dtype), "tokens": tokens},
+            ):
+                rc = lib.prism_kv_rotate_store(
+                    q.data_ptr(), _native.row_strides(q), key.data_ptr(), _native.row_strides(key), value.data_ptr(),
+                    _native.row_strides(value), _native.dtype_code(q.dtype), cos_sin.data_ptr(), cos_sin.shape[0],
+                    cos_sin.shape[1], int(bool(interleaved)), positions.data_ptr(), tokens,
+                    1 if position_axes is None else positions.shape[0],
+                    None if position_axes is None else position_axes.data_ptr(), q_out.data_ptr(),
+                    None if key_out is None else key_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                    _native.dtype_code(k_cache.dtype), k_scale_cache.data_ptr() if scaled else None,
+                    v_scale_cache.data_ptr() if scaled else None, slot_mapping.data_ptr(), tokens, q.shape[1], heads, dim,
+                    k_cache.numel() // (k_cache.shape[-2] * k_cache.shape[-1]) if k_cache.numel() else 0,
+                    _native.stream_handle(device),
+                )
+                _native.check(rc, "rotate_store_kvcache")
     return q_out if key_out is None else (q_out, key_out)
 
 
