@@ -63,7 +63,7 @@ def _aligned_scales(scales: torch.Tensor) -> torch.Tensor:
     if (scales.stride(-1) == 1 and scales.data_ptr() % row == 0
             and all(n == 1 or s % row == 0 for n, s in zip(scales.shape[:-1], scales.stride()))):
         return scales
-    return scales.contiguous()
+    return scales.clone(memory_format=torch.contiguous_format)
 
 
 def launch_fp4(what: str, q, k_cache, v_cache, k_scale_cache, v_scale_cache, block_tables, context_lens, scale, *,
