@@ -80,7 +80,7 @@ struct Fp4Args {
   int splits;      // descriptions
   bool by_number;
   uint8_t* work;
-  Divisor by_page, by_shares;
+  Divisor by_page, by_shares, by_cus;
 };
 
 // A sequence's part of the list (of a block of rows and a group of kv heads): how many
@@ -169,18 +169,20 @@ struct Shape {
   static constexpr int kPer = 16 / R;         // blocks of 32 dims beside each other
   static constexpr int kSets = D / 32 / kPer;
   static constexpr int kVecs = 2 * kSets;
+  static constexpr int kJoined = 2;  // vectors of a workgroup that joins parts
   static __device__ __forceinline__ int dim(int x, int lane) {
     return 32 * (x / 2 * kPer + lane % 16 / R) + 16 * (x % 2) + 4 * (lane / 16);
   }
 };
 
-template <bool F16, int D, int R>
-__device__ __forceinline__ void write_row(const Fp4Args& a, const floatx4 (&o)[Shape<D, R>::kVecs], float l, int seq, int head, int row, int lane) {
+// N vectors from x0 on
+template <bool F16, int D, int R, int N>
+__device__ __forceinline__ void write_row(const Fp4Args& a, const floatx4 (&o)[N], float l, int seq, int head, int row, int x0, int lane) {
   const float inv = l == 0.f ? 0.f : 1.f / l;  // (no visible key: zeros; a NaN sum goes through)
   uint16_t* dst = a.out + static_cast<int64_t>(seq) * a.o_st + static_cast<int64_t>(head * a.group + row) * a.o_sh;
 #pragma unroll
-  for (int x = 0; x < Shape<D, R>::kVecs; ++x)
-    *reinterpret_cast<u32x2*>(dst + Shape<D, R>::dim(x, lane)) =
+  for (int x = 0; x < N; ++x)
+    *reinterpret_cast<u32x2*>(dst + Shape<D, R>::dim(x0 + x, lane)) =
         u32x2{pack_out<F16>(o[x][0] * inv, o[x][1] * inv), pack_out<F16>(o[x][2] * inv, o[x][3] * inv)};
 }
 
@@ -234,7 +236,10 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   mine *= blocks;
   const int incl = wave_scan(mine, Add());
   const int total = __builtin_amdgcn_readlane(incl, 63);
-  const int share = divide(total - 1, a.by_shares) + 1;
+  // Its steps: as many as spread the list over the chip's places, but up to three where
+  // it is shorter, for fewer parts (one conversation of 16000 keys 22 -> 17 us, eight of
+  // 2600 18.7 -> 18; of up to a step a CU one: 1800 keys 10.7, with two 14).
+  const int share = max(divide(total - 1, a.by_shares), min(divide(total - 1, a.by_cus), 2)) + 1;
   const int from = me * share;
   int left = min(share, total - from);
   if (!a.by_number && threadIdx.x == 0) scratch.splits[me].parts = 0;
@@ -557,7 +562,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     }
     const bool begins = step0 == 0, ends = step0 + steps == seq_steps;
     if (begins && ends) {
-      if (sub == 0 && real) write_row<F16, D, R>(a, o, l_tot, seq, h, row_block * R + le % R, le);
+      if (sub == 0 && real) write_row<F16, D, R>(a, o, l_tot, seq, h, row_block * R + le % R, 0, le);
     } else if (sub == 0) {
       float* part = scratch.parts + (((static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) << heads_log2) + my_head) * Scratch<D, R>::kPart;
 #pragma unroll
@@ -573,25 +578,25 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   }
 }
 
-// Joins the parts of split sequences: a workgroup per description and head, its waves
-// taking parts in turn.
+// Joins the parts of split sequences: a workgroup per description, head and two
+// vectors, its waves taking parts in turn.
 constexpr int kJoinWaves = 8;
 
 template <bool F16, int D, int R>
 __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const Fp4Args a) {
-  constexpr int kVecs = Shape<D, R>::kVecs, kPart = Scratch<D, R>::kPart;
+  constexpr int kVecs = Shape<D, R>::kJoined, kPart = Scratch<D, R>::kPart;
   __shared__ floatx4 rows[kJoinWaves][kVecs * 64];
   __shared__ floatx2 stats[kJoinWaves][64];
   const Scratch<D, R> scratch(a.work, a.shares);
   const int my_head = static_cast<int>(blockIdx.x) & ((1 << a.heads_log2) - 1);
   const Split s = scratch.splits[blockIdx.x >> a.heads_log2];
   if (s.parts == 0) return;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, x0 = static_cast<int>(blockIdx.y) * kVecs;
   float m_run = -INFINITY, l_run = 0.f;
   floatx4 o[kVecs];
 #pragma unroll
   for (int x = 0; x < kVecs; ++x) o[x] = floatx4{0.f, 0.f, 0.f, 0.f};
-  constexpr int kAtOnce = kVecs <= 2 ? 4 : 2;
+  constexpr int kAtOnce = 4;
   for (int p0 = wave * kAtOnce; p0 < s.parts; p0 += kJoinWaves * kAtOnce) {
     floatx4 v[kAtOnce][kVecs];
     floatx2 ml[kAtOnce];
@@ -601,7 +606,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const F
       const int64_t slot = p == 0 ? 2 * static_cast<int64_t>(s.share) + 1 : 2 * (static_cast<int64_t>(s.share) + p);
       const float* part = scratch.parts + ((slot << a.heads_log2) + my_head) * kPart;
 #pragma unroll
-      for (int x = 0; x < kVecs; ++x) v[y][x] = reinterpret_cast<const floatx4*>(part)[x * 64 + lane];
+      for (int x = 0; x < kVecs; ++x) v[y][x] = reinterpret_cast<const floatx4*>(part)[(x0 + x) * 64 + lane];
       ml[y] = reinterpret_cast<const floatx2*>(part + R * D)[lane % R];
     }
 #pragma unroll
@@ -620,7 +625,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) paged_fp4_join_kernel(const F
     join(m_run, l_run, o, stats[y][lane][0], stats[y][lane][1], v);
   }
   const int row = s.row0 + lane % R;
-  if (row < a.group) write_row<F16, D, R>(a, o, l_run, s.seq, s.head + my_head, row, lane);
+  if (row < a.group) write_row<F16, D, R>(a, o, l_run, s.seq, s.head + my_head, row, x0, lane);
 }
 
 int heads_log2(int kv_heads) { return kv_heads % 4 == 0 ? 2 : kv_heads % 2 == 0 ? 1 : 0; }
@@ -642,7 +647,7 @@ int launch(const Fp4Args& a, hipStream_t stream) {
   else
     hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, false>), dim3(a.shares), dim3(64 * kWaves), 0, stream, a);
   if (int rc = check_launch("paged_fp4_kernel launch")) return rc;
-  hipLaunchKernelGGL((paged_fp4_join_kernel<F16, D, R>), dim3(a.splits << a.heads_log2), dim3(64 * kJoinWaves), 0, stream, a);
+  hipLaunchKernelGGL((paged_fp4_join_kernel<F16, D, R>), dim3(a.splits << a.heads_log2, Shape<D, R>::kVecs / Shape<D, R>::kJoined), dim3(64 * kJoinWaves), 0, stream, a);
   return check_launch("paged_fp4_join_kernel launch");
 }
 
@@ -769,6 +774,7 @@ extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strid
     return PRISM_ERR_INVALID;
   }
   a.by_shares = divisor(a.shares);
+  a.by_cus = divisor(device_cu_count());
   a.by_number = numbers <= a.shares;
   a.splits = a.by_number ? static_cast<int>(numbers) : a.shares;
   a.work = static_cast<uint8_t*>(workspace);
