@@ -466,7 +466,8 @@ int prism_step_metadata(const int32_t* block_tables, const int64_t bt_strides[2]
  * k/v_cache, cache_dtype, k/v_scale, slot_mapping, num_slots : as in
  *              prism_kv_store, or PRISM_DTYPE_FP4_E2M1 with its exponents.  What is
  *              stored of a key is what key_out holds.  With slots < 0 and >=
- *              num_slots only q_out and key_out are written.
+ *              num_slots only q_out and key_out are written.  A slot that several
+ *              tokens name holds parts of any of them.
  * limits     : num_tokens * (num_heads + 2 num_kv_heads) below 2^31.
  */
 int prism_kv_rotate_store(const void* q, const int64_t q_strides[3], const void* key, const int64_t key_strides[3],
@@ -497,7 +498,8 @@ int prism_kv_load(const void* k_cache, const void* v_cache, int cache_dtype, con
  *              or 128, any group num_heads / num_kv_heads.
  * k/v_cache  : [num_blocks, page_size, num_kv_heads, head_dim / 2] bytes, strides
  *              {block, token, head, byte}; byte stride 1, rows 16-byte aligned;
- *              page_size a multiple of 16, pages of less than 2^31 bytes.
+ *              page_size a multiple of 16; page_size token strides at most 2^30
+ *              - 1 bytes, a head stride 2^28 - 1 (k/v_scale likewise).
  * k/v_scale  : [num_blocks, page_size, num_kv_heads, head_dim / 32] exponent bytes,
  *              strides likewise; byte stride 1, rows aligned to their length.
  * block_tables, context_lens, cu_seqlens_q : as in the two entry points.
@@ -512,6 +514,14 @@ int prism_kv_load(const void* k_cache, const void* v_cache, int cache_dtype, con
  *              prism_paged_fp4_workspace_bytes() bytes for the same geometry, as
  *              much as it needs (chunks is 0 where cu_seqlens_q is NULL, else 1).
  *              Calls that may run at once need one each.
+ * precision  : scores, weights' sums and outputs in fp32.  Weights are rounded to
+ *              q_dtype, one token a sequence with F16 queries to 16 bits.  With F16
+ *              queries keys of 2^20 and more (one token a sequence), keys and values
+ *              of 65520 and more (chunks) count as infinite.
+ * limits     : one token a sequence: batch times row blocks (of 4 to 16 heads of a
+ *              group) times kv heads (a quarter of them where 4 divides them, half
+ *              where 2 does), times 64-key steps of the table, at most 2^30.  Chunks
+ *              as prism_paged_prefill_ws over 16-bit caches.
  */
 int64_t prism_paged_fp4_workspace_bytes(int chunks, int batch, int total_q, int num_heads, int num_kv_heads, int head_dim,
                                         int page_size, int width);

@@ -4,8 +4,10 @@ No counterpart in the reference.  The payloads are ``torch.float4_e2m1fn_x2``
 [blocks, page, kv_heads, head_dim / 2] and the exponents ``torch.float8_e8m0fnu``
 [blocks, page, kv_heads, head_dim / 32], as ``store_kvcache`` fills them.  Queries are
 bf16 or fp16, head_dim 64 or 128, any GQA group, pages of a multiple of 16 tokens.
-Scores are exact products of queries and stored keys, summed in fp32; the softmax
-weights, times the values' exponents, are rounded to bf16.
+Scores are exact products of queries and stored keys, summed in fp32.  Softmax
+weights are rounded to the queries' type against fp32 sums (in decode after the values'
+exponents are multiplied in, and for fp16 queries to 16 bits).  With fp16 queries stored
+numbers count as infinite from 65520 on in chunks, keys from 2**20 on in decode.
 """
 
 from __future__ import annotations

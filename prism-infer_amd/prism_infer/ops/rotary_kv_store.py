@@ -18,7 +18,8 @@ and v once, writes the rotated queries, and stores the rotated keys and the valu
 - the caches, scales and slots are those of ``store_kvcache``.  What is stored is bit
   for bit what ``store_kvcache`` stores of the rotated keys, which are rounded to
   their dtype first.  Tokens with slots that are negative or behind the cache are
-  rotated and not stored.
+  rotated and not stored.  Slots are distinct: one that several tokens name holds
+  parts of any of them.
 
 There is no backward pass: inputs that require gradients are refused while gradients
 are recorded.

@@ -160,3 +160,25 @@ def test_a_captured_check_of_drafts():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[:15].clone(), call())
+
+
+@pytest.mark.parametrize("new", [[1, 1], [5, 3], [60, 44]])
+def test_float16_ends_of_the_range(new):
+    """Keys and values from float16's smallest to its largest: all exact there, in chunks and one token at a time."""
+
+    require_gpu()
+    from _fp4 import decode_reference
+    from test_gpu_fp4_attention import decode
+
+    pool = Pool([150, 64], page=16, kv_heads=2, dim=128, seed=45, spread=False)
+    g = torch.Generator().manual_seed(45)
+    for scales in (pool.ks, pool.vs):  # 0.5 * 2^-23 to 6 * 2^13
+        e = scales.view(torch.uint8)
+        e.copy_(torch.randint(104, 141, e.shape, generator=g))
+    cu = [0, new[0], sum(new)]
+    q = queries(cu[-1], 8, 128, F16, seed=45)
+    q = q * 2.0 ** -13  # scores of up to a few hundred
+    want, bound = chunk_reference(pool, q, cu, 0.09)
+    check(chunk(pool, q, cu, 0.09, 2), want, bound, "chunks")
+    want, bound = decode_reference(pool, q[:2], 0.09)
+    check(decode(pool, q[:2], 0.09), want, bound, "one token")
