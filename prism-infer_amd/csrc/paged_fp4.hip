@@ -649,6 +649,8 @@ int launch(const Fp4Args& a, hipStream_t stream) {
   else
     hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, false>), dim3(a.shares), dim3(64 * kWaves), 0, stream, a);
   if (int rc = check_launch("paged_fp4_kernel launch")) return rc;
+  // (of one step a sequence has no parts: 10 sequences of 16 tokens, pages of 16, 8.4 -> 6.8 us)
+  if (a.room <= kTile << (kWavesLog2 - a.heads_log2)) return PRISM_OK;
   hipLaunchKernelGGL((paged_fp4_join_kernel<F16, D, R>), dim3(a.splits << a.heads_log2, Shape<D, R>::kVecs / Shape<D, R>::kJoined), dim3(64 * kJoinWaves), 0, stream, a);
   return check_launch("paged_fp4_join_kernel launch");
 }
