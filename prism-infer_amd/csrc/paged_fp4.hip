@@ -200,7 +200,13 @@ __device__ __forceinline__ void join(float& m, float& l, floatx4 (&o)[N], float 
   m = top;
 }
 
-template <bool F16, int D, int R, bool ONE>
+// How a workgroup's waves meet kv heads and pages: a head each; fewer heads, and the
+// 16 subs keys of a wave's loads in one page; fewer heads, any pages.  (Keys in one
+// page have one base and 32-bit offsets: 64 x 16000 keys of 2 heads, pages of 256,
+// 67.5 us with the last, 57.8 with the second.)
+enum Heads { kFour, kOnePage, kAnyPages };
+
+template <bool F16, int D, int R, Heads HEADS>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3))) paged_fp4_kernel(const Fp4Args a) {
   constexpr int kRow = D / 2;             // bytes of a key
   constexpr int kChunks = kRow / 16, kChunksLog2 = D == 128 ? 2 : 1;
@@ -218,7 +224,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 
   const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
   const int wave = uniform_int(threadIdx.x / 64);
-  const int heads_log2 = ONE ? kWavesLog2 : a.heads_log2;  // ONE: a wave is a head
+  const int heads_log2 = HEADS == kFour ? kWavesLog2 : a.heads_log2;
   const int subs_log2 = kWavesLog2 - heads_log2;
   const int my_head = wave & ((1 << heads_log2) - 1), sub = wave >> heads_log2;
   const int step_log2 = 6 + subs_log2;
@@ -308,7 +314,8 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     int missing = 0;  // bit x: the x-th 16 keys of the wave's loads are not there
     typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type exponents;
     auto issue = [&](int step) {
-      constexpr int kGroups = ONE ? 1 : 4;
+      constexpr int kGroups = HEADS == kAnyPages ? 4 : 1;
+      const int all = HEADS == kOnePage ? (1 << subs) - 1 : 1;
       missing = 0;
       int blk[kGroups], row[kGroups];
 #pragma unroll
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         const int key = first_key(step) + 16 * x;
         blk[x] = row[x] = 0;
         if (x >= subs || key >= klen) {  // (nobody's keys: any bytes of the cache)
-          missing |= 1 << x;
+          missing |= all << x;
           continue;
         }
         const int p = divide(key, a.by_page);
@@ -324,13 +331,13 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         if (p >= ids_base + 64) load_ids(p);
         blk[x] = uniform_int(__builtin_amdgcn_readlane(ids, p - ids_base));
         if (blk[x] < 0 || blk[x] >= a.num_blocks) {
-          missing |= 1 << x;
+          missing |= all << x;
           blk[x] = row[x] = 0;
         }
       }
       // a lane's rows: `key` of the wave's, in the page of its 16
       auto at = [&](const uint8_t* head, int64_t sn, int st, uint32_t key, uint32_t offset) {
-        if constexpr (ONE) {  // a uniform base, 32-bit offsets of the lanes
+        if constexpr (HEADS != kAnyPages) {  // a uniform base, 32-bit offsets of the lanes
           return head + blk[0] * sn + static_cast<int64_t>(row[0]) * st + (key * st + offset);
         } else {
           int b = blk[0], r = row[0];
@@ -644,10 +651,10 @@ int64_t scratch_bytes(int group, int kv_heads, int head_dim) {
 
 template <bool F16, int D, int R>
 int launch(const Fp4Args& a, hipStream_t stream) {
-  if (a.heads_log2 == kWavesLog2)
-    hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, true>), dim3(a.shares), dim3(64 * kWaves), 0, stream, a);
-  else
-    hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, false>), dim3(a.shares), dim3(64 * kWaves), 0, stream, a);
+  const dim3 grid(a.shares), threads(64 * kWaves);
+  if (a.heads_log2 == kWavesLog2) hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, kFour>), grid, threads, 0, stream, a);
+  else if (a.page % (16 << (kWavesLog2 - a.heads_log2)) == 0) hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, kOnePage>), grid, threads, 0, stream, a);
+  else hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, kAnyPages>), grid, threads, 0, stream, a);
   if (int rc = check_launch("paged_fp4_kernel launch")) return rc;
   // (of one step a sequence has no parts: 10 sequences of 16 tokens, pages of 16, 8.4 -> 6.8 us)
   if (a.room <= kTile << (kWavesLog2 - a.heads_log2)) return PRISM_OK;
@@ -667,7 +674,7 @@ int dispatch(const Fp4Args& a, int head_dim, hipStream_t stream) {
 
 int preload_paged_fp4() {
   hipFuncAttributes attr;
-  return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&paged_fp4_kernel<false, 128, 4, true>)), "preload_paged_fp4");
+  return check_hip(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&paged_fp4_kernel<false, 128, 4, kFour>)), "preload_paged_fp4");
 }
 
 }  // namespace prism

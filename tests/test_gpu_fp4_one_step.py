@@ -23,3 +23,17 @@ def test_tables_of_one_step_and_just_more(heads, kv_heads, page, top, batch):
     q = queries(batch, heads, 128, torch.bfloat16, seed=top)
     want, bound = decode_reference(pool, q, 0.09)
     check(decode(pool, q, 0.09), want, bound, f"{batch} of up to {top}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,page,dim", [(4, 1, 64, 128), (8, 2, 32, 128), (6, 3, 128, 64), (4, 1, 48, 128), (8, 2, 16, 64), (8, 4, 16, 128)])
+def test_missing_blocks_by_heads_and_pages(heads, kv_heads, page, dim):
+    """Blocks below 0 and behind the cache are left out, whatever share of a step a page is."""
+
+    require_gpu()
+    pool = Pool([5 * page + 7, 3 * page, 20 * page - 1], page=page, kv_heads=kv_heads, dim=dim, seed=page)
+    pool.tables[0, 1], pool.tables[0, 4], pool.tables[1, :3], pool.tables[2, 19] = -1, pool.kc.shape[0], 2 ** 31 - 1, -5
+    q = queries(3, heads, dim, torch.bfloat16, seed=page)
+    want, bound = decode_reference(pool, q, 0.1)
+    got = decode(pool, q, 0.1)
+    check(got, want, bound, "missing blocks")
+    assert bool((got[1] == 0).all())
