@@ -215,3 +215,24 @@ def test_a_bad_query_spoils_its_own_rows_only(dtype, group):
             for out, weight in ((got, 2.0 ** -8 if dtype == BF16 else 2.0 ** -16), (chunk, 2.0 ** -8 if dtype == BF16 else 2.0 ** -11)):
                 want, bound = attend(q[i, h][None].double(), k[:, h // group], v[:, h // group], 0.09, seen, weight)
                 check(out[i, h][None], want, bound, f"{i}, {h}")
+
+
+@pytest.mark.parametrize("kind", ["fp4", "fp8", "bf16"])
+def test_flat_caches_and_slots_named_twice(monkeypatch, kind):
+    """[slots, heads, dim] caches are the paged ones' rows; a slot may be read back any number of times."""
+
+    require_gpu()
+    q, k, v, g = make(24, 8, 2, 128, BF16, seed=10)
+    cos_sin, slots = table(64, 128).cuda(), torch.randperm(64, generator=g)[:24].int().cuda()
+    positions = torch.arange(24, dtype=torch.int32, device="cuda")
+    paged = make_cache(kind, 4, 16, 2, 128)
+    flat = [None if c is None else c.clone().flatten(0, 1) for c in paged]
+    want = rotary_kv_store.rotate_store_kvcache(q, k, v, cos_sin, positions, *paged[:2], slots, *paged[2:])
+    twice = torch.cat([slots, slots.flip(0), torch.tensor([-1, 64, 2 ** 31 - 1], dtype=torch.int32, device="cuda")])
+    for native in (True, False):
+        call = lambda: (rotary_kv_store.rotate_store_kvcache(q, k, v, cos_sin, positions, *flat[:2], slots, *flat[2:]),  # noqa: E731
+                        kv_cache_load.load_kvcache(*flat[:2], twice, *flat[2:]))
+        got, (key, value) = call() if native else python(monkeypatch, call)
+        assert same_bytes(got, want) and all(same_bytes(a.flatten(0, 1), b) for a, b in zip(paged, flat) if a is not None)
+        for rows in (key, value):
+            assert same_bytes(rows[:24], rows[24:48].flip(0)) and bool((rows[48:] == 0).all())
