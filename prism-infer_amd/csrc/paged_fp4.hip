@@ -56,6 +56,7 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
 constexpr int kWavesLog2 = 2, kWaves = 1 << kWavesLog2;
 constexpr int kTile = 64;        // keys of a wave's step
+constexpr int kWholeSteps = 2;   // up to which a sequence is not split
 constexpr int kMostKeys = 0x7FFFF000;  // of a sequence: positions a few steps further fit in 32 bits
 
 struct Fp4Args {
@@ -81,6 +82,8 @@ struct Fp4Args {
   int shares;      // workgroups
   int splits;      // descriptions
   bool by_number;
+  bool whole;      // sequences are not split: they have few steps each
+  int numbers;     // blocks of rows times groups of kv heads, of all sequences
   uint8_t* work;
   Divisor by_page, by_shares, by_cus;
 };
@@ -233,21 +236,24 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   // a sequence's blocks: of R rows, for each group of kv heads
   const int head_groups = a.kv_heads >> heads_log2, blocks = head_groups * ((a.group + R - 1) / R);
   auto steps_of = [&](int keys) { return max((keys + (1 << step_log2) - 1) >> step_log2, 1); };
+  auto listed = [&](int keys) { return a.whole ? 1 : steps_of(keys); };  // entries of the list
 
   // ---- this workgroup's share of the list.  A lane has `each` sequences.
   const int each = (a.batch + 63) / 64;
   int mine = 0;
   for (int j = 0; j < each; ++j) {
     const int i = static_cast<int>(lane) * each + j;
-    if (i < a.batch) mine += steps_of(keys_of(a, i));
+    if (i < a.batch) mine += listed(keys_of(a, i));
   }
   mine *= blocks;
   const int incl = wave_scan(mine, Add());
   const int total = __builtin_amdgcn_readlane(incl, 63);
   // Its steps: as many as spread the list over the chip's places, but up to three where
-  // it is shorter, for fewer parts (one conversation of 16000 keys 22 -> 17 us, eight of
-  // 2600 18.7 -> 18; of up to a step a CU one: 1800 keys 10.7, with two 14).
-  const int share = max(divide(total - 1, a.by_shares), min(divide(total - 1, a.by_cus), 2)) + 1;
+  // it is shorter and sequences have several, for fewer parts (one conversation of 16000
+  // keys 22 -> 17 us, eight of 2600 18.7 -> 18; of up to a step a CU one: 1800 keys 10.7,
+  // with two 14; 300 sequences of a step or two, one after the other 26.5, else 20).
+  const int least = !a.whole && total / 4 >= a.numbers ? min(divide(total - 1, a.by_cus), 2) : 0;
+  const int share = max(divide(total - 1, a.by_shares), least) + 1;
   const int from = me * share;
   int left = min(share, total - from);
   if (!a.by_number && threadIdx.x == 0) scratch.splits[me].parts = 0;
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   const float scale = (a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2)) * (F16 ? static_cast<float>(1u << kKeyShift) : 1.f);
 
   while (left > 0) {
-    const int klen = uniform_int(keys_of(a, seq)), seq_steps = uniform_int(steps_of(klen));
+    const int klen = uniform_int(keys_of(a, seq)), seq_steps = uniform_int(listed(klen));
     const int all = blocks * seq_steps;
     if (offset >= all) {
       offset -= all;
@@ -393,7 +399,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
     float m_run = -INFINITY, l_run = 0.f;
     int nan_blocks = 0;  // bit x: a key has a NaN exponent for values' 32 dims x; the last one: for its own
 
-    const int end = klen > 0 ? step0 + steps : step0;  // (without keys there may be no cache)
+    const int end = klen > 0 ? step0 + (a.whole ? steps_of(klen) : steps) : step0;  // (without keys there may be no cache)
     if (step0 < end) {
       if (first_key(step0) < klen) load_ids(uniform_int(divide(first_key(step0), a.by_page)));
       issue(step0);
@@ -656,8 +662,7 @@ int launch(const Fp4Args& a, hipStream_t stream) {
   else if (a.page % (16 << (kWavesLog2 - a.heads_log2)) == 0) hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, kOnePage>), grid, threads, 0, stream, a);
   else hipLaunchKernelGGL((paged_fp4_kernel<F16, D, R, kAnyPages>), grid, threads, 0, stream, a);
   if (int rc = check_launch("paged_fp4_kernel launch")) return rc;
-  // (of one step a sequence has no parts: 10 sequences of 16 tokens, pages of 16, 8.4 -> 6.8 us)
-  if (a.room <= kTile << (kWavesLog2 - a.heads_log2)) return PRISM_OK;
+  if (a.whole) return PRISM_OK;
   hipLaunchKernelGGL((paged_fp4_join_kernel<F16, D, R>), dim3(a.splits << a.heads_log2, Shape<D, R>::kVecs / Shape<D, R>::kJoined), dim3(64 * kJoinWaves), 0, stream, a);
   return check_launch("paged_fp4_join_kernel launch");
 }
@@ -787,6 +792,11 @@ extern "C" int prism_paged_fp4(const void* q, int q_dtype, const int64_t q_strid
   a.by_shares = divisor(a.shares);
   a.by_cus = divisor(device_cu_count());
   a.by_number = numbers <= a.shares;
+  a.numbers = static_cast<int>(numbers);
+  // Tables of few steps: parts and their join cost more than a second step in turn (8
+  // heads, pages of 64: 64 sequences of 128 keys 11.1 us split, 9.2 whole; of four steps
+  // 13.8 and 13.9, one sequence 10.1 and 12.4).
+  a.whole = a.room <= kWholeSteps * kTile << (kWavesLog2 - a.heads_log2);
   a.splits = a.by_number ? static_cast<int>(numbers) : a.shares;
   a.work = static_cast<uint8_t*>(workspace);
   a.by_page = divisor(page_size);

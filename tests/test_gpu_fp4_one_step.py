@@ -1,4 +1,4 @@
-"""Decode over 4-bit caches whose tables hold one step of keys a sequence: nothing is split, however many sequences there are."""
+"""Decode over 4-bit caches whose tables hold a few steps of keys a sequence, split or not, and few or many sequences."""
 
 from __future__ import annotations
 
@@ -12,7 +12,8 @@ from test_gpu_fp4_attention import decode, queries
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("heads,kv_heads,page,top", [(32, 8, 16, 64), (8, 2, 64, 128), (4, 1, 256, 256), (20, 1, 16, 255), (32, 8, 16, 65), (8, 2, 64, 129)])
+@pytest.mark.parametrize("heads,kv_heads,page,top", [(32, 8, 16, 64), (8, 2, 64, 128), (4, 1, 256, 256), (20, 1, 16, 255), (32, 8, 16, 65), (8, 2, 64, 129),
+                                                     (32, 8, 64, 128), (8, 2, 64, 256), (4, 1, 256, 512), (32, 8, 16, 129), (8, 2, 64, 257), (4, 1, 16, 600)])
 @pytest.mark.parametrize("batch", [1, 300])
 def test_tables_of_one_step_and_just_more(heads, kv_heads, page, top, batch):
     require_gpu()
