@@ -514,10 +514,10 @@ int prism_kv_load(const void* k_cache, const void* v_cache, int cache_dtype, con
  *              prism_paged_fp4_workspace_bytes() bytes for the same geometry, as
  *              much as it needs (chunks is 0 where cu_seqlens_q is NULL, else 1).
  *              Calls that may run at once need one each.
- * precision  : scores, weights' sums and outputs in fp32.  Weights are rounded to
- *              q_dtype, one token a sequence with F16 queries to 16 bits.  With F16
- *              queries keys of 2^20 and more (one token a sequence), keys and values
- *              of 65520 and more (chunks) count as infinite.
+ * precision  : scores (of keys as they are stored), weights' sums and outputs in
+ *              fp32.  Weights are rounded to q_dtype, one token a sequence with F16
+ *              queries to 16 bits.  With F16 queries keys and values of 65520 and more
+ *              (chunks) count as infinite.
  * limits     : one token a sequence: batch times row blocks (of 4 to 16 heads of a
  *              group) times kv heads (a quarter of them where 4 divides them, half
  *              where 2 does), times 64-key steps of the table, at most 2^30.  Chunks

@@ -10,7 +10,9 @@
 // have one exponent and become bf16 with it, exactly.  (The block-scaled MFMA takes
 // the bytes as they are, but aligns products to the largest with few bits: sums were
 // off by up to 2^-11 of the largest product.)  Float16 queries meet float16 keys,
-// 2^-4 of them, which ends at keys of 2^20.  A row of scores is one lane column.  P^T is
+// 2^-4 of them, where all of a step's keys are such numbers; else bf16 keys, which are
+// exact at every exponent, meet the queries as the sum of two bf16 numbers, exact too, in
+// twice the products.  A row of scores is one lane column.  P^T is
 // the B operand of O^T += V^T P^T as it stands; V^T comes from
 // ds_read_b64_tr_b4, 16 keys of a dim at a time, and becomes bf16 exactly.  Values'
 // exponents are by key and 32 dims: they go into the weights.  With R rows a 16-row
@@ -134,13 +136,37 @@ __device__ __forceinline__ uint32_t pack_out(float lo, float up) {
 }
 
 // Eight E2M1 codes times a power of two -> bf16, exact.
-constexpr uint32_t kKeyShift = 4;  // float16 keys are 2^-4 of themselves: 65504 rounds to 65536, no float16 number
+constexpr uint32_t kKeyShift = 4;  // float16 keys are 2^-4 of themselves: 65504 is held as 65536, no float16 number
 __device__ __forceinline__ bf16x8 fp4x8_to_bf16x8(uint32_t w, float scale = 1.0f) {
   const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
   return __builtin_bit_cast(bf16x8, r);
+}
+
+// Exponent bytes of keys, four a word, that 2^-4 of a float16 number does not hold all
+// codes of: 0.5 * 2^(108 - 127 - 4) is its smallest, 6 * 2^(144 - 127 - 4) ends below its
+// largest.  Of 0 and 1, nobody's keys and blocks of zeros, it makes 0, which such keys'
+// scores are to 2^-100.
+__device__ __forceinline__ uint32_t off_float16(uint32_t w) {
+  const uint32_t low = w & 0x7F7F7F7Fu;
+  const uint32_t above = (low + 0x6F6F6F6Fu) & w;                                // 145 to 255
+  const uint32_t below = (low + 0x7E7E7E7Eu) & ~(low + 0x14141414u) & ~w;        // 2 to 107
+  return (above | below) & 0x80808080u;
+}
+
+// Eight float16 values times 2^-4 -> the sum of two bf16 ones, exact (11 bits are in 8
+// and 3; infinities and NaN are the first's alone).
+__device__ __forceinline__ void split_queries(const u32x4& q, u32x4& first, u32x4& second) {
+  constexpr float unit = 1.0f / (1u << kKeyShift);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float lo = f16_bits_to_f32(q[j] & 0xFFFFu) * unit, up = f16_bits_to_f32(q[j] >> 16) * unit;
+    first[j] = pack_bf16(lo, up);
+    second[j] = pack_bf16(fabsf(lo) < INFINITY ? lo - __uint_as_float(first[j] << 16) : 0.f,
+                          fabsf(up) < INFINITY ? up - __uint_as_float(first[j] & 0xFFFF0000u) : 0.f);
+  }
 }
 
 // ... times 2^(e - 127) of an exponent byte, as the scores' operand.
@@ -430,24 +456,45 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) numbers[x * kTile + lw] = __uint_as_float((vx >> (8 * x) & 0xFFu) << 23);
       wave_lds_order();
+      const bool wide = F16 && __builtin_amdgcn_ballot_w64(off_float16(kx) != 0) != 0;
       floatx4 sc[4];
       auto scores = [&]() __attribute__((always_inline)) {
         const uint32_t k_rd = n * kRow + (((D == 128 ? g : g / 2) ^ (n / 4 % kChunks)) << 4) + (D == 128 ? 0 : g % 2 * 8);
         auto read_k = [&](int x) { return *reinterpret_cast<const k_words*>(stage + k_rd + 16 * x * kRow); };
         auto read_ke = [&](int x) { return static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(ks_stage)[(16 * x + n) * 4 + (D == 128 ? g : g / 2)]); };
-        k_words w[4];
         uint32_t ke[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          w[x] = read_k(x);
           ke[x] = read_ke(x);
           sc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
-        // (four products that do not wait for each other)
+        if (F16 && __builtin_expect(wide, false)) {
 #pragma unroll
-        for (int y = 0; y < kWords; ++y)
+          for (int y = 0; y < kWords; ++y) {
+            uint32_t w[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) sc[x] = score_product<F16>(widen_key<F16>(w[x][y], ke[x]), qop[y], sc[x]);
+            for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<const uint32_t*>(stage + k_rd + 16 * x * kRow + 4 * y);
+            u32x4 whole = qop[y], q[2];
+            asm volatile("" : "+v"(whole));  // (split where it is used: kept, the terms spill)
+            split_queries(whole, q[0], q[1]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const u32x4 k = widen_key<false>(w[x], ke[x]);
+#pragma unroll
+              for (int term = 0; term < 2; ++term) sc[x] = score_product<false>(k, q[term], sc[x]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        } else {
+          k_words w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[x] = read_k(x);
+          // (four products that do not wait for each other)
+#pragma unroll
+          for (int y = 0; y < kWords; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[x] = score_product<F16>(widen_key<F16>(w[x][y], ke[x]), qop[y], sc[x]);
+        }
         __builtin_amdgcn_sched_barrier(0);
         if (partial) {
 #pragma unroll

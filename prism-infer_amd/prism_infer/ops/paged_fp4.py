@@ -7,7 +7,7 @@ bf16 or fp16, head_dim 64 or 128, any GQA group, pages of a multiple of 16 token
 Scores are exact products of queries and stored keys, summed in fp32.  Softmax
 weights are rounded to the queries' type against fp32 sums (in decode after the values'
 exponents are multiplied in, and for fp16 queries to 16 bits).  With fp16 queries stored
-numbers count as infinite from 65520 on in chunks, keys from 2**20 on in decode.
+numbers count as infinite from 65520 on in chunks.
 """
 
 from __future__ import annotations
