@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) acc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;
+    float above = 0.f, most = 256.f;  // of the running max over the scores' own, and of a lane's sum of weights
     int nan_blocks = 0;  // bit x: a key has a NaN exponent for values' 32 dims x; the last one: for its own
 
     const int end = klen > 0 ? step0 + (a.whole ? steps_of(klen) : steps) : step0;  // (without keys there may be no cache)
@@ -446,11 +447,14 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
       uint32_t kx = ks_stage[lw], vx = vs_stage[lw];
       if (partial && (static_cast<int>(key0 + lw) >= klen || (gone >> (lw / 16) & 1))) kx = vx = 0;  // nobody's: 0 times anything finite
       auto has_nan = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & w & 0x80808080u; };
-      if (__builtin_amdgcn_ballot_w64((has_nan(kx) | has_nan(vx)) != 0) != 0) {
+      auto has_large = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x30303030u) & w & 0x80808080u; };  // 208 and more
+      if (__builtin_amdgcn_ballot_w64((has_nan(kx) | has_large(vx)) != 0) != 0) {
         if (has_nan(kx) != 0) nan_blocks |= 1 << (D / 32);
 #pragma unroll
         for (int x = 0; x < D / 32; ++x)
           if ((vx >> (8 * x) & 0xFFu) == 0xFFu) vx &= ~(0xFFu << (8 * x)), nan_blocks |= 1 << x;
+        // Values of up to 2^128: weights of at most 2^-24 leave 2^22 keys' sum of them finite.
+        if (__builtin_amdgcn_ballot_w64(has_large(vx) != 0) != 0) above = 32.f, most = 0x1p-24f;
       }
       if (partial) ks_stage[lw] = kx;
 #pragma unroll
@@ -508,7 +512,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
       scores();
 
       // ---- softmax.  Weights against the running max as it stands; their sum tells
-      // whether that is high enough (2^8 leaves them finite), or is no number, as
+      // whether that is high enough (2^8, beside large values 2^-24), or is no number, as
       // before the first: only then the scores are taken once more, and their max.
       auto weights = [&](float m) __attribute__((always_inline)) {
         float sum = 0.f;
@@ -522,13 +526,13 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
         return sum;
       };
       float sum = weights(m_run);
-      if (__builtin_amdgcn_ballot_w64(!(sum <= 256.f)) != 0) {
+      if (__builtin_amdgcn_ballot_w64(!(sum <= most)) != 0) {
         scores();
         float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
 #pragma unroll
         for (int x = 1; x < 4; ++x) top = fmaxf(top, fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])));
         top = wave_max_across_groups(top) * scale;
-        const float m_new = fmaxf(m_run, top);
+        const float m_new = fmaxf(m_run, top + above);
         const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
         l_run *= alpha;
 #pragma unroll
