@@ -516,8 +516,7 @@ int prism_kv_load(const void* k_cache, const void* v_cache, int cache_dtype, con
  *              Calls that may run at once need one each.
  * precision  : scores (of keys as they are stored), weights' sums and outputs in
  *              fp32.  Weights are rounded to q_dtype, one token a sequence with F16
- *              queries to 16 bits.  With F16 queries keys and values of 65520 and more
- *              (chunks) count as infinite.
+ *              queries to 16 bits.
  * limits     : one token a sequence: batch times row blocks (of 4 to 16 heads of a
  *              group) times kv heads (a quarter of them where 4 divides them, half
  *              where 2 does), times 64-key steps of the table, at most 2^30.  Chunks

@@ -385,7 +385,7 @@ __device__ __forceinline__ uint32_t pack(float lo, float up) {
 }
 
 // Eight 4-bit values times a power of two -> 16-bit ones: exact, but that float16
-// ends at 65504 and at 2^-24, as it does where a cache holds it.
+// ends at 65504 and at 2^-24 (the kernel's last walk is for those beyond).
 template <bool F16>
 __device__ __forceinline__ u32x4 widen8(uint32_t w, float scale) {
   if constexpr (F16)
@@ -415,6 +415,7 @@ attention16_kernel(const AttnArgs a) {
   constexpr int kLoads = kKeys / kLoadRows / kWaves;
   constexpr int kV = 2 * kPayload;            // two stages of K, then two of V
   constexpr int kShare = 4 * kPayload + 2 * kCols * kRow;  // of a group, with the last two waves' queries
+  constexpr bool kNoted = F16 && four_bits(SRC);  // whether a wave has keys that are no float16 numbers
   __shared__ __attribute__((aligned(256))) uint8_t lds[GROUPS * kShare];
 
   // With a report the first workgroups (one per kv head, which keeps the others'
@@ -450,7 +451,7 @@ attention16_kernel(const AttnArgs a) {
   const int wave = uniform_int(tid / 64);
   const int group = GROUPS == 1 ? 0 : uniform_int(threadIdx.x / (64 * kWaves));
   const int lane = tid % 64;
-  const int c = lane % 32;
+  int c = lane % 32;
   const int g = lane / 32;
 
   const Seq s = work.s;
@@ -624,6 +625,15 @@ attention16_kernel(const AttnArgs a) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) *reinterpret_cast<u32x4*>(share + (at ^ (x << 4))) = widen8<F16>(f.w[x], e);
   };
+  // The wave's keys of tile t: whether there are exponents of which float16 does not hold
+  // all codes.  (0.5 * 2^(104 - 127) is its smallest number, 6 * 2^(140 - 127) ends below
+  // its largest; of 0 and 1, which blocks of zeros have, it makes 0, as their scores are
+  // to 2^-100.  Behind the last key there may be anything.)
+  uint32_t noted = 0;
+  auto note = [&](const Fours& f, int t) __attribute__((always_inline)) {
+    if (t * kKeys + (D == 128 ? 16 * wave : 32 * (wave % 2)) < kend)
+      noted |= __builtin_amdgcn_ballot_w64(f.e - 104u > 36u && f.e > 1u) != 0;
+  };
   uint32_t exp4 = 0;  // 64 dims; with 128 a key's four come to LDS behind the bytes, by lanes' rows
   auto fetch_raw = [&](const Place& place, bool isv, const u32x4& from) __attribute__((always_inline)) {
     const uint8_t *bytes, *exponent;
@@ -636,10 +646,12 @@ attention16_kernel(const AttnArgs a) {
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                    : : "v"(exponent), "s"(uniform_int(raw + 4096u + static_cast<uint32_t>(wave) * 256u)) : "memory", "m0");
   };
-  auto put_raw = [&](bool isv, uint32_t stage, const u32x2& to) __attribute__((always_inline)) {
+  auto put_raw = [&](int t, bool isv, uint32_t stage, const u32x2& to) __attribute__((always_inline)) {
     if (D == 64 && isv != values4) return;
     const uint8_t* raw = share + kRaw + (D == 128 && isv ? kHalf : 0u);
-    put(Fours{*reinterpret_cast<const u32x4*>(raw + wave * 1024 + fresh_lane() * 16), D == 64 ? exp4 : raw[wave * 256 + to[1]]}, to[0], stage);
+    const Fours f{*reinterpret_cast<const u32x4*>(raw + wave * 1024 + fresh_lane() * 16), D == 64 ? exp4 : raw[wave * 256 + to[1]]};
+    if (kNoted && !isv) note(f, t);
+    put(f, to[0], stage);
   };
   auto issue = [&](int t, const Place& place, bool isv, uint32_t stage) {
     if (!place.ok) return;
@@ -773,13 +785,14 @@ attention16_kernel(const AttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[b][r] = 32 * b + 8 * (r / 4) + r % 4 <= last ? sc[b][r] : -INFINITY;
   };
-  // Weights of a tile against its maxima, which the accumulators are rescaled to.
-  auto settle = [&](const floatx16 (&sc)[2], u32x4 (&pa)[4], float& ps) {
+  // The running max over a tile's, 2^shift below them, which the accumulators are
+  // rescaled to; returns what weights are formed against.
+  auto rise = [&](const floatx16 (&sc)[2], float shift) __attribute__((always_inline)) {
     float tmax = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
     for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, fmaxf(sc[0][r], sc[1][r]));
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
-    tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale - T::kShift;
+    tmax = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale - shift;
     const float m_new = tmax > m_run ? tmax : m_run;
     // (no key seen: keep the accumulators, all zero, from (-inf) - (-inf))
     const float alpha = m_new > m_run ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
@@ -789,7 +802,11 @@ attention16_kernel(const AttnArgs a) {
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    return m_new == -INFINITY ? 0.f : m_new;
+  };
+  // Weights of a tile against its maxima.
+  auto settle = [&](const floatx16 (&sc)[2], u32x4 (&pa)[4], float& ps) {
+    const float m_use = rise(sc, T::kShift);
     ps = 0.f;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -817,6 +834,7 @@ attention16_kernel(const AttnArgs a) {
   reset();
   {
     uint32_t k_next = kPayload, v_prev = kV;  // stages of K of tile t + 1 and V of tile t - 1
+    if (kNoted && (D == 128 || !values4)) note(first[0], t0), note(first[2], t0 + 1);
     if constexpr (four_bits(SRC)) {
       if (D == 128 || !values4) put(first[0], kept.to[0], 0);
       if (D == 128 || values4) put(first[1], kept.to[0], kV + kPayload);
@@ -924,8 +942,8 @@ attention16_kernel(const AttnArgs a) {
       landed();
       if constexpr (four_bits(SRC)) {  // (their stages' last readers are past the barrier before)
         const u32x2 to = to4();
-        if (t > t0 && t + 1 < t1) put_raw(false, k_next, to);
-        if (t > t0 + 1 && t - 1 < t1) put_raw(true, v_prev, to);
+        if (t > t0 && t + 1 < t1) put_raw(t + 1, false, k_next, to);
+        if (t > t0 + 1 && t - 1 < t1) put_raw(t - 1, true, v_prev, to);
       }
       barrier();
       if constexpr (four_bits(SRC)) {
@@ -993,13 +1011,24 @@ attention16_kernel(const AttnArgs a) {
   // 0.  A wave with an output that is not finite walks its tiles once more, one
   // thing after the other and straight from memory (the others may be done):
   // such values are taken out of the product and added to the rows that see
-  // their key.
+  // their key.  So do waves of float16 queries whose 4-bit keys or values are no
+  // float16 numbers: as bf16, with the queries and weights in two terms.
+  if constexpr (kNoted && !small_pages(SRC)) c = static_cast<int>(fresh_lane()) % 32;  // (kept over the loop, beside the notes, it spills)
+  using E = Type<F16 && !four_bits(SRC)>;
+  typedef typename E::vec evec;
   float check = 0.f;  // no finite number if one of them is none
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) check = fmaf(acc[d][r], 0.f, check);
-  if (__builtin_amdgcn_ballot_w64(check != 0.f) != 0 && (SRC == kPacked || a.num_blocks > 0)) {
+  bool again = __builtin_amdgcn_ballot_w64(check != 0.f) != 0;
+  if constexpr (kNoted) {  // (a tile's keys are of all waves)
+    auto word = [&](int w) { return reinterpret_cast<uint32_t*>(share + kRaw + w * 1024); };  // among the wave's own bytes
+    *word(wave) = noted;
+    barrier();
+    again = again || uniform_int(*word(0) | *word(1) | *word(2) | *word(3)) != 0;
+  }
+  if (again && (SRC == kPacked || a.num_blocks > 0)) {
     reset();
     // eight dims of a 4-bit row, and one
     auto exponent_row = [&](bool isv, int key) {
@@ -1017,29 +1046,54 @@ attention16_kernel(const AttnArgs a) {
     for (int t = t0; t < tw; ++t) {
       const int key0 = t * kKeys;
       floatx16 sc[2];
-      u32x4 pa[4];
-      float ps;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const uint8_t* row = key_row(k_head, a.k_sn * 2, k_st, key0 + 32 * b + c);
         if constexpr (four_bits(SRC)) {
           const uint8_t* exponents = exponent_row(false, key0 + 32 * b + c);
 #pragma unroll
-          for (int x = 0; x < kSteps; ++x)
-            scores_step(x, widen8<F16>(*reinterpret_cast<const uint32_t*>(row + 8 * x + 4 * g), e8m0_value(exponents[x / 2])), sc[b]);
+          for (int x = 0; x < kSteps; ++x) {
+            const u32x4 k = widen8<false>(*reinterpret_cast<const uint32_t*>(row + 8 * x + 4 * g), e8m0_value(exponents[x / 2]));
+            if constexpr (!F16) {
+              scores_step(x, k, sc[b]);
+            } else {
+              if (x == 0)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[b][r] = 0.f;
+              u32x4 whole = __builtin_bit_cast(u32x4, qop[x]), q[2];
+              asm volatile("" : "+v"(whole));  // (kept over the tiles, the terms spill)
+              split_float16(whole, 1.f, q[0], q[1]);
+#pragma unroll
+              for (int term = 0; term < 2; ++term) sc[b] = E::mfma(__builtin_bit_cast(evec, k), __builtin_bit_cast(evec, q[term]), sc[b]);
+            }
+          }
         } else {
 #pragma unroll
           for (int x = 0; x < kSteps; ++x) scores_step(x, *reinterpret_cast<const u32x4*>(row + 16 * g + 32 * x), sc[b]);
         }
       }
       mask(key0, sc);
-      settle(sc, pa, ps);
-      l_run += ps;
+      const float m_use = rise(sc, E::kShift);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          sc[b][r] = __builtin_amdgcn_exp2f(fmaf(sc[b][r], scale, -m_use));
+          l_run += sc[b][r];
+        }
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
+        constexpr int kTerms = kNoted ? 2 : 1;
+        u32x4 pw[kTerms];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float lo = sc[m / 2][m % 2 * 8 + 2 * j], up = sc[m / 2][m % 2 * 8 + 2 * j + 1];
+          pw[0][j] = pack<F16 && !four_bits(SRC)>(lo, up);
+          if constexpr (kNoted) pw[1][j] = pack_bf16(lo - __uint_as_float(pw[0][j] << 16), up - __uint_as_float(pw[0][j] & 0xFFFF0000u));
+        }
         const uint8_t *row[8], *exponents[8];
         u32x4 seen;  // 1 where the lane's row sees the key of the slot
-        constexpr uint32_t kOne = F16 ? 0x3C00u : 0x3F80u;
+        constexpr uint32_t kOne = F16 && !four_bits(SRC) ? 0x3C00u : 0x3F80u;
         const int first = key0 + 16 * m + 4 * g;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -1056,19 +1110,20 @@ attention16_kernel(const AttnArgs a) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             if constexpr (four_bits(SRC))
-              value[j] = widen8<F16>(row[j][16 * n + c / 2] >> (c % 2 * 4), e8m0_value(exponents[j][n]))[0] & 0xFFFFu;
+              value[j] = widen8<false>(row[j][16 * n + c / 2] >> (c % 2 * 4), e8m0_value(exponents[j][n]))[0] & 0xFFFFu;
             else
               value[j] = *reinterpret_cast<const uint16_t*>(row[j] + 2 * c + 64 * n);
-            const uint32_t finite = (value[j] & T::kInf) == T::kInf ? 0u : value[j];
+            const uint32_t finite = (value[j] & E::kInf) == E::kInf ? 0u : value[j];
             clean[j / 2] = j % 2 ? clean[j / 2] | (finite << 16) : finite;
           }
-          output_step(m * kDims + n, clean, pa);
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) acc[n] = E::mfma(__builtin_bit_cast(evec, clean), __builtin_bit_cast(evec, pw[term]), acc[n]);
 #pragma unroll 1
           for (int kind = 0; kind < 3; ++kind) {  // infinities of either sign, NaN: how many of them a row sees
             u32x4 is;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const bool hit = kind == 2 ? (value[j] & 0x7FFFu) > T::kInf : value[j] == (T::kInf | (kind == 1 ? 0x8000u : 0u));
+              const bool hit = kind == 2 ? (value[j] & 0x7FFFu) > E::kInf : value[j] == (E::kInf | (kind == 1 ? 0x8000u : 0u));
               const uint32_t bit = hit ? kOne : 0u;
               is[j / 2] = j % 2 ? is[j / 2] | (bit << 16) : bit;
             }
@@ -1076,7 +1131,7 @@ attention16_kernel(const AttnArgs a) {
             floatx16 count;
 #pragma unroll
             for (int r = 0; r < 16; ++r) count[r] = 0.f;
-            count = T::mfma(__builtin_bit_cast(vec, is), __builtin_bit_cast(vec, seen), count);
+            count = E::mfma(__builtin_bit_cast(evec, is), __builtin_bit_cast(evec, seen), count);
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[n][r] = count[r] > 0.f ? acc[n][r] + what : acc[n][r];
           }

@@ -52,6 +52,24 @@ __device__ __forceinline__ uint32_t fp4_quantize8(const float (&x)[8], uint32_t&
   return fp4_encode8(x, exponent);
 }
 
+// Two fp32 values -> two bf16 ones, to nearest even.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float up) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, up}, bf16x2));
+}
+
+// Eight float16 queries times a power of two -> the sum of two bf16 numbers, exact (11
+// bits are in 8 and 3), to meet bf16 keys, which hold every code times every power of
+// two.  Infinities and NaN are the first's alone.
+__device__ __forceinline__ void split_float16(const u32x4& q, float unit, u32x4& first, u32x4& second) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float lo = f16_bits_to_f32(q[j] & 0xFFFFu) * unit, up = f16_bits_to_f32(q[j] >> 16) * unit;
+    first[j] = pack_bf16(lo, up);
+    second[j] = pack_bf16(fabsf(lo) < INFINITY ? lo - __uint_as_float(first[j] << 16) : 0.f,
+                          fabsf(up) < INFINITY ? up - __uint_as_float(first[j] & 0xFFFF0000u) : 0.f);
+  }
+}
+
 // Eight codes times a scale.
 __device__ __forceinline__ void fp4_decode8(uint32_t w, float scale, float (&x)[8]) {
   const floatx2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);

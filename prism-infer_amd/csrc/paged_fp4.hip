@@ -124,11 +124,6 @@ __device__ __forceinline__ void wave_lds_order() {
 // A sequence's keys.
 __device__ __forceinline__ int keys_of(const Fp4Args& a, int i) { return min(max(min(a.ctx[i], *a.max_ctx), 0), a.room); }
 
-// Two fp32 values -> two bf16 ones, to nearest even.
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float up) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, up}, bf16x2));
-}
-
 template <bool F16>
 __device__ __forceinline__ uint32_t pack_out(float lo, float up) {
   if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, up}, f16x2));
@@ -154,19 +149,6 @@ __device__ __forceinline__ uint32_t off_float16(uint32_t w) {
   const uint32_t above = (low + 0x6F6F6F6Fu) & w;                                // 145 to 255
   const uint32_t below = (low + 0x7E7E7E7Eu) & ~(low + 0x14141414u) & ~w;        // 2 to 107
   return (above | below) & 0x80808080u;
-}
-
-// Eight float16 values times 2^-4 -> the sum of two bf16 ones, exact (11 bits are in 8
-// and 3; infinities and NaN are the first's alone).
-__device__ __forceinline__ void split_queries(const u32x4& q, u32x4& first, u32x4& second) {
-  constexpr float unit = 1.0f / (1u << kKeyShift);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float lo = f16_bits_to_f32(q[j] & 0xFFFFu) * unit, up = f16_bits_to_f32(q[j] >> 16) * unit;
-    first[j] = pack_bf16(lo, up);
-    second[j] = pack_bf16(fabsf(lo) < INFINITY ? lo - __uint_as_float(first[j] << 16) : 0.f,
-                          fabsf(up) < INFINITY ? up - __uint_as_float(first[j] & 0xFFFF0000u) : 0.f);
-  }
 }
 
 // ... times 2^(e - 127) of an exponent byte, as the scores' operand.
@@ -480,7 +462,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
             for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<const uint32_t*>(stage + k_rd + 16 * x * kRow + 4 * y);
             u32x4 whole = qop[y], q[2];
             asm volatile("" : "+v"(whole));  // (split where it is used: kept, the terms spill)
-            split_queries(whole, q[0], q[1]);
+            split_float16(whole, 1.0f / (1u << kKeyShift), q[0], q[1]);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const u32x4 k = widen_key<false>(w[x], ke[x]);

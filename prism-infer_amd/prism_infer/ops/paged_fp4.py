@@ -6,8 +6,7 @@ No counterpart in the reference.  The payloads are ``torch.float4_e2m1fn_x2``
 bf16 or fp16, head_dim 64 or 128, any GQA group, pages of a multiple of 16 tokens.
 Scores are exact products of queries and stored keys, summed in fp32.  Softmax
 weights are rounded to the queries' type against fp32 sums (in decode after the values'
-exponents are multiplied in, and for fp16 queries to 16 bits).  With fp16 queries stored
-numbers count as infinite from 65520 on in chunks.
+exponents are multiplied in, and for fp16 queries to 16 bits).
 """
 
 from __future__ import annotations
