@@ -1011,17 +1011,19 @@ attention16_kernel(const AttnArgs a) {
   // 0.  A wave with an output that is not finite walks its tiles once more, one
   // thing after the other and straight from memory (the others may be done):
   // such values are taken out of the product and added to the rows that see
-  // their key.  So do waves of float16 queries whose 4-bit keys or values are no
-  // float16 numbers: as bf16, with the queries and weights in two terms.
+  // their key.  So do waves whose values may leave fp32 in sums (2^64 and more),
+  // with smaller weights, and those of float16 queries whose 4-bit keys or values
+  // are no float16 numbers: as bf16, with the queries and weights in two terms.
   if constexpr (kNoted && !small_pages(SRC)) c = static_cast<int>(fresh_lane()) % 32;  // (kept over the loop, beside the notes, it spills)
   using E = Type<F16 && !four_bits(SRC)>;
   typedef typename E::vec evec;
-  float check = 0.f;  // no finite number if one of them is none
+  constexpr float kLeast = F16 && !four_bits(SRC) ? T::kShift : -24.f;  // (values of 2^128: 2^24 keys)
+  float check = 0.f;  // no finite number if one of them is none, or large
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) check = fmaf(acc[d][r], 0.f, check);
-  bool again = __builtin_amdgcn_ballot_w64(check != 0.f) != 0;
+    for (int r = 0; r < 16; ++r) check = fmaf(acc[d][r], acc[d][r], check);
+  bool again = __builtin_amdgcn_ballot_w64(!(check < INFINITY)) != 0;
   if constexpr (kNoted) {  // (a tile's keys are of all waves)
     auto word = [&](int w) { return reinterpret_cast<uint32_t*>(share + kRaw + w * 1024); };  // among the wave's own bytes
     *word(wave) = noted;
@@ -1073,7 +1075,7 @@ attention16_kernel(const AttnArgs a) {
         }
       }
       mask(key0, sc);
-      const float m_use = rise(sc, E::kShift);
+      const float m_use = rise(sc, kLeast);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
