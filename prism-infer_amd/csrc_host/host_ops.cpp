@@ -27,6 +27,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "prism_kv.h"
 
@@ -43,13 +44,24 @@ const at::Tensor* tensor(PyObject* o) {
   return t.defined() && t.has_storage() && t.layout() == at::kStrided ? &t : nullptr;
 }
 
+// The types of 4-bit caches, where torch has them (2.8 on); else no tensor's.
+template <typename T, typename = void>
+struct Fp4Types {
+  static constexpr T payload = T::Undefined, scale = T::Undefined;
+};
+template <typename T>
+struct Fp4Types<T, std::void_t<decltype(T::Float4_e2m1fn_x2), decltype(T::Float8_e8m0fnu)>> {
+  static constexpr T payload = T::Float4_e2m1fn_x2, scale = T::Float8_e8m0fnu;
+};
+constexpr at::ScalarType kFp4 = Fp4Types<at::ScalarType>::payload, kFp4Scale = Fp4Types<at::ScalarType>::scale;
+
 int dtype_code(at::ScalarType t) {
   switch (t) {
     case at::kFloat: return PRISM_DTYPE_F32;
     case at::kBFloat16: return PRISM_DTYPE_BF16;
     case at::kHalf: return PRISM_DTYPE_F16;
     case at::kFloat8_e4m3fn: return PRISM_DTYPE_FP8_E4M3FN;
-    case at::kFloat4_e2m1fn_x2: return PRISM_DTYPE_FP4_E2M1;
+    case kFp4: return PRISM_DTYPE_FP4_E2M1;
     default: return -1;
   }
 }
@@ -75,10 +87,10 @@ bool scale_pair(const at::Tensor& cache, const at::Tensor* ks, const at::Tensor*
 
 // The exponents of a 4-bit cache: one per 32 dims (16 payload bytes).
 bool fp4_scale_pair(const at::Tensor& cache, const at::Tensor* ks, const at::Tensor* vs) {
-  if (!ks || !vs || cache.scalar_type() != at::kFloat4_e2m1fn_x2 || cache.dim() < 3 || cache.size(-1) <= 0 || cache.size(-1) % 16 != 0)
+  if (!ks || !vs || cache.scalar_type() != kFp4 || cache.dim() < 3 || cache.size(-1) <= 0 || cache.size(-1) % 16 != 0)
     return false;
   for (const at::Tensor* t : {ks, vs}) {
-    if (t->scalar_type() != at::kFloat8_e8m0fnu || t->dim() != cache.dim() || t->size(-1) != cache.size(-1) / 16) return false;
+    if (t->scalar_type() != kFp4Scale || t->dim() != cache.dim() || t->size(-1) != cache.size(-1) / 16) return false;
     for (int64_t i = 0; i + 1 < cache.dim(); ++i)
       if (t->size(i) != cache.size(i)) return false;
   }
@@ -145,7 +157,7 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t n) {
       kc->sizes() != vc->sizes() || kc->scalar_type() != vc->scalar_type())
     Py_RETURN_NONE;
   const int64_t tokens = key->size(0), heads = key->size(1), dim = key->size(2);
-  const bool four = kc->scalar_type() == at::kFloat4_e2m1fn_x2;
+  const bool four = kc->scalar_type() == kFp4;
   if (tokens <= 0 || heads <= 0 || dim <= 0 || heads > INT32_MAX || dim > INT32_MAX || kc->size(-2) != heads ||
       kc->size(-1) * (four ? 2 : 1) != dim || slots->dim() != 1 || slots->numel() != tokens || slots->scalar_type() != at::kInt ||
       !slots->is_contiguous() || !(four ? fp4_scale_pair(*kc, ks, vs) : scale_pair(*kc, ks, vs)))
@@ -230,7 +242,7 @@ PyObject* rotate_store(PyObject*, PyObject* const* args, Py_ssize_t n) {
       kc->sizes() != vc->sizes() || kc->scalar_type() != vc->scalar_type() || table->dim() != 2 || slots->dim() != 1)
     Py_RETURN_NONE;
   const int64_t tokens = key->size(0), heads = key->size(1), dim = key->size(2), q_heads = q->size(1), rotary = table->size(1);
-  const bool four = kc->scalar_type() == at::kFloat4_e2m1fn_x2;
+  const bool four = kc->scalar_type() == kFp4;
   const int in = dtype_code(q->scalar_type()), out = dtype_code(kc->scalar_type());
   if (tokens <= 0 || heads <= 0 || dim <= 0 || q_heads <= 0 || q_heads > INT32_MAX || heads > INT32_MAX || dim > INT32_MAX ||
       q->size(0) != tokens || q->size(2) != dim || kc->size(-2) != heads || kc->size(-1) * (four ? 2 : 1) != dim ||
@@ -278,7 +290,7 @@ PyObject* load(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!on_current_device(device, kc, vc, slots, ks, vs) || (kc->dim() != 3 && kc->dim() != 4) || kc->sizes() != vc->sizes() ||
       kc->scalar_type() != vc->scalar_type() || !int32_vector(*slots) || (to < 0 || !plain_dtype(static_cast<int>(to))))
     Py_RETURN_NONE;
-  const bool four = kc->scalar_type() == at::kFloat4_e2m1fn_x2;
+  const bool four = kc->scalar_type() == kFp4;
   const int from = dtype_code(kc->scalar_type());
   const int64_t tokens = slots->numel(), heads = kc->size(-2), row = kc->size(-1), dim = four ? 2 * row : row;
   if (from < 0 || !(four ? fp4_scale_pair(*kc, ks, vs) : scale_pair(*kc, ks, vs)) || tokens <= 0 || heads <= 0 || row <= 0 ||
@@ -441,7 +453,7 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   DecodeCall d;
   if (n != 11) Py_RETURN_NONE;
-  if (const at::Tensor* kc = tensor(args[1]); kc && kc->scalar_type() == at::kFloat4_e2m1fn_x2) return decode_fp4(args);
+  if (const at::Tensor* kc = tensor(args[1]); kc && kc->scalar_type() == kFp4) return decode_fp4(args);
   if (!check_decode(args, d)) Py_RETURN_NONE;
   at::Tensor out;
   int rc;
@@ -567,7 +579,7 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const double scale = PyFloat_AS_DOUBLE(args[8]);
   int device;
   if (over1 || over2 || !on_current_device(device, q, kc, vc, bt, ctx, cu, ks, vs) || capturing()) Py_RETURN_NONE;
-  if (kc->scalar_type() == at::kFloat4_e2m1fn_x2) return prefill_fp4(q, kc, vc, ks, vs, bt, ctx, cu, heads, kv_heads, scale, args[11]);
+  if (kc->scalar_type() == kFp4) return prefill_fp4(q, kc, vc, ks, vs, bt, ctx, cu, heads, kv_heads, scale, args[11]);
   if (q->dim() != 3 || kc->dim() != 4 || kc->sizes() != vc->sizes() || bt->dim() != 2 ||
       (kc->scalar_type() != at::kFloat8_e4m3fn && kc->scalar_type() != q->scalar_type()) ||
       vc->scalar_type() != kc->scalar_type() || !scale_pair(*kc, ks, vs) ||

@@ -39,8 +39,9 @@ KV_COMPONENT_COUNT = 2
 
 _SCALE_ITEMSIZE = 4  # bytes of one KV_SCALE_DTYPE element
 
-FP4_DTYPE = torch.float4_e2m1fn_x2
-FP4_SCALE_DTYPE = torch.float8_e8m0fnu
+# None where torch does not have them (before 2.8): no tensor is 4-bit there
+FP4_DTYPE = getattr(torch, "float4_e2m1fn_x2", None)
+FP4_SCALE_DTYPE = getattr(torch, "float8_e8m0fnu", None)
 FP4_SCALE_BLOCK = 32  # dims that share an exponent
 FP4_MOST = 7.0        # of a block, in units of its power of two (6 is the largest value)
 FP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)  # by code; 8 more for the sign
