@@ -370,13 +370,26 @@ int launch_passes(RotateArgs& a, hipStream_t stream) {
   const int passes = static_cast<int>(ceil_div(a.q_heads + 2 * a.heads, 64 / LANES));
   a.waves_per_token = static_cast<int>(ceil_div(passes, PASSES));
   a.by_waves = divisor(a.waves_per_token);
-  const int64_t waves = a.tokens * a.waves_per_token;
-  if (waves * 64 > UINT32_MAX - 255) {
-    set_error("prism_kv_rotate_store: too many rows for one launch");
+  // A launch holds 2^32 threads; beyond that the tokens are of several.
+  const int64_t most = (UINT32_MAX - 255) / 64 / a.waves_per_token, row = LANES * (IN == PRISM_DTYPE_F32 ? 32 : 16);
+  if (most == 0) {
+    set_error("prism_kv_rotate_store: too many heads for one launch");
     return PRISM_ERR_INVALID;
   }
-  hipLaunchKernelGGL((rotate_store_kernel<IN, LANES, PASSES>), dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0, stream, a);
-  return check_launch("rotate_store_kernel launch");
+  for (int64_t left = a.tokens; left > 0;) {
+    a.tokens = std::min(left, most);
+    const int64_t waves = a.tokens * a.waves_per_token;
+    hipLaunchKernelGGL((rotate_store_kernel<IN, LANES, PASSES>), dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0, stream, a);
+    if (int rc = check_launch("rotate_store_kernel launch")) return rc;
+    left -= a.tokens;
+    if (left == 0) break;
+    a.q += a.tokens * a.q_st, a.k += a.tokens * a.k_st, a.v += a.tokens * a.v_st;
+    if (a.positions != nullptr) a.positions += a.tokens;
+    if (a.q_out != nullptr) a.q_out += a.tokens * a.q_heads * row;
+    if (a.k_out != nullptr) a.k_out += a.tokens * a.heads * row;
+    a.slots += a.tokens;
+  }
+  return PRISM_OK;
 }
 
 // A wave's passes share a token's cosines and sines: as many as leave the chip 16
