@@ -1309,7 +1309,7 @@ int launch(const AttnArgs& a, hipStream_t stream) {
   const int64_t checks = SRC != kPacked && a.report != nullptr ? a.kv_heads : 0;
   const int64_t grid = checks + (a.work == nullptr ? blocks : std::max<int64_t>(blocks, a.slots + a.kv_heads));  // (parts never outnumber the slots)
   if (rows > kMostRows || grid * 64 * kWaves * GROUPS > UINT32_MAX) {
-    set_error("attention over 16-bit keys: too many query rows for one launch");
+    set_error("%s: too many query rows for one launch", a.four ? "prism_paged_fp4" : "attention over 16-bit keys");
     return PRISM_ERR_INVALID;
   }
   hipLaunchKernelGGL((attention16_kernel<F16, D, SRC, GROUPS>), dim3(static_cast<unsigned>(grid)), dim3(64 * kWaves * GROUPS), 0,
