@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_e
   constexpr int kShare = (kStage > kJoin ? kStage : kJoin) + 64;  // (heads' rows a quarter of the banks apart)
   static_assert(kShare % 256 == 64, "rows of four heads meet different banks");
   __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * kShare];
-  __shared__ int absent[kWaves * 4];  // by 16 keys of a step: 1 where they have no block
+  __shared__ __attribute__((aligned(16))) int absent[kWaves * 4];  // by 16 keys of a step: 1 where they have no block (read four at a time)
 
   const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
   const int wave = uniform_int(threadIdx.x / 64);
