@@ -1,6 +1,6 @@
-// What the kernels over chunks of a paged cache have in common: the sequences'
-// validity, reported to the host, and the rows outside every sequence.  `Args` has
-// the fields of the launch's arguments that are named here.
+// What the kernel over chunks of a paged cache does beside its attention: the
+// sequences' validity, reported to the host, and the rows outside every sequence.
+// `Args` has the fields of the launch's arguments that are named here.
 #pragma once
 
 #include "common.h"

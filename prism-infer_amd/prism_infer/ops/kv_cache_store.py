@@ -27,6 +27,7 @@ import torch
 from prism_infer import _native, observability
 from prism_infer.engine.kv_quantization import (
     FP4_DTYPE,
+    FP4_MOST,
     FP4_SCALE_BLOCK,
     FP4_SCALE_DTYPE,
     FP4_VALUES,
@@ -206,7 +207,7 @@ def _quantize_rows_fp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     amax = blocks.abs().amax(-1)
     good = torch.isfinite(amax)
     mantissa, exponent = torch.frexp(torch.where(good, amax, 0.0))  # the mantissa is in [0.5, 1)
-    exponent = torch.where(amax > 0, torch.where(mantissa > 0.875, exponent - 2, exponent - 3), -126).clamp(min=-126)
+    exponent = torch.where(amax > 0, torch.where(mantissa > FP4_MOST / 8, exponent - 2, exponent - 3), -126).clamp(min=-126)
     units = torch.ldexp(torch.where(good[..., None], blocks, 0.0), -exponent[..., None])
     steps = torch.tensor([(a + b) / 2 for a, b in zip(FP4_VALUES, FP4_VALUES[1:])], dtype=torch.float64)
     size = units.abs()
