@@ -415,7 +415,6 @@ attention16_kernel(const AttnArgs a) {
   constexpr int kLoads = kKeys / kLoadRows / kWaves;
   constexpr int kV = 2 * kPayload;            // two stages of K, then two of V
   constexpr int kShare = 4 * kPayload + 2 * kCols * kRow;  // of a group, with the last two waves' queries
-  constexpr bool kNoted = F16 && four_bits(SRC);  // whether a wave has keys that are no float16 numbers
   __shared__ __attribute__((aligned(256))) uint8_t lds[GROUPS * kShare];
 
   // With a report the first workgroups (one per kv head, which keeps the others'
@@ -451,7 +450,7 @@ attention16_kernel(const AttnArgs a) {
   const int wave = uniform_int(tid / 64);
   const int group = GROUPS == 1 ? 0 : uniform_int(threadIdx.x / (64 * kWaves));
   const int lane = tid % 64;
-  int c = lane % 32;
+  const int c = lane % 32;
   const int g = lane / 32;
 
   const Seq s = work.s;
@@ -619,20 +618,17 @@ attention16_kernel(const AttnArgs a) {
     f.w = *reinterpret_cast<const u32x4*>(bytes);
     f.e = *exponent;
   };
-  auto put = [&](const Fours& f, uint32_t to, uint32_t stage) __attribute__((always_inline)) {
-    const float e = f.e == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(f.e << 23);
+  // Keys with exponents of which float16 does not hold all codes become NaN, and the rows
+  // that see one are taken anew below.  (0.5 * 2^(104 - 127) is its smallest number, 6 *
+  // 2^(140 - 127) ends below its largest; of 0 and 1, which blocks of zeros have, it makes
+  // 0, as their scores are to 2^-100.  Of values it loses at most 2^-25, or makes an
+  // infinity, which is as good.)
+  auto put = [&](const Fours& f, bool isv, uint32_t to, uint32_t stage) __attribute__((always_inline)) {
+    const bool off = F16 && !isv ? f.e - 104u > 36u && f.e > 1u : f.e == 255u;
+    const float e = off ? __uint_as_float(0x7FC00000u) : __uint_as_float(f.e << 23);
     const uint32_t at = to + stage + (D == 128 ? 16 * wave : 32 * (wave % 2)) * kRow;
 #pragma unroll
     for (int x = 0; x < 4; ++x) *reinterpret_cast<u32x4*>(share + (at ^ (x << 4))) = widen8<F16>(f.w[x], e);
-  };
-  // The wave's keys of tile t: whether there are exponents of which float16 does not hold
-  // all codes.  (0.5 * 2^(104 - 127) is its smallest number, 6 * 2^(140 - 127) ends below
-  // its largest; of 0 and 1, which blocks of zeros have, it makes 0, as their scores are
-  // to 2^-100.  Behind the last key there may be anything.)
-  uint32_t noted = 0;
-  auto note = [&](const Fours& f, int t) __attribute__((always_inline)) {
-    if (t * kKeys + (D == 128 ? 16 * wave : 32 * (wave % 2)) < kend)
-      noted |= __builtin_amdgcn_ballot_w64(f.e - 104u > 36u && f.e > 1u) != 0;
   };
   uint32_t exp4 = 0;  // 64 dims; with 128 a key's four come to LDS behind the bytes, by lanes' rows
   auto fetch_raw = [&](const Place& place, bool isv, const u32x4& from) __attribute__((always_inline)) {
@@ -646,12 +642,10 @@ attention16_kernel(const AttnArgs a) {
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                    : : "v"(exponent), "s"(uniform_int(raw + 4096u + static_cast<uint32_t>(wave) * 256u)) : "memory", "m0");
   };
-  auto put_raw = [&](int t, bool isv, uint32_t stage, const u32x2& to) __attribute__((always_inline)) {
+  auto put_raw = [&](bool isv, uint32_t stage, const u32x2& to) __attribute__((always_inline)) {
     if (D == 64 && isv != values4) return;
     const uint8_t* raw = share + kRaw + (D == 128 && isv ? kHalf : 0u);
-    const Fours f{*reinterpret_cast<const u32x4*>(raw + wave * 1024 + fresh_lane() * 16), D == 64 ? exp4 : raw[wave * 256 + to[1]]};
-    if (kNoted && !isv) note(f, t);
-    put(f, to[0], stage);
+    put(Fours{*reinterpret_cast<const u32x4*>(raw + wave * 1024 + fresh_lane() * 16), D == 64 ? exp4 : raw[wave * 256 + to[1]]}, isv, to[0], stage);
   };
   auto issue = [&](int t, const Place& place, bool isv, uint32_t stage) {
     if (!place.ok) return;
@@ -834,11 +828,10 @@ attention16_kernel(const AttnArgs a) {
   reset();
   {
     uint32_t k_next = kPayload, v_prev = kV;  // stages of K of tile t + 1 and V of tile t - 1
-    if (kNoted && (D == 128 || !values4)) note(first[0], t0), note(first[2], t0 + 1);
     if constexpr (four_bits(SRC)) {
-      if (D == 128 || !values4) put(first[0], kept.to[0], 0);
-      if (D == 128 || values4) put(first[1], kept.to[0], kV + kPayload);
-      if (D == 128 || !values4) put(first[2], kept.to[0], kPayload);
+      if (D == 128 || !values4) put(first[0], false, kept.to[0], 0);
+      if (D == 128 || values4) put(first[1], true, kept.to[0], kV + kPayload);
+      if (D == 128 || !values4) put(first[2], false, kept.to[0], kPayload);
     }
     landed();
     barrier();
@@ -942,8 +935,8 @@ attention16_kernel(const AttnArgs a) {
       landed();
       if constexpr (four_bits(SRC)) {  // (their stages' last readers are past the barrier before)
         const u32x2 to = to4();
-        if (t > t0 && t + 1 < t1) put_raw(t + 1, false, k_next, to);
-        if (t > t0 + 1 && t - 1 < t1) put_raw(t - 1, true, v_prev, to);
+        if (t > t0 && t + 1 < t1) put_raw(false, k_next, to);
+        if (t > t0 + 1 && t - 1 < t1) put_raw(true, v_prev, to);
       }
       barrier();
       if constexpr (four_bits(SRC)) {
@@ -1014,7 +1007,6 @@ attention16_kernel(const AttnArgs a) {
   // their key.  So do waves whose values may leave fp32 in sums (2^64 and more),
   // with smaller weights, and those of float16 queries whose 4-bit keys or values
   // are no float16 numbers: as bf16, with the queries and weights in two terms.
-  if constexpr (kNoted && !small_pages(SRC)) c = static_cast<int>(fresh_lane()) % 32;  // (kept over the loop, beside the notes, it spills)
   using E = Type<F16 && !four_bits(SRC)>;
   typedef typename E::vec evec;
   constexpr float kLeast = F16 && !four_bits(SRC) ? T::kShift : -24.f;  // (values of 2^128: 2^24 keys)
@@ -1023,14 +1015,7 @@ attention16_kernel(const AttnArgs a) {
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) check = fmaf(acc[d][r], acc[d][r], check);
-  bool again = __builtin_amdgcn_ballot_w64(!(check < INFINITY)) != 0;
-  if constexpr (kNoted) {  // (a tile's keys are of all waves)
-    auto word = [&](int w) { return reinterpret_cast<uint32_t*>(share + kRaw + w * 1024); };  // among the wave's own bytes
-    *word(wave) = noted;
-    barrier();
-    again = again || uniform_int(*word(0) | *word(1) | *word(2) | *word(3)) != 0;
-  }
-  if (again && (SRC == kPacked || a.num_blocks > 0)) {
+  if (__builtin_amdgcn_ballot_w64(!(check < INFINITY)) != 0 && (SRC == kPacked || a.num_blocks > 0)) {
     reset();
     // eight dims of a 4-bit row, and one
     auto exponent_row = [&](bool isv, int key) {
@@ -1085,13 +1070,13 @@ attention16_kernel(const AttnArgs a) {
         }
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        constexpr int kTerms = kNoted ? 2 : 1;
+        constexpr int kTerms = F16 && four_bits(SRC) ? 2 : 1;
         u32x4 pw[kTerms];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float lo = sc[m / 2][m % 2 * 8 + 2 * j], up = sc[m / 2][m % 2 * 8 + 2 * j + 1];
           pw[0][j] = pack<F16 && !four_bits(SRC)>(lo, up);
-          if constexpr (kNoted) pw[1][j] = pack_bf16(lo - __uint_as_float(pw[0][j] << 16), up - __uint_as_float(pw[0][j] & 0xFFFF0000u));
+          if constexpr (kTerms == 2) pw[1][j] = pack_bf16(lo - __uint_as_float(pw[0][j] << 16), up - __uint_as_float(pw[0][j] & 0xFFFF0000u));
         }
         const uint8_t *row[8], *exponents[8];
         u32x4 seen;  // 1 where the lane's row sees the key of the slot
