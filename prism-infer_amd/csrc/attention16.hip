@@ -1004,7 +1004,7 @@ attention16_kernel(const AttnArgs a) {
   // 0.  A wave with an output that is not finite walks its tiles once more, one
   // thing after the other and straight from memory (the others may be done):
   // such values are taken out of the product and added to the rows that see
-  // their key.  So do waves whose values may leave fp32 in sums (2^64 and more),
+  // their key.  So do waves whose values may leave fp32 in sums (2^61 and more),
   // with smaller weights, and those of float16 queries whose 4-bit keys or values
   // are no float16 numbers: as bf16, with the queries and weights in two terms.
   using E = Type<F16 && !four_bits(SRC)>;
